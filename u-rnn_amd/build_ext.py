@@ -17,7 +17,10 @@ HEADERS = ["urnn_common.h", "urnn_kernels.h", "urnn_gemm.h", os.path.join("..", 
 # every ring slot poisoned with NaN until its DMA landed (no NaN ever appeared: the ring protocol was not the cause).  The same
 # sources without packed instructions: 0 of 8000 launches, 0 of 30 whole-event rollouts, and 1.5 % faster (tools/diag_dec1.py,
 # tools/stress_overlap.py; MI355X_MICROARCH.md prices the packed ops as an anti-lever beside MFMAs anyway).
-NO_PACKED_F32 = ("-fno-slp-vectorize", "-DURNN_NO_PACKED_F32=1")   # urnn_common.h refuses to compile without the define
+# The target feature is switched off as well, so that no other pass can make such an instruction (hipcc's host pass warns that it does not
+# know the feature: harmless).
+NO_PACKED_F32 = ("-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                 "-DURNN_NO_PACKED_F32=1")   # urnn_common.h refuses to compile without the define
 
 
 def _newest(paths):
@@ -30,8 +33,6 @@ def build(force=False, verbose=False, extra_flags=(), out=None, tag=""):
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     deps = srcs + [os.path.normpath(os.path.join(CSRC, h)) for h in HEADERS]
     LIB = out or globals()["LIB"]
-    if not force and not extra_flags and os.path.isfile(LIB) and os.path.getmtime(LIB) >= _newest(deps):
-        return LIB
     if extra_flags and (not out or not tag):
         raise ValueError("a build with extra flags needs its own library path (out=) and object tag (tag=): it must not replace the product library or its objects")
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
