@@ -429,6 +429,71 @@ int urnn_step_f32(const urnn_net_f32 *net, const float *x_t, float *const states
                   const int *frame_index, void *workspace, size_t workspace_bytes, int B, int H, int W, float cls_thred, float eps,
                   float slope, void *stream);
 
+/* ---- sequence operators: a state space block next to the recurrent cells ---------------------------------------------------
+ * Short causal convolution, selective state space scan and the norms around a block, over a whole time axis (prompts, training
+ * windows) or for one token.  The reference has no such layers.  They depart from the conventions above in two points:
+ *   - the activations' element type is an argument (URNN_F32 / URNN_BF16 / URNN_F16, one for all of a call's (B,L,*) tensors);
+ *     parameters, their gradients, scan states and workspaces are float32, and all arithmetic is fp32 with one rounding at a store;
+ *   - (B,L,C) inputs are channels-last with element strides for batch and token (channels adjacent), so that the parts of one
+ *     projection can be handed over in place; outputs are contiguous.
+ * lengths (B) int32 or NULL: sequence b counts its first lengths[b] tokens (clamped to [0, L]); later tokens are not read, their
+ * outputs and gradients are zeros.  Nothing is read or written outside the tensors whatever lengths hold.
+ * No atomics: the same inputs give the same bits.  In-place: only where stated. */
+#define URNN_F32 0
+#define URNN_BF16 1
+#define URNN_F16 2
+
+/* y[t] = act(bias + sum_k weight[:, k] line[t + k]), line = [state | x], act = SiLU (silu != 0) or identity; weight (D,K) with
+ * K = 2..4, bias (D) or NULL, state (B,K-1,D) or NULL (zeros): the inputs before the first token, oldest first.  state_out
+ * (B,K-1,D) or NULL: the last K-1 entries of each sequence's line; must not overlap state. */
+int urnn_causal_conv(const void *x, long x_batch, long x_token, const float *weight, const float *bias, const void *state,
+                     const int *lengths, void *y, void *state_out, int dtype, int B, int L, int D, int K, int silu, void *stream);
+/* One token: x, y (B,D), x with row stride x_batch; state_out may be state (in place). */
+int urnn_causal_conv_step(const void *x, long x_batch, const float *weight, const float *bias, const void *state, void *y,
+                          void *state_out, int dtype, int B, int D, int K, int silu, void *stream);
+/* Gradients of urnn_causal_conv given dout (B,L,D) and, where state_out was used further, dstate_out (B,K-1,D) or NULL.  dx (B,L,D);
+ * dstate (B,K-1,D) or NULL; dweight (D,K) and dbias (D, or NULL) float32, overwritten or added to (accumulate != 0). */
+size_t urnn_causal_conv_backward_workspace_bytes(int B, int L, int D, int K);
+int urnn_causal_conv_backward(const void *x, long x_batch, long x_token, const float *weight, const float *bias, const void *state,
+                              const int *lengths, const void *dout, long dout_batch, long dout_token, const void *dstate_out, void *dx,
+                              void *dstate, float *dweight, float *dbias, void *workspace, size_t workspace_bytes, int dtype, int B,
+                              int L, int D, int K, int silu, int accumulate, void *stream);
+
+/* step = softplus(delta + delta_bias) (softplus == 0: delta + delta_bias);  h_t = exp(step A) h_(t-1) + step u B_t;
+ * y = (C_t . h_t + skip u) * silu(z).   u, delta, z (B,L,D); B, C (B,L,G,N) with the D / G channels of a group sharing a row (groups
+ * and states adjacent); A (D,N), skip (D) or NULL, delta_bias (D) or NULL, z NULL: no gate; state (B,D,N) float32 or NULL (zeros);
+ * state_out (B,D,N) or NULL: each sequence's state after its last token; may not overlap state.  1 <= N <= 64, G divides D.
+ * strides: u, delta, B, C, z, each (batch, token).  keep != 0: the workspace is left as the record that the backward reads
+ * (urnn_selective_scan_workspace_bytes(..., keep)). */
+size_t urnn_selective_scan_workspace_bytes(int B, int L, int D, int N, int keep);
+int urnn_selective_scan(const void *u, const void *delta, const void *Bmat, const void *Cmat, const void *z, const long *strides,
+                        const float *A, const float *skip, const float *delta_bias, const float *state, const int *lengths, void *y,
+                        float *state_out, void *workspace, size_t workspace_bytes, int keep, int dtype, int B, int L, int D, int G,
+                        int N, int softplus, void *stream);
+/* One token: u, delta, z, y (B,D), B, C (B,G,N); strides: the batch strides of u, delta, B, C, z; state_out may be state. */
+int urnn_selective_scan_step(const void *u, const void *delta, const void *Bmat, const void *Cmat, const void *z, const long *strides,
+                             const float *A, const float *skip, const float *delta_bias, const float *state, void *y, float *state_out,
+                             int dtype, int B, int D, int G, int N, int softplus, void *stream);
+
+/* The norms around a block: per row of D channels (D <= 16384)
+ *   residual_out = residual + scale * act(gate) * post_w * y / rms(y),   normed = pre_w * residual_out / rms(residual_out),
+ * rms(x) = sqrt(mean(x^2) + eps).  post_w NULL: y enters as it is; gate / residual / scale NULL: left out; act: URNN_GATE_*.
+ * strides: row strides of y, gate, residual.  normed, residual_out (rows,D) contiguous, residual_out may be NULL; either may be y, gate or
+ * residual themselves where those are contiguous. */
+#define URNN_GATE_NONE 0
+#define URNN_GATE_SIGMOID 1
+#define URNN_GATE_SILU 2
+int urnn_norm_residual(const void *y, const void *gate, const void *residual, const long *strides, const float *pre_w,
+                       const float *post_w, const float *scale, void *normed, void *residual_out, int dtype, long rows, int D, int act,
+                       float eps, void *stream);
+/* Gradients, given dnormed and dresidual_out (either may be NULL: zeros).  strides: y, gate, residual, dnormed, dresidual_out.  dgate /
+ * dresidual may be NULL; dpre_w, dpost_w, dscale (D) float32, each may be NULL, overwritten or added to (accumulate != 0). */
+size_t urnn_norm_residual_backward_workspace_bytes(long rows, int D);
+int urnn_norm_residual_backward(const void *y, const void *gate, const void *residual, const void *dnormed, const void *dresidual_out,
+                                const long *strides, const float *pre_w, const float *post_w, const float *scale, void *dy, void *dgate,
+                                void *dresidual, float *dpre_w, float *dpost_w, float *dscale, void *workspace, size_t workspace_bytes,
+                                int dtype, long rows, int D, int act, float eps, int accumulate, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

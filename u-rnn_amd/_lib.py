@@ -12,7 +12,7 @@ LIB_PATH = os.environ.get("URNN_LIB") or os.path.join(_HERE, "liburnn_hip.so")  
 _lib = None
 
 c_float_p = ctypes.c_void_p  # raw device pointers (tensor.data_ptr())
-_i, _f, _p, _sz = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_i, _f, _p, _sz, _l = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_long
 
 # name -> (restype, argtypes); mirrors include/urnn_hip.h exactly
 SIGNATURES = {
@@ -75,6 +75,16 @@ SIGNATURES = {
     "urnn_step_workspace_bytes": (_sz, [_p, _i, _i, _i]),
     "urnn_step_workspace_init": (_i, [_p, _p, _sz, _i, _i, _i, _p, _p, _p]),
     "urnn_step_f32": (_i, [_p] * 8 + [_sz, _i, _i, _i, _f, _f, _f, _p]),
+    "urnn_causal_conv": (_i, [_p, _l, _l] + [_p] * 6 + [_i] * 6 + [_p]),
+    "urnn_causal_conv_step": (_i, [_p, _l] + [_p] * 5 + [_i] * 5 + [_p]),
+    "urnn_causal_conv_backward_workspace_bytes": (_sz, [_i] * 4),
+    "urnn_causal_conv_backward": (_i, [_p, _l, _l] + [_p] * 5 + [_l, _l] + [_p] * 6 + [_sz] + [_i] * 7 + [_p]),
+    "urnn_selective_scan_workspace_bytes": (_sz, [_i] * 5),
+    "urnn_selective_scan": (_i, [_p] * 14 + [_sz] + [_i] * 8 + [_p]),
+    "urnn_selective_scan_step": (_i, [_p] * 12 + [_i] * 6 + [_p]),
+    "urnn_norm_residual": (_i, [_p] * 9 + [_i, _l, _i, _i, _f, _p]),
+    "urnn_norm_residual_backward_workspace_bytes": (_sz, [_l, _i]),
+    "urnn_norm_residual_backward": (_i, [_p] * 16 + [_sz, _i, _l, _i, _i, _f, _i, _p]),
 }
 
 

@@ -2,6 +2,7 @@
 // kernel sequencing.  Enqueue-only: nothing here synchronises, allocates or keeps state besides the thread-local error text.
 #include "urnn_common.h"
 #include "urnn_kernels.h"
+#include "urnn_seq.h"
 #include "../../include/urnn_hip.h"
 
 #include <stdarg.h>
@@ -1523,5 +1524,224 @@ extern "C" int urnn_step_workspace_init(const urnn_net_f32 *net, void *workspace
     CHECK_HIP(urnn_train_zero(reinterpret_cast<float *>(ws.head), URNN_STATUS_BYTES / sizeof(float), (hipStream_t)stream), "zero the head status words");
     if (cell_status) *cell_status = reinterpret_cast<int *>(ws.cell);
     if (head_status) *head_status = reinterpret_cast<int *>(ws.head);
+    return URNN_OK;
+}
+
+// ---- sequence operators --------------------------------------------------------------------------------------------------
+static inline bool seq_type(int dtype) { return dtype == URNN_F32 || dtype == URNN_BF16 || dtype == URNN_F16; }
+static inline int seq_elem(int dtype) { return dtype == URNN_F32 ? 4 : 2; }
+// Rows start on 16 bytes: base and strides
+static inline bool wide_rows(const void *base, long s1, long s2, int elem)
+{
+    return !base || (aligned16(base) && s1 * elem % 16 == 0 && s2 * elem % 16 == 0);
+}
+
+static int conv_seq_args(const char *what, const void *x, const void *weight, int dtype, long B, long L, long D, int K)
+{
+    if (!x || !weight) return fail(URNN_ENULL, "%s: NULL argument", what);
+    if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
+    if (B < 1 || L < 1 || D < 1) return fail(URNN_EINVAL, "%s: B=%ld L=%ld D=%ld", what, B, L, D);
+    if (K < 2 || K > URNN_SEQ_MAX_TAPS) return fail(URNN_EINVAL, "%s: K=%d taps (2..%d)", what, K, URNN_SEQ_MAX_TAPS);
+    if ((double)B * D > 2147483648.0) return fail(URNN_EINVAL, "%s: B * D = %ld * %ld is beyond one launch", what, B, D);
+    return URNN_OK;
+}
+
+extern "C" int urnn_causal_conv(const void *x, long x_batch, long x_token, const float *weight, const float *bias, const void *state,
+                                const int *lengths, void *y, void *state_out, int dtype, int B, int L, int D, int K, int silu, void *stream)
+{
+    const int rc = conv_seq_args("urnn_causal_conv", x, weight, dtype, B, L, D, K);
+    if (rc) return rc;
+    if (!y) return fail(URNN_ENULL, "urnn_causal_conv: NULL argument");
+    if (state && state == state_out) return fail(URNN_EINVAL, "urnn_causal_conv: state_out must not be state (the step may run in place)");
+    ConvSeqParams p = {};
+    p.x = x; p.sx = {x_batch, x_token};
+    p.weight = weight; p.bias = bias; p.state = state; p.lengths = lengths; p.y = y; p.state_out = state_out;
+    p.batch = B; p.L = L; p.dim = D; p.K = K; p.silu = silu;
+    const int e = seq_elem(dtype);
+    const bool wide = wide_rows(x, x_batch, x_token, e) && (long)D * e % 16 == 0 && aligned16(y) && aligned16(weight) &&
+                      (!bias || aligned16(bias)) && (!state || aligned16(state)) && (!state_out || aligned16(state_out));
+    CHECK_HIP(urnn_launch_conv_seq(p, dtype, wide, (hipStream_t)stream), "causal_conv");
+    return URNN_OK;
+}
+
+extern "C" int urnn_causal_conv_step(const void *x, long x_batch, const float *weight, const float *bias, const void *state, void *y,
+                                     void *state_out, int dtype, int B, int D, int K, int silu, void *stream)
+{
+    const int rc = conv_seq_args("urnn_causal_conv_step", x, weight, dtype, B, 1, D, K);
+    if (rc) return rc;
+    if (!state || !y || !state_out) return fail(URNN_ENULL, "urnn_causal_conv_step: NULL argument");
+    ConvSeqParams p = {};
+    p.x = x; p.sx = {x_batch, 0};
+    p.weight = weight; p.bias = bias; p.state = state; p.y = y; p.state_out = state_out;
+    p.batch = B; p.L = 1; p.dim = D; p.K = K; p.silu = silu;
+    const int e = seq_elem(dtype);
+    const bool wide = wide_rows(x, x_batch, 0, e) && (long)D * e % 16 == 0 && aligned16(y) && aligned16(weight) && (!bias || aligned16(bias)) &&
+                      aligned16(state) && aligned16(state_out);
+    CHECK_HIP(urnn_launch_conv_seq_step(p, dtype, wide, (hipStream_t)stream), "causal_conv_step");
+    return URNN_OK;
+}
+
+extern "C" size_t urnn_causal_conv_backward_workspace_bytes(int B, int L, int D, int K)
+{
+    if (B < 1 || L < 1 || D < 1 || K < 2 || K > URNN_SEQ_MAX_TAPS) return 0;
+    return align_up((size_t)urnn_conv_seq_parts(B, L, D) * (K + 1) * D * sizeof(float), 256);
+}
+
+extern "C" int urnn_causal_conv_backward(const void *x, long x_batch, long x_token, const float *weight, const float *bias, const void *state,
+                                         const int *lengths, const void *dout, long dout_batch, long dout_token, const void *dstate_out,
+                                         void *dx, void *dstate, float *dweight, float *dbias, void *workspace, size_t workspace_bytes,
+                                         int dtype, int B, int L, int D, int K, int silu, int accumulate, void *stream)
+{
+    const int rc = conv_seq_args("urnn_causal_conv_backward", x, weight, dtype, B, L, D, K);
+    if (rc) return rc;
+    if (!dout || !dx || !dweight || !workspace) return fail(URNN_ENULL, "urnn_causal_conv_backward: NULL argument");
+    if (dx == dout || dx == x) return fail(URNN_EINVAL, "urnn_causal_conv_backward: dx must be a buffer of its own");
+    if (!aligned16(workspace)) return fail(URNN_EALIGN, "urnn_causal_conv_backward: workspace not 16-byte aligned");
+    if (workspace_bytes < urnn_causal_conv_backward_workspace_bytes(B, L, D, K)) return fail(URNN_EWORKSPACE, "urnn_causal_conv_backward: workspace too small");
+    ConvSeqParams p = {};
+    p.x = x; p.sx = {x_batch, x_token};
+    p.dout = dout; p.so = {dout_batch, dout_token};
+    p.weight = weight; p.bias = bias; p.state = state; p.lengths = lengths; p.dstate_out = dstate_out; p.dx = dx; p.dstate = dstate;
+    p.partial = reinterpret_cast<float *>(workspace);
+    p.batch = B; p.L = L; p.dim = D; p.K = K; p.silu = silu;
+    const int e = seq_elem(dtype);
+    const bool wide = wide_rows(x, x_batch, x_token, e) && wide_rows(dout, dout_batch, dout_token, e) && (long)D * e % 16 == 0 && aligned16(dx) &&
+                      aligned16(weight) && (!bias || aligned16(bias)) && (!state || aligned16(state)) && (!dstate || aligned16(dstate)) &&
+                      (!dstate_out || aligned16(dstate_out));
+    CHECK_HIP(urnn_launch_conv_seq_backward(p, dtype, wide, dweight, dbias, accumulate, (hipStream_t)stream), "causal_conv_backward");
+    return URNN_OK;
+}
+
+static int scan_args(const char *what, int dtype, long B, long L, long D, long G, long N)
+{
+    if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
+    if (B < 1 || L < 1 || D < 1) return fail(URNN_EINVAL, "%s: B=%ld L=%ld D=%ld", what, B, L, D);
+    if (G < 1 || D % G) return fail(URNN_EINVAL, "%s: G=%ld groups do not divide D=%ld channels", what, G, D);
+    if (N < 1 || N > URNN_SEQ_MAX_STATES) return fail(URNN_EINVAL, "%s: N=%ld states (1..%d)", what, N, URNN_SEQ_MAX_STATES);
+    const long cbs = G * ((D / G + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
+    if ((double)B * (cbs > D / 16 ? cbs : D / 16 + 1) > 8388608.0) return fail(URNN_EINVAL, "%s: B=%ld x D=%ld is beyond one launch", what, B, D);
+    return URNN_OK;
+}
+
+// Workspace: [checkpoints, if kept][sums of steps][chunk states]
+struct ScanWork { size_t keep, sum, S, total; };
+static ScanWork scan_work(int B, int L, int D, int N, int keep)
+{
+    int CL;
+    const size_t np = urnn_scan_np(N), chunks = urnn_scan_chunks(B, L, D, &CL), segs = (L + URNN_SCAN_CK - 1) / URNN_SCAN_CK;
+    ScanWork w;
+    w.keep = 0;
+    w.sum = keep ? align_up((size_t)B * segs * D * np * sizeof(float), 256) : 0;
+    w.S = w.sum + (chunks > 1 ? align_up((size_t)B * chunks * D * sizeof(float), 256) : 0);
+    w.total = w.S + (chunks > 1 ? align_up((size_t)B * chunks * D * np * sizeof(float), 256) : 0);
+    return w;
+}
+
+extern "C" size_t urnn_selective_scan_workspace_bytes(int B, int L, int D, int N, int keep)
+{
+    if (B < 1 || L < 1 || D < 1 || N < 1 || N > URNN_SEQ_MAX_STATES) return 0;
+    return scan_work(B, L, D, N, keep).total;
+}
+
+extern "C" int urnn_selective_scan(const void *u, const void *delta, const void *Bmat, const void *Cmat, const void *z, const long *strides,
+                                   const float *A, const float *skip, const float *delta_bias, const float *state, const int *lengths, void *y,
+                                   float *state_out, void *workspace, size_t workspace_bytes, int keep, int dtype, int B, int L, int D, int G,
+                                   int N, int softplus, void *stream)
+{
+    const int rc = scan_args("urnn_selective_scan", dtype, B, L, D, G, N);
+    if (rc) return rc;
+    if (!u || !delta || !Bmat || !Cmat || !strides || !A || !y) return fail(URNN_ENULL, "urnn_selective_scan: NULL argument");
+    if (state && state == state_out) return fail(URNN_EINVAL, "urnn_selective_scan: state_out must not be state (the step may run in place)");
+    const ScanWork w = scan_work(B, L, D, N, keep);
+    if (w.total && !workspace) return fail(URNN_ENULL, "urnn_selective_scan: NULL workspace");
+    if (!aligned16(workspace)) return fail(URNN_EALIGN, "urnn_selective_scan: workspace not 16-byte aligned");
+    if (workspace_bytes < w.total) return fail(URNN_EWORKSPACE, "urnn_selective_scan: workspace too small");
+    char *base = reinterpret_cast<char *>(workspace);
+    ScanParams p = {};
+    p.u = u; p.delta = delta; p.B = Bmat; p.C = Cmat; p.z = z;
+    p.su = {strides[0], strides[1]}; p.sd = {strides[2], strides[3]}; p.sB = {strides[4], strides[5]}; p.sC = {strides[6], strides[7]}; p.sz = {strides[8], strides[9]};
+    p.A = A; p.D = skip; p.bias = delta_bias; p.state = state; p.lengths = lengths; p.y = y; p.state_out = state_out;
+    p.keep = keep ? reinterpret_cast<float *>(base + w.keep) : nullptr;
+    p.sum = reinterpret_cast<float *>(base + w.sum);
+    p.S = reinterpret_cast<float *>(base + w.S);
+    p.batch = B; p.L = L; p.dim = D; p.N = N; p.G = G; p.softplus = softplus;
+    p.chunks = urnn_scan_chunks(B, L, D, &p.CL);
+    CHECK_HIP(urnn_launch_scan(p, dtype, (hipStream_t)stream), "selective_scan");
+    return URNN_OK;
+}
+
+extern "C" int urnn_selective_scan_step(const void *u, const void *delta, const void *Bmat, const void *Cmat, const void *z, const long *strides,
+                                        const float *A, const float *skip, const float *delta_bias, const float *state, void *y, float *state_out,
+                                        int dtype, int B, int D, int G, int N, int softplus, void *stream)
+{
+    const int rc = scan_args("urnn_selective_scan_step", dtype, B, 1, D, G, N);
+    if (rc) return rc;
+    if (!u || !delta || !Bmat || !Cmat || !strides || !A || !state || !y || !state_out) return fail(URNN_ENULL, "urnn_selective_scan_step: NULL argument");
+    ScanParams p = {};
+    p.u = u; p.delta = delta; p.B = Bmat; p.C = Cmat; p.z = z;
+    p.su.b = strides[0]; p.sd.b = strides[1]; p.sB.b = strides[2]; p.sC.b = strides[3]; p.sz.b = strides[4];
+    p.A = A; p.D = skip; p.bias = delta_bias; p.state = state; p.y = y; p.state_out = state_out;
+    p.batch = B; p.L = 1; p.dim = D; p.N = N; p.G = G; p.softplus = softplus;
+    CHECK_HIP(urnn_launch_scan_step(p, dtype, (hipStream_t)stream), "selective_scan_step");
+    return URNN_OK;
+}
+
+static int norm_args(const char *what, const void *y, const long *strides, const float *pre_w, int dtype, long rows, int D, int act)
+{
+    if (!y || !strides || !pre_w) return fail(URNN_ENULL, "%s: NULL argument", what);
+    if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
+    if (rows < 1 || rows > 8388608 || D < 1 || D > URNN_SEQ_MAX_NORM) return fail(URNN_EINVAL, "%s: rows=%ld (1..8388608) D=%d (1..%d)", what, rows, D, URNN_SEQ_MAX_NORM);
+    if (act < URNN_GATE_NONE || act > URNN_GATE_SILU) return fail(URNN_EINVAL, "%s: act=%d", what, act);
+    return URNN_OK;
+}
+
+extern "C" int urnn_norm_residual(const void *y, const void *gate, const void *residual, const long *strides, const float *pre_w,
+                                  const float *post_w, const float *scale, void *normed, void *residual_out, int dtype, long rows, int D, int act,
+                                  float eps, void *stream)
+{
+    const int rc = norm_args("urnn_norm_residual", y, strides, pre_w, dtype, rows, D, act);
+    if (rc) return rc;
+    if (!normed) return fail(URNN_ENULL, "urnn_norm_residual: NULL argument");
+    if (normed == residual_out) return fail(URNN_EINVAL, "urnn_norm_residual: normed and residual_out are the same buffer");
+    NormParams p = {};
+    p.y = y; p.gate = gate; p.residual = residual; p.sy = strides[0]; p.sg = strides[1]; p.sr = strides[2];
+    p.pre_w = pre_w; p.post_w = post_w; p.scale = scale; p.normed = normed; p.res_out = residual_out;
+    p.rows = rows; p.dim = D; p.act = act; p.eps = eps;
+    const int e = seq_elem(dtype);
+    const bool wide = wide_rows(y, strides[0], 0, e) && wide_rows(gate, strides[1], 0, e) && wide_rows(residual, strides[2], 0, e) && (long)D * e % 16 == 0 &&
+                      aligned16(pre_w) && (!post_w || aligned16(post_w)) && (!scale || aligned16(scale)) && aligned16(normed) && (!residual_out || aligned16(residual_out));
+    CHECK_HIP(urnn_launch_norm(p, dtype, wide, (hipStream_t)stream), "norm_residual");
+    return URNN_OK;
+}
+
+extern "C" size_t urnn_norm_residual_backward_workspace_bytes(long rows, int D)
+{
+    if (rows < 1 || D < 1 || D > URNN_SEQ_MAX_NORM) return 0;
+    return align_up((size_t)urnn_norm_parts(rows, D) * 3 * D * sizeof(float), 256);
+}
+
+extern "C" int urnn_norm_residual_backward(const void *y, const void *gate, const void *residual, const void *dnormed, const void *dresidual_out,
+                                           const long *strides, const float *pre_w, const float *post_w, const float *scale, void *dy, void *dgate,
+                                           void *dresidual, float *dpre_w, float *dpost_w, float *dscale, void *workspace, size_t workspace_bytes,
+                                           int dtype, long rows, int D, int act, float eps, int accumulate, void *stream)
+{
+    const int rc = norm_args("urnn_norm_residual_backward", y, strides, pre_w, dtype, rows, D, act);
+    if (rc) return rc;
+    if (!dy || !workspace) return fail(URNN_ENULL, "urnn_norm_residual_backward: NULL argument");
+    if (dgate && !gate) return fail(URNN_ENULL, "urnn_norm_residual_backward: dgate without gate");
+    if (!aligned16(workspace)) return fail(URNN_EALIGN, "urnn_norm_residual_backward: workspace not 16-byte aligned");
+    if (workspace_bytes < urnn_norm_residual_backward_workspace_bytes(rows, D)) return fail(URNN_EWORKSPACE, "urnn_norm_residual_backward: workspace too small");
+    NormParams p = {};
+    p.y = y; p.gate = gate; p.residual = residual; p.dnormed = dnormed; p.dres = dresidual_out;
+    p.sy = strides[0]; p.sg = strides[1]; p.sr = strides[2]; p.sdn = strides[3]; p.sdr = strides[4];
+    p.pre_w = pre_w; p.post_w = post_w; p.scale = scale; p.dy = dy; p.dgate = dgate; p.dresidual = dresidual;
+    p.partial = reinterpret_cast<float *>(workspace);
+    p.rows = rows; p.dim = D; p.act = act; p.eps = eps; p.parts = urnn_norm_parts(rows, D);
+    const int e = seq_elem(dtype);
+    const bool wide = wide_rows(y, strides[0], 0, e) && wide_rows(gate, strides[1], 0, e) && wide_rows(residual, strides[2], 0, e) &&
+                      wide_rows(dnormed, strides[3], 0, e) && wide_rows(dresidual_out, strides[4], 0, e) && (long)D * e % 16 == 0 && aligned16(pre_w) &&
+                      (!post_w || aligned16(post_w)) && (!scale || aligned16(scale)) && aligned16(dy) && (!dgate || aligned16(dgate)) &&
+                      (!dresidual || aligned16(dresidual));
+    CHECK_HIP(urnn_launch_norm_backward(p, dtype, wide, dpre_w, dpost_w, dscale, accumulate, (hipStream_t)stream), "norm_residual_backward");
     return URNN_OK;
 }

@@ -1,0 +1,314 @@
+// urnn_norm.hip -- the norms around a block in one pass, forward and backward.  Per row of D channels:
+//   p  = act(g) * (y * ry) * w,   ry = 1 / sqrt(mean(y^2) + eps)        the norm after the block and its gate
+//   r' = r + s * p                                                      the residual with its scale
+//   n  = r' * rr * v,             rr = 1 / sqrt(mean(r'^2) + eps)       the norm before the next block
+// without w there is no first norm (ry = 1), without g, r or s that factor or term is left out.
+// Backward, with t = dn v, hat = r' rr, yh = y ry:
+//   dr = dr' + rr (t - hat mean(t hat)),  dp = s dr,  q = dp act(g) w,  dy = ry (q - yh mean(q yh)),  dg = dp yh w act'(g),
+//   dv = sum_rows dn hat,  dw = sum_rows dp act(g) yh,  ds = sum_rows dr p.
+//
+// Memory-bound.  A row lives in the registers of NT threads, EPT values each, so that everything is read once and both means are
+// taken on the way: NT = 16 (D <= 128), 64 (<= 1024), 256 (<= 4096), 512, 1024.  The backward reads y, g, r again instead of r' and
+// the forward's statistics: r' was rounded on its way out, and it is as many bytes.  Its column sums stay in registers over all rows
+// of a block and are folded in a fixed order.
+#include "urnn_seq.h"
+
+enum { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_SILU = 2 };
+
+template <int NT>
+__device__ __forceinline__ void row_sum2(float &a, float &b, float (*red)[2])
+{
+    float v[2] = {a, b};
+    if (NT == 16) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v[i] += dpp_move<0xB1>(v[i]);
+            v[i] += dpp_move<0x4E>(v[i]);
+            v[i] += dpp_move<0x141>(v[i]);
+            v[i] += dpp_move<0x140>(v[i]);
+        }
+    } else {
+        wave_sum_n<2>(v);
+        if (NT > 64) {                               // red: this reduction's own NT / 64 pairs; the caller's next ones use others
+            if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6][0] = v[0]; red[threadIdx.x >> 6][1] = v[1]; }
+            __syncthreads();
+            v[0] = v[1] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NT / 64; ++w) { v[0] += red[w][0]; v[1] += red[w][1]; }
+        }
+    }
+    a = v[0];
+    b = v[1];
+}
+
+// act(g) and act'(g)
+__device__ __forceinline__ void gate_of(int act, float g, float &a, float &da)
+{
+    if (act == ACT_NONE) { a = g; da = 1.0f; return; }
+    const float s = sigmoid_f(g);
+    if (act == ACT_SIGMOID) { a = s; da = s * (1.0f - s); return; }
+    a = g * s;
+    da = s * fmaf(g, 1.0f - s, 1.0f);
+}
+
+// Values of a thread: EPT / V groups of V adjacent channels, NT V apart.
+template <typename T, int V, int NT, int EPT>
+__device__ __forceinline__ void row_load(const T *row, int ln, int D, float (&v)[EPT])
+{
+#pragma unroll
+    for (int c = 0; c < EPT / V; ++c) {
+        const int d = (c * NT + ln) * V;
+        Pack<T, V> t = {};
+        if (d < D) t = *reinterpret_cast<const Pack<T, V> *>(row + d);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[c * V + i] = to_f(t.v[i]);
+    }
+}
+template <typename T, int V, int NT, int EPT>
+__device__ __forceinline__ void row_store(T *row, int ln, int D, const float (&v)[EPT])
+{
+#pragma unroll
+    for (int c = 0; c < EPT / V; ++c) {
+        const int d = (c * NT + ln) * V;
+        Pack<T, V> t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) t.v[i] = from_f<T>(v[c * V + i]);
+        if (d < D) *reinterpret_cast<Pack<T, V> *>(row + d) = t;
+    }
+}
+// A parameter (fp32): in groups of at most four
+template <int V, int NT, int EPT>
+__device__ __forceinline__ void par_load(const float *w, int ln, int D, float fill, float (&v)[EPT])
+{
+    constexpr int W = V % 4 == 0 ? 4 : 1;
+#pragma unroll
+    for (int c = 0; c < EPT / V; ++c)
+#pragma unroll
+        for (int k = 0; k < V; k += W) {
+            const int d = (c * NT + ln) * V + k;
+            Pack<float, W> t;
+#pragma unroll
+            for (int i = 0; i < W; ++i) t.v[i] = fill;
+            if (w && d < D) t = *reinterpret_cast<const Pack<float, W> *>(w + d);
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[c * V + k + i] = t.v[i];
+        }
+}
+
+template <int V, int NT, int EPT>
+__device__ __forceinline__ void par_store(float *w, int ln, int D, const float (&v)[EPT])
+{
+    constexpr int W = V % 4 == 0 ? 4 : 1;
+#pragma unroll
+    for (int c = 0; c < EPT / V; ++c)
+#pragma unroll
+        for (int k = 0; k < V; k += W) {
+            const int d = (c * NT + ln) * V + k;
+            Pack<float, W> t;
+#pragma unroll
+            for (int i = 0; i < W; ++i) t.v[i] = v[c * V + k + i];
+            if (d < D) *reinterpret_cast<Pack<float, W> *>(w + d) = t;
+        }
+}
+
+template <typename T, int V, int NT, int EPT>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const NormParams p)
+{
+    __shared__ float red[2][NT > 64 ? NT / 64 : 1][2];
+    constexpr int RB = NT < 256 ? 256 / NT : 1;
+    const int ln = threadIdx.x % NT, D = p.dim;
+    const long row0 = (long)blockIdx.x * RB + threadIdx.x / NT;
+    const bool ok = row0 < p.rows;
+    const long row = ok ? row0 : 0;
+    const float inv = 1.0f / (float)D;
+    float y[EPT], r[EPT], w[EPT], s[EPT], v[EPT];
+    row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.y) + row * p.sy, ln, D, y);
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) r[i] = 0.0f;
+    if (p.residual) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.residual) + row * p.sr, ln, D, r);
+    float g[EPT];
+    if (p.gate) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.gate) + row * p.sg, ln, D, g);
+    par_load<V, NT, EPT>(p.post_w, ln, D, 1.0f, w);
+    par_load<V, NT, EPT>(p.scale, ln, D, 1.0f, s);
+    par_load<V, NT, EPT>(p.pre_w, ln, D, 0.0f, v);
+    float ss = 0.0f, none = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) ss = fmaf(y[i], y[i], ss);
+    row_sum2<NT>(ss, none, red[0]);
+    const float ry = p.post_w ? __builtin_amdgcn_rsqf(fmaf(ss, inv, p.eps)) : 1.0f;
+    ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+        float q = y[i] * ry * w[i];
+        if (p.gate) {
+            float a, da;
+            gate_of(p.act, g[i], a, da);
+            q *= a;
+        }
+        r[i] = fmaf(s[i], q, r[i]);
+        ss = fmaf(r[i], r[i], ss);
+    }
+    row_sum2<NT>(ss, none, red[1]);
+    const float rr = __builtin_amdgcn_rsqf(fmaf(ss, inv, p.eps));
+    if (!ok) return;
+    if (p.res_out) row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.res_out) + row * D, ln, D, r);
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) r[i] *= rr * v[i];
+    row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.normed) + row * D, ln, D, r);
+}
+
+template <typename T, int V, int NT, int EPT>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(const NormParams p)
+{
+    __shared__ float red[3][NT > 64 ? NT / 64 : 1][2];
+    constexpr int RB = NT < 256 ? 256 / NT : 1;
+    __shared__ float fold[RB > 1 ? 256 * EPT : 1];
+    const int ln = threadIdx.x % NT, rg = threadIdx.x / NT, D = p.dim;
+    const float inv = 1.0f / (float)D;
+    float w[EPT], s[EPT], v[EPT], cv[EPT] = {}, cw[EPT] = {}, cs[EPT] = {};
+    par_load<V, NT, EPT>(p.post_w, ln, D, 1.0f, w);
+    par_load<V, NT, EPT>(p.scale, ln, D, 1.0f, s);
+    par_load<V, NT, EPT>(p.pre_w, ln, D, 0.0f, v);
+    for (long base = (long)blockIdx.x * RB; base < p.rows; base += (long)gridDim.x * RB) {
+        const long row0 = base + rg;
+        const bool ok = row0 < p.rows;
+        const long row = ok ? row0 : base;
+        float y[EPT], r[EPT], g[EPT], dn[EPT], dr[EPT], a[EPT], da[EPT];
+        row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.y) + row * p.sy, ln, D, y);
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) { r[i] = dn[i] = dr[i] = 0.0f; a[i] = 1.0f; da[i] = 0.0f; }
+        if (p.residual) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.residual) + row * p.sr, ln, D, r);
+        if (p.gate) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.gate) + row * p.sg, ln, D, g);
+        if (p.dnormed) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.dnormed) + row * p.sdn, ln, D, dn);
+        if (p.dres) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.dres) + row * p.sdr, ln, D, dr);
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) s1 = fmaf(y[i], y[i], s1);
+        row_sum2<NT>(s1, s2, red[0]);
+        const float ry = p.post_w ? __builtin_amdgcn_rsqf(fmaf(s1, inv, p.eps)) : 1.0f;
+        s1 = s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            if (p.gate) gate_of(p.act, g[i], a[i], da[i]);
+            y[i] *= ry;                                          // yh
+            g[i] = a[i] * y[i];                                  // act(g) yh; p = g w
+            r[i] = fmaf(s[i] * w[i], g[i], r[i]);                // r'
+            s1 = fmaf(r[i], r[i], s1);
+            s2 = fmaf(dn[i] * v[i], r[i], s2);
+        }
+        row_sum2<NT>(s1, s2, red[1]);
+        const float rr = __builtin_amdgcn_rsqf(fmaf(s1, inv, p.eps)), m1 = s2 * inv * rr;
+        s1 = s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            const float hat = r[i] * rr;
+            dr[i] += rr * fmaf(-hat, m1, dn[i] * v[i]);
+            if (ok) {
+                cv[i] = fmaf(dn[i], hat, cv[i]);
+                cw[i] = fmaf(dr[i] * s[i], g[i], cw[i]);
+                cs[i] = fmaf(dr[i], g[i] * w[i], cs[i]);
+            }
+            const float dpw = dr[i] * s[i] * w[i];
+            r[i] = dpw * a[i];                                   // q
+            da[i] *= dpw * y[i];                                 // dg
+            s2 = fmaf(r[i], y[i], s2);
+        }
+        row_sum2<NT>(s1, s2, red[2]);
+        const float m2 = p.post_w ? s2 * inv : 0.0f;
+        if (ok) {
+            if (p.dresidual) row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.dresidual) + row * D, ln, D, dr);
+            if (p.dgate) row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.dgate) + row * D, ln, D, da);
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) r[i] = ry * fmaf(-y[i], m2, r[i]);
+            row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.dy) + row * D, ln, D, r);
+        }
+    }
+    auto put = [&](int which, const float (&c)[EPT]) {
+        float *out = p.partial + ((long)blockIdx.x * 3 + which) * D;
+        if (RB == 1) {
+            par_store<V, NT, EPT>(out, ln, D, c);
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) fold[(rg * EPT + i) * NT + ln] = c[i];
+            __syncthreads();
+            for (int k = threadIdx.x; k < NT * EPT; k += 256) {
+                float t = 0.0f;
+#pragma unroll
+                for (int l = 0; l < RB; ++l) t += fold[l * NT * EPT + k];
+                const int i = k / NT, d = ((i / V) * NT + k % NT) * V + i % V;
+                if (d < D) out[d] = t;
+            }
+        }
+    };
+    put(0, cv);
+    put(1, cw);
+    put(2, cs);
+}
+
+// out[i] (+)= sum over parts of src[part * stride + i], in double: 64 columns and four lanes of parts per block.
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float *__restrict__ src, long stride, int parts, long n, float *out, int accumulate)
+{
+    __shared__ double s[4][64];
+    const long i = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int r = threadIdx.x >> 6;
+    double a = 0.0;
+    if (i < n)
+        for (int t = r; t < parts; t += 4) a += (double)src[t * stride + i];
+    s[r][threadIdx.x & 63] = a;
+    __syncthreads();
+    if (r || i >= n) return;
+    const int l = threadIdx.x;
+    const float v = (float)((s[0][l] + s[1][l]) + (s[2][l] + s[3][l]));
+    out[i] = accumulate ? out[i] + v : v;
+}
+hipError_t urnn_launch_sum_parts(const float *src, long stride, int parts, long n, float *out, int accumulate, hipStream_t st)
+{
+    sum_parts_kernel<<<dim3((unsigned)((n + 63) / 64)), 256, 0, st>>>(src, stride, parts, n, out, accumulate);
+    return hipGetLastError();
+}
+
+static int row_threads(int D) { return D <= 128 ? 16 : D <= 1024 ? 64 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024; }
+int urnn_norm_parts(long rows, int D)
+{
+    const int nt = row_threads(D), rb = nt < 256 ? 256 / nt : 1;
+    const long blocks = (rows + rb - 1) / rb, most = nt <= 256 ? 1024 : 512;
+    return (int)(blocks < most ? blocks : most);
+}
+
+template <typename T, int V, int NT, int EPT>
+static hipError_t launch_norm(const NormParams &p, bool backward, hipStream_t st)
+{
+    constexpr int threads = NT < 256 ? 256 : NT, RB = NT < 256 ? 256 / NT : 1;
+    if (backward) norm_backward_kernel<T, V, NT, EPT><<<dim3((unsigned)p.parts), threads, 0, st>>>(p);
+    else norm_kernel<T, V, NT, EPT><<<dim3((unsigned)((p.rows + RB - 1) / RB)), threads, 0, st>>>(p);
+    return hipGetLastError();
+}
+template <typename T, int V>
+static hipError_t by_width(const NormParams &p, bool backward, hipStream_t st)
+{
+    const int D = p.dim;
+    if (D <= 128) return launch_norm<T, V, 16, 8>(p, backward, st);
+    if (D <= 512) return launch_norm<T, V, 64, 8>(p, backward, st);
+    if (D <= 1024) return launch_norm<T, V, 64, 16>(p, backward, st);
+    if (D <= 2048) return launch_norm<T, V, 256, 8>(p, backward, st);
+    if (D <= 4096) return launch_norm<T, V, 256, 16>(p, backward, st);
+    if (D <= 8192) return launch_norm<T, V, 512, 16>(p, backward, st);
+    return launch_norm<T, V, 1024, 16>(p, backward, st);
+}
+static hipError_t by_type(const NormParams &p, int dtype, bool wide, bool backward, hipStream_t st)
+{
+    if (dtype == URNN_F32) return wide ? by_width<float, 4>(p, backward, st) : by_width<float, 1>(p, backward, st);
+    if (dtype == URNN_BF16) return wide ? by_width<bf16_t, 8>(p, backward, st) : by_width<bf16_t, 1>(p, backward, st);
+    return wide ? by_width<f16_t, 8>(p, backward, st) : by_width<f16_t, 1>(p, backward, st);
+}
+
+hipError_t urnn_launch_norm(const NormParams &p, int dtype, bool wide, hipStream_t st) { return by_type(p, dtype, wide, false, st); }
+hipError_t urnn_launch_norm_backward(const NormParams &p, int dtype, bool wide, float *dpre, float *dpost, float *dscale, int accumulate, hipStream_t st)
+{
+    hipError_t e = by_type(p, dtype, wide, true, st);
+    float *const outs[3] = {dpre, dpost, dscale};
+    for (int k = 0; k < 3 && e == hipSuccess; ++k)
+        if (outs[k]) e = urnn_launch_sum_parts(p.partial + (long)k * p.dim, 3l * p.dim, p.parts, p.dim, outs[k], accumulate, st);
+    return e;
+}

@@ -1,0 +1,133 @@
+// urnn_seq.h -- shared pieces of the sequence operators (short causal convolution, selective state space scan, norms around a block):
+// element types, the activations, parameter blocks and launchers.
+#pragma once
+#include "urnn_common.h"
+#include "urnn_kernels.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// One rounding to nearest even from fp32; everything between a load and a store is fp32.
+template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
+
+// V consecutive elements as one access (V * sizeof(T) <= 16 bytes, naturally aligned).
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+#define URNN_LOG2E 1.44269504088896340736f
+#define URNN_LN2 0.69314718055994530942f
+
+// exp(x) as 2^(x log2 e): v_exp_f32, relative error about 2^-23 + |x| 2^-24.
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * URNN_LOG2E); }
+__device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x)); }
+__device__ __forceinline__ float silu_f(float x) { return x * sigmoid_f(x); }
+
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1].  log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the series
+// 2 s (1 + s^2/3 + s^4/5 + ...) to s^12/13 leaves 1.4e-8 of the value, and keeps full relative accuracy where e is tiny (a step of
+// exp(x) for x << 0), which log(1 + e) loses.
+__device__ __forceinline__ float softplus_f(float x)
+{
+    const float e = exp_fast(-fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+    float p = 1.0f / 13.0f;
+    p = fmaf(p, q, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    p = fmaf(p, q, 1.0f);
+    return fmaxf(x, 0.0f) + 2.0f * s * p;
+}
+
+// Sum over the four lanes of a quad, returned to all of them.
+__device__ __forceinline__ float quad_sum(float v)
+{
+    v += dpp_move<0xB1>(v);
+    v += dpp_move<0x4E>(v);
+    return v;
+}
+
+// Tokens of sequence b that count: lengths clamped to [0, L], so that no length can reach outside the tensors.
+__device__ __forceinline__ int seq_len(const int *lengths, int b, int L)
+{
+    if (!lengths) return L;
+    const int n = lengths[b];
+    return n < 0 ? 0 : (n > L ? L : n);
+}
+
+// A (B, L, C) tensor: element strides of batch and token, the channels are adjacent.
+struct SeqStride { long b, t; };
+
+enum { URNN_SEQ_MAX_STATES = 64, URNN_SEQ_MAX_TAPS = 4, URNN_SEQ_MAX_NORM = 16384 };
+
+// ---- selective scan --------------------------------------------------------------------------------------------------
+struct ScanParams {
+    const void *u, *delta, *B, *C, *z, *dout;        // (B,L,D), B / C (B,L,G,N)
+    SeqStride su, sd, sB, sC, sz, so;
+    const float *A, *D, *bias;                       // (D,N), (D) or NULL, (D) or NULL
+    const float *state;                              // (B,D,N) or NULL
+    const int *lengths;                              // (B) or NULL
+    void *y;                                         // (B,L,D) contiguous
+    float *state_out;                                // (B,D,N) or NULL
+    float *keep;                                     // checkpoints [B][ceil(L/URNN_SCAN_CK)][D][NP], or NULL
+    float *sum;                                      // chunk summaries: sum of the steps [B][chunks][D] ...
+    float *S;                                        // ... and the state of a chunk that starts from zero [B][chunks][D][NP]
+    int batch, L, dim, N, G, chunks, CL, softplus;
+    // backward
+    const float *dstate_out;                         // (B,D,N) or NULL
+    void *du, *ddelta, *dz;                          // (B,L,D) contiguous
+    float *dstate;                                   // (B,D,N) or NULL
+    float *dBp, *dCp;                                // per channel block: [blocks of a group][B][L][G][N]
+    float *dAp, *dDp, *dbp;                          // per (batch slot, chunk): [parts][D][NP], [parts][D], [parts][D]
+};
+
+#define URNN_SCAN_CK 8      // tokens between two checkpoints of the state
+#define URNN_SCAN_CB 64     // channels of a block
+
+static inline int urnn_scan_np(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+
+hipError_t urnn_launch_scan(const ScanParams &p, int dtype, hipStream_t st);
+hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st);
+int urnn_scan_chunks(int B, int L, int D, int *CL);
+
+// ---- short causal convolution ----------------------------------------------------------------------------------------
+struct ConvSeqParams {
+    const void *x, *dout;                            // (B,L,D)
+    SeqStride sx, so;
+    const float *weight, *bias;                      // (D,K), (D) or NULL
+    const void *state;                               // (B,K-1,D) contiguous or NULL: the inputs before the first, oldest first
+    const int *lengths;
+    void *y, *state_out;                             // (B,L,D), (B,K-1,D) or NULL
+    int batch, L, dim, K, silu;
+    int T, chunks;                                   // tokens of a thread's chunk, chunks of a sequence
+    // backward
+    const void *dstate_out;                          // (B,K-1,D) or NULL
+    void *dx, *dstate;                               // (B,L,D), (B,K-1,D) or NULL
+    float *partial;                                  // [parts][K + 1][dim]: sums of a block's tokens for weight and bias
+    int parts;
+};
+
+hipError_t urnn_launch_conv_seq(ConvSeqParams p, int dtype, bool wide, hipStream_t st);
+hipError_t urnn_launch_conv_seq_step(const ConvSeqParams &p, int dtype, bool wide, hipStream_t st);
+hipError_t urnn_launch_conv_seq_backward(ConvSeqParams p, int dtype, bool wide, float *dweight, float *dbias, int accumulate, hipStream_t st);
+int urnn_conv_seq_parts(int B, int L, int D);
+
+// ---- norms around a block ----------------------------------------------------------------------------------------------
+struct NormParams {
+    const void *y, *gate, *residual, *dnormed, *dres; // (M,D) rows; gate, residual, dnormed, dres may be NULL
+    long sy, sg, sr, sdn, sdr;                       // row strides in elements
+    const float *pre_w, *post_w, *scale;             // (D); post_w / scale may be NULL
+    void *normed, *res_out;                          // (M,D) contiguous
+    void *dy, *dgate, *dresidual;                    // (M,D) contiguous; dgate / dresidual may be NULL
+    float *partial;                                  // [parts][3][D]: dpre_w, dpost_w, dscale
+    long rows;
+    int dim, act, parts;
+    float eps;
+};
+
+hipError_t urnn_launch_norm(const NormParams &p, int dtype, bool wide, hipStream_t st);
+hipError_t urnn_launch_norm_backward(const NormParams &p, int dtype, bool wide, float *dpre, float *dpost, float *dscale, int accumulate, hipStream_t st);
+int urnn_norm_parts(long rows, int D);
+
+// out[i] (+)= sum over parts of src[part][i], in ascending order of parts within fixed groups (bit-reproducible)
+hipError_t urnn_launch_sum_parts(const float *src, long stride, int parts, long n, float *out, int accumulate, hipStream_t st);

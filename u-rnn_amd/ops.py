@@ -3,6 +3,7 @@
 Every function takes contiguous float32 CUDA(=HIP) tensors, passes ``data_ptr()`` + dims + the current
 stream across the ABI and returns torch tensors.  No op has a PyTorch fallback.
 """
+import ctypes
 import os
 
 import torch
@@ -446,3 +447,306 @@ def stage1_scalar_rain(S, rain, cumsum, weight, bias, t, nums, rain_max, cumsum_
 
 def advance_counter(counter, delta=1):
     check(lib().urnn_advance_counter(_ptr(counter), int(delta), _stream()), "urnn_advance_counter")
+
+
+# ---- sequence operators --------------------------------------------------------------------------------------------------
+# Short causal convolution, selective state space scan and the norms around a block, over (batch, length, channels) tensors.  They take
+# float32, bfloat16 or float16 activations (parameters, states of the scan and parameter gradients are float32) whose channels are
+# adjacent: a slice of a wider projection goes in as it is.  Their gradients are in train_ops.
+SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # include/urnn_hip.h URNN_F32 / URNN_BF16 / URNN_F16
+GATE_ACTS = {"none": 0, "sigmoid": 1, "silu": 2}                         # include/urnn_hip.h URNN_GATE_*
+
+
+def _seq_dtype(what, t):
+    code = SEQ_DTYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{what}: activations are float32, bfloat16 or float16 (got {t.dtype})")
+    return code
+
+
+def _seq_check(what, name, t, shape, dtype, contiguous=False):
+    """Shape, type and layout of an argument (no device is needed to refuse a wrong one)."""
+    if tuple(t.shape) != shape:
+        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+    if contiguous:
+        if not t.is_contiguous():
+            raise RuntimeError(f"{what}: {name} must be contiguous")
+    elif t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise RuntimeError(f"{what}: the channels of {name} must be adjacent (stride {t.stride(-1)})")
+
+
+def _seq_device(what, *tensors):
+    """All on the current device: kernels are enqueued on its current stream."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: urnn_amd ops need tensors on the GPU (cuda:N / HIP device); there is no CPU path")
+        if dev is None:
+            dev = t.device
+            if dev.index != torch.cuda.current_device():
+                raise RuntimeError(f"{what}: tensors are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+        elif t.device != dev:
+            raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
+
+
+def _span(t):
+    return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _seq_out(what, name, t, shape, dtype, inputs, same=()):
+    """A given output buffer: contiguous, of the result's shape, and apart from every input (``same``: inputs it may be exactly)."""
+    _seq_check(what, name, t, shape, dtype, contiguous=True)
+    lo, hi = _span(t)
+    for x in inputs:
+        if x is None or x.numel() == 0:
+            continue
+        a, b = _span(x)
+        if a < hi and lo < b and not any(x is s and a == lo and x.is_contiguous() for s in same):
+            raise RuntimeError(f"{what}: {name} overlaps an input")
+
+
+def _lengths_check(what, lengths, B):
+    if lengths is not None:
+        _seq_check(what, "lengths", lengths, (B,), torch.int32, contiguous=True)
+
+
+def _no_empty(what, t):
+    if t.numel() == 0:
+        raise RuntimeError(f"{what}: empty input of shape {tuple(t.shape)}")
+
+
+def _conv_seq_check(what, x, weight, bias, state, lead):
+    _no_empty(what, x)
+    D = x.shape[-1]
+    if weight.dim() != 2 or weight.shape[0] != D or not 2 <= weight.shape[1] <= 4:
+        raise RuntimeError(f"{what}: weight has shape {tuple(weight.shape)}, expected ({D}, 2..4)")
+    K = weight.shape[1]
+    _seq_check(what, "x", x, lead + (D,), x.dtype)
+    _seq_check(what, "weight", weight, (D, K), torch.float32, contiguous=True)
+    if bias is not None:
+        _seq_check(what, "bias", bias, (D,), torch.float32, contiguous=True)
+    if state is not None:
+        _seq_check(what, "state", state, (lead[0], K - 1, D), x.dtype, contiguous=True)
+    return D, K
+
+
+def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, out=None, want_state=False, state_out=None):
+    """Short causal depthwise convolution along time: y[:, t] = silu(bias + sum_k weight[:, k] * line[:, t + k]), line = [state | x].
+
+    x (B,L,D); weight (D,K), K = 2..4; bias (D); ``state`` (B,K-1,D): the inputs before the first token, oldest first (None: zeros);
+    ``lengths`` (B) int32: tokens of each sequence of a padded batch -- later ones are not read and give zeros.  ``silu`` False: no
+    activation.  Returns y (B,L,D), or (y, state (B,K-1,D)) with ``want_state``: the last K-1 inputs of every sequence, what the next
+    call or ``causal_conv_step`` goes on from."""
+    what = "causal_conv"
+    dt = _seq_dtype(what, x)
+    if x.dim() != 3:
+        raise RuntimeError(f"{what}: x has shape {tuple(x.shape)}, expected (B, L, D)")
+    B, L = x.shape[0], x.shape[1]
+    D, K = _conv_seq_check(what, x, weight, bias, state, (B, L))
+    _lengths_check(what, lengths, B)
+    if out is not None:
+        _seq_out(what, "out", out, (B, L, D), x.dtype, (x, weight, bias, state, state_out))
+    if state_out is not None:
+        _seq_out(what, "state_out", state_out, (B, K - 1, D), x.dtype, (x, weight, bias, state))
+    _seq_device(what, x, weight, bias, state, lengths, out, state_out)
+    if out is None:
+        out = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
+    if want_state and state_out is None:
+        state_out = torch.empty((B, K - 1, D), dtype=x.dtype, device=x.device)
+    sb, st, _ = x.stride()
+    check(lib().urnn_causal_conv(_ptr(x), sb, st, _ptr(weight), _ptr(bias), _ptr(state), _ptr(lengths), _ptr(out), _ptr(state_out), dt, B, L,
+                                 D, K, 1 if silu else 0, _stream()), "urnn_causal_conv")
+    return (out, state_out) if want_state else out
+
+
+def causal_conv_step(x, state, weight, bias=None, silu=True, out=None, state_out=None):
+    """``causal_conv`` for one token: x (B,D), state (B,K-1,D) -> (y (B,D), new state).  ``state_out`` may be ``state``: in place."""
+    what = "causal_conv_step"
+    dt = _seq_dtype(what, x)
+    if x.dim() != 2:
+        raise RuntimeError(f"{what}: x has shape {tuple(x.shape)}, expected (B, D)")
+    if state is None:
+        raise RuntimeError(f"{what}: state is None")
+    B = x.shape[0]
+    D, K = _conv_seq_check(what, x, weight, bias, state, (B,))
+    if out is not None:
+        _seq_out(what, "out", out, (B, D), x.dtype, (x, weight, bias, state, state_out))
+    if state_out is not None:
+        _seq_out(what, "state_out", state_out, (B, K - 1, D), x.dtype, (x, weight, bias, state), same=(state,))
+    _seq_device(what, x, weight, bias, state, out, state_out)
+    if out is None:
+        out = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    if state_out is None:
+        state_out = torch.empty_like(state)
+    check(lib().urnn_causal_conv_step(_ptr(x), x.stride(0), _ptr(weight), _ptr(bias), _ptr(state), _ptr(out), _ptr(state_out), dt, B, D, K,
+                                      1 if silu else 0, _stream()), "urnn_causal_conv_step")
+    return out, state_out
+
+
+def _scan_check(what, u, delta, A, B, C, D, z, delta_bias, lead):
+    """-> (channels, groups, states, B, C) with B and C as (..., groups, states)."""
+    _no_empty(what, u)
+    dim = u.shape[-1]
+    if A.dim() != 2 or A.shape[0] != dim or not 1 <= A.shape[1] <= 64:
+        raise RuntimeError(f"{what}: A has shape {tuple(A.shape)}, expected ({dim}, 1..64)")
+    N = A.shape[1]
+    _seq_check(what, "u", u, lead + (dim,), u.dtype)
+    _seq_check(what, "delta", delta, lead + (dim,), u.dtype)
+    if z is not None:
+        _seq_check(what, "z", z, lead + (dim,), u.dtype)
+    _seq_check(what, "A", A, (dim, N), torch.float32, contiguous=True)
+    for name, t in (("D", D), ("delta_bias", delta_bias)):
+        if t is not None:
+            _seq_check(what, name, t, (dim,), torch.float32, contiguous=True)
+    if B.dim() == len(lead) + 1:
+        B = B.unsqueeze(-2)
+    if C.dim() == len(lead) + 1:
+        C = C.unsqueeze(-2)
+    G = B.shape[-2] if B.dim() == len(lead) + 2 else 0
+    if G < 1 or dim % G:
+        raise RuntimeError(f"{what}: B has shape {tuple(B.shape)}; its groups must divide {dim} channels")
+    for name, t in (("B", B), ("C", C)):
+        _seq_check(what, name, t, lead + (G, N), u.dtype)
+        if G > 1 and t.stride(-2) != N:
+            raise RuntimeError(f"{what}: the groups of {name} must be adjacent (stride {t.stride(-2)}, {N} states)")
+    return dim, G, N, B, C
+
+
+def selective_scan_workspace(u, A):
+    """The record that a training forward leaves for ``train_ops.selective_scan_backward``: a buffer for ``selective_scan(..., ws=)``."""
+    B, L, dim = u.shape
+    n = lib().urnn_selective_scan_workspace_bytes(B, L, dim, A.shape[1], 1)
+    return torch.empty(int(n), dtype=torch.uint8, device=u.device)
+
+
+def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=True, state=None, lengths=None, out=None, want_state=False,
+                   state_out=None, ws=None):
+    """Selective state space scan: step = softplus(delta + delta_bias), h_t = exp(step A) h_(t-1) + step u B_t,
+    y = (C_t . h_t + D u) * silu(z).
+
+    u, delta, z (batch,L,dim); A (dim,N), N = 1..64; B, C (batch,L,N) or (batch,L,G,N) with dim / G channels to a group; D, delta_bias
+    (dim).  ``softplus`` False: step = delta + delta_bias.  ``state`` (batch,dim,N) float32: the state before the first token (None: zeros);
+    ``lengths`` (batch) int32: tokens of each sequence of a padded batch -- later ones are not read and give zeros.  ``ws``: a buffer of
+    ``selective_scan_workspace(u, A)`` (or an Arena) that the backward will read: a training forward; None: scratch for this call.
+    Returns y, or (y, state after each sequence's last token) with ``want_state``."""
+    what = "selective_scan"
+    dt = _seq_dtype(what, u)
+    if u.dim() != 3:
+        raise RuntimeError(f"{what}: u has shape {tuple(u.shape)}, expected (batch, L, dim)")
+    nb, L = u.shape[0], u.shape[1]
+    dim, G, N, B, C = _scan_check(what, u, delta, A, B, C, D, z, delta_bias, (nb, L))
+    if state is not None:
+        _seq_check(what, "state", state, (nb, dim, N), torch.float32, contiguous=True)
+    _lengths_check(what, lengths, nb)
+    inputs = (u, delta, A, B, C, D, z, delta_bias, state)
+    if out is not None:
+        _seq_out(what, "out", out, (nb, L, dim), u.dtype, inputs + (state_out,))
+    if state_out is not None:
+        _seq_out(what, "state_out", state_out, (nb, dim, N), torch.float32, inputs)
+    _seq_device(what, *inputs, lengths, out, state_out)
+    Lb = lib()
+    keep = ws is not None
+    nbytes = Lb.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1 if keep else 0)
+    if keep:
+        ws = _scratch(ws, nbytes, u.device, key="scan")
+        _seq_device(what, u, ws)
+    elif nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=u.device)
+    if out is None:
+        out = torch.empty((nb, L, dim), dtype=u.dtype, device=u.device)
+    if want_state and state_out is None:
+        state_out = torch.empty((nb, dim, N), dtype=torch.float32, device=u.device)
+    strides = (ctypes.c_long * 10)(*u.stride()[:2], *delta.stride()[:2], *B.stride()[:2], *C.stride()[:2], *(z.stride()[:2] if z is not None else (0, 0)))
+    check(Lb.urnn_selective_scan(_ptr(u), _ptr(delta), _ptr(B), _ptr(C), _ptr(z), strides, _ptr(A), _ptr(D), _ptr(delta_bias), _ptr(state),
+                                 _ptr(lengths), _ptr(out), _ptr(state_out), _ptr(ws), nbytes if not keep else ws.numel(), 1 if keep else 0, dt, nb, L,
+                                 dim, G, N, 1 if softplus else 0, _stream()), "urnn_selective_scan")
+    return (out, state_out) if want_state else out
+
+
+def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=None, softplus=True, out=None, state_out=None):
+    """``selective_scan`` for one token: u, delta, z (batch,dim), B, C (batch,N) or (batch,G,N), state (batch,dim,N) float32 -> (y, new state).
+    ``state_out`` may be ``state``: in place."""
+    what = "selective_scan_step"
+    dt = _seq_dtype(what, u)
+    if u.dim() != 2:
+        raise RuntimeError(f"{what}: u has shape {tuple(u.shape)}, expected (batch, dim)")
+    if state is None:
+        raise RuntimeError(f"{what}: state is None")
+    nb = u.shape[0]
+    dim, G, N, B, C = _scan_check(what, u, delta, A, B, C, D, z, delta_bias, (nb,))
+    _seq_check(what, "state", state, (nb, dim, N), torch.float32, contiguous=True)
+    inputs = (u, delta, A, B, C, D, z, delta_bias, state)
+    if out is not None:
+        _seq_out(what, "out", out, (nb, dim), u.dtype, inputs + (state_out,))
+    if state_out is not None:
+        _seq_out(what, "state_out", state_out, (nb, dim, N), torch.float32, inputs, same=(state,))
+    _seq_device(what, *inputs, out, state_out)
+    if out is None:
+        out = torch.empty((nb, dim), dtype=u.dtype, device=u.device)
+    if state_out is None:
+        state_out = torch.empty_like(state)
+    strides = (ctypes.c_long * 5)(u.stride(0), delta.stride(0), B.stride(0), C.stride(0), z.stride(0) if z is not None else 0)
+    check(lib().urnn_selective_scan_step(_ptr(u), _ptr(delta), _ptr(B), _ptr(C), _ptr(z), strides, _ptr(A), _ptr(D), _ptr(delta_bias), _ptr(state),
+                                         _ptr(out), _ptr(state_out), dt, nb, dim, G, N, 1 if softplus else 0, _stream()),
+          "urnn_selective_scan_step")
+    return out, state_out
+
+
+def _rows(what, name, t, shape, dtype):
+    """(..., D) as rows of D adjacent channels a fixed stride apart: the row stride."""
+    _seq_check(what, name, t, shape, dtype)
+    stride, n = None, 1
+    for size, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if stride is None:
+            stride = s
+        elif s != stride * n:
+            raise RuntimeError(f"{what}: the rows of {name} are not evenly spaced (strides {t.stride()})")
+        n *= size
+    return t.shape[-1] if stride is None else stride
+
+
+def _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act):
+    _no_empty(what, y)
+    D = y.shape[-1]
+    if gate_act not in GATE_ACTS:
+        raise RuntimeError(f"{what}: gate_act {gate_act!r} is none of {sorted(GATE_ACTS)}")
+    if D > 16384:
+        raise RuntimeError(f"{what}: {D} channels (at most 16384)")
+    for name, t in (("pre_w", pre_w), ("post_w", post_w), ("scale", scale)):
+        if t is not None:
+            _seq_check(what, name, t, (D,), torch.float32, contiguous=True)
+    shape = tuple(y.shape)
+    return [_rows(what, name, t, shape, y.dtype) if t is not None else 0 for name, t in (("y", y), ("gate", gate), ("residual", residual))]
+
+
+def norm_residual(y, pre_w, residual=None, post_w=None, gate=None, scale=None, gate_act="silu", eps=NORM_EPS, out=None, residual_out=None):
+    """The norms around a block in one pass over (..., D) rows: the norm after it (``post_w``) with its gate, the residual with its
+    scale, and the norm before the next one (``pre_w``):
+
+        r' = residual + scale * act(gate) * post_w * y / rms(y),    normed = pre_w * r' / rms(r'),    rms(x) = sqrt(mean(x^2) + eps).
+
+    post_w None: y enters as it is; residual, gate or scale None: left out.  ``gate_act``: "silu", "sigmoid" or "none" (the gate itself).
+    Parameters (D) float32.  Returns (normed, r'), both contiguous.  ``residual_out`` may be ``residual`` (in place)."""
+    what = "norm_residual"
+    dt = _seq_dtype(what, y)
+    sy, sg, sr = _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act)
+    shape, inputs = tuple(y.shape), (y, residual, gate)
+    if out is not None:
+        _seq_out(what, "out", out, shape, y.dtype, inputs + (residual_out,), same=inputs)
+    if residual_out is not None:
+        _seq_out(what, "residual_out", residual_out, shape, y.dtype, inputs, same=inputs)
+    _seq_device(what, y, pre_w, residual, post_w, gate, scale, out, residual_out)
+    if out is None:
+        out = torch.empty(shape, dtype=y.dtype, device=y.device)
+    if residual_out is None:
+        residual_out = torch.empty(shape, dtype=y.dtype, device=y.device)
+    D = shape[-1]
+    check(lib().urnn_norm_residual(_ptr(y), _ptr(gate), _ptr(residual), (ctypes.c_long * 3)(sy, sg, sr), _ptr(pre_w), _ptr(post_w), _ptr(scale),
+                                   _ptr(out), _ptr(residual_out), dt, y.numel() // D, D, GATE_ACTS[gate_act], float(eps), _stream()), "urnn_norm_residual")
+    return out, residual_out

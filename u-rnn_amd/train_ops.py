@@ -1,6 +1,8 @@
 """ctypes wrappers of the training entry points of the C ABI: backward of the ConvGRU / Skip-ConvGRU cell, the
 stage convs, the transposed convs and the head; the loss; the clipped Adam step.  ``urnn_amd.training`` assembles them into SWP
 windows and the training loop.  A backward call reads the scratch buffer its forward ran on (``fwd_ws``)."""
+import ctypes
+
 import torch
 
 from . import ops
@@ -185,3 +187,89 @@ def adam_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.9
     check(L.urnn_adam_step_f32(p(params), p(grads), p(exp_avg), p(exp_avg_sq), n, float(lr), float(betas[0]), float(betas[1]), float(eps),
                                int(step), p(step_dev), float(max_grad_norm), p(out), p(ws), ws.numel(), ops._stream()), "urnn_adam_step_f32")
     return out
+
+
+# ---- sequence operators (ops.causal_conv, ops.selective_scan, ops.norm_residual) --------------------------------------------
+def _param_grads_check(what, grads, accumulate, shapes):
+    """-> (the dict that receives the gradients, the buffers in it that the caller gave)."""
+    g = {} if grads is None else grads
+    if accumulate and any(g.get(k) is None for k in shapes):
+        raise RuntimeError(f"{what}: accumulate needs the gradients {sorted(shapes)} in grads")
+    given = [g[k] for k in shapes if g.get(k) is not None]
+    for k, shape in shapes.items():
+        if g.get(k) is not None:
+            ops._seq_check(what, k, g[k], shape, torch.float32, contiguous=True)
+    return g, given
+
+
+def _param_grads(grads, shapes, dev):
+    """Buffers of the parameters' gradients: those of a former call's dict or the caller's own views, and new ones."""
+    for k, shape in shapes.items():
+        if grads.get(k) is None:
+            grads[k] = torch.empty(shape, dtype=torch.float32, device=dev)
+    return grads
+
+
+def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, silu=True, dstate_out=None, grads=None, accumulate=False,
+                         scratch=None):
+    """Backward of ``ops.causal_conv`` given dout (B,L,D) and, where the returned state was used further, ``dstate_out`` (B,K-1,D).
+    Returns a dict: dx, dstate (None without state), dweight, dbias (None without bias); parameter gradients are float32, into the buffers
+    of ``grads`` if given, added to them with ``accumulate``."""
+    what = "causal_conv_backward"
+    dt = ops._seq_dtype(what, x)
+    if x.dim() != 3:
+        raise RuntimeError(f"{what}: x has shape {tuple(x.shape)}, expected (B, L, D)")
+    B, L = x.shape[0], x.shape[1]
+    D, K = ops._conv_seq_check(what, x, weight, bias, state, (B, L))
+    ops._seq_check(what, "dout", dout, (B, L, D), x.dtype)
+    ops._lengths_check(what, lengths, B)
+    if dstate_out is not None:
+        ops._seq_check(what, "dstate_out", dstate_out, (B, K - 1, D), x.dtype, contiguous=True)
+    shapes = {"dweight": (D, K), **({"dbias": (D,)} if bias is not None else {})}
+    g, given = _param_grads_check(what, grads, accumulate, shapes)
+    ops._seq_device(what, x, weight, dout, bias, state, lengths, dstate_out, *given)
+    L_ = lib()
+    _param_grads(g, shapes, x.device)
+    g.setdefault("dbias", None)
+    g["dx"] = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
+    g["dstate"] = torch.empty_like(state) if state is not None else None
+    ws = _seq_scratch(scratch, L_.urnn_causal_conv_backward_workspace_bytes(B, L, D, K), x.device)
+    p = ops._ptr
+    check(L_.urnn_causal_conv_backward(p(x), *x.stride()[:2], p(weight), p(bias), p(state), p(lengths), p(dout), *dout.stride()[:2], p(dstate_out),
+                                       p(g["dx"]), p(g["dstate"]), p(g["dweight"]), p(g["dbias"]), p(ws), ws.numel(), dt, B, L, D, K,
+                                       int(bool(silu)), int(bool(accumulate)), ops._stream()), "urnn_causal_conv_backward")
+    return g
+
+
+def _seq_scratch(scratch, nbytes, dev):
+    """Scratch of a sequence operator's backward (no status words: nothing in it needs to start at zero)."""
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=dev) if scratch is None else _bwd_scratch(scratch, nbytes, dev)
+
+
+def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None, post_w=None, gate=None, scale=None, gate_act="silu",
+                           eps=ops.NORM_EPS, grads=None, accumulate=False, scratch=None):
+    """Backward of ``ops.norm_residual`` given the gradients of its two outputs (either may be None).  Returns a dict: dy, dgate, dresidual
+    (None without them), dpre_w, dpost_w, dscale (float32; None without them), as ``causal_conv_backward``."""
+    what = "norm_residual_backward"
+    dt = ops._seq_dtype(what, y)
+    strides = ops._norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act)
+    shape, D = tuple(y.shape), y.shape[-1]
+    strides += [ops._rows(what, name, t, shape, y.dtype) if t is not None else 0 for name, t in (("dnormed", dnormed), ("dresidual_out", dresidual_out))]
+    params = {"dpre_w": pre_w, "dpost_w": post_w, "dscale": scale}
+    shapes = {k: (D,) for k, w in params.items() if w is not None}
+    g, given = _param_grads_check(what, grads, accumulate, shapes)
+    ops._seq_device(what, y, pre_w, dnormed, dresidual_out, residual, post_w, gate, scale, *given)
+    L_ = lib()
+    _param_grads(g, shapes, y.device)
+    new = lambda: torch.empty(shape, dtype=y.dtype, device=y.device)      # noqa: E731
+    g["dy"], g["dgate"], g["dresidual"] = new(), new() if gate is not None else None, new() if residual is not None else None
+    rows = y.numel() // D
+    ws = _seq_scratch(scratch, L_.urnn_norm_residual_backward_workspace_bytes(rows, D), y.device)
+    p = ops._ptr
+    out = [p(g[k]) if w is not None else 0 for k, w in params.items()]
+    for k in params:
+        g.setdefault(k, None)
+    check(L_.urnn_norm_residual_backward(p(y), p(gate), p(residual), p(dnormed), p(dresidual_out), (ctypes.c_long * 5)(*strides), p(pre_w), p(post_w),
+                                         p(scale), p(g["dy"]), p(g["dgate"]), p(g["dresidual"]), *out, p(ws), ws.numel(), dt, rows, D,
+                                         ops.GATE_ACTS[gate_act], float(eps), int(bool(accumulate)), ops._stream()), "urnn_norm_residual_backward")
+    return g
