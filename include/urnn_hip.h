@@ -470,6 +470,17 @@ int urnn_selective_scan(const void *u, const void *delta, const void *Bmat, cons
                         const float *A, const float *skip, const float *delta_bias, const float *state, const int *lengths, void *y,
                         float *state_out, void *workspace, size_t workspace_bytes, int keep, int dtype, int B, int L, int D, int G,
                         int N, int softplus, void *stream);
+/* Gradients of urnn_selective_scan given dout (B,L,D) and, where state_out was used further, dstate_out (B,D,N) or NULL.  record: the
+ * workspace that the forward of the SAME inputs left with keep != 0 (read only).  du, ddelta (B,L,D), dz (B,L,D; with z only), dB, dC
+ * (B,L,G,N) contiguous in the activations' type; dstate (B,D,N) or NULL; dA (D,N), dskip (D, with skip only), ddelta_bias (D, with
+ * delta_bias only) float32, overwritten or added to (accumulate != 0).  strides: u, delta, B, C, z, dout, each (batch, token). */
+size_t urnn_selective_scan_backward_workspace_bytes(int B, int L, int D, int G, int N);
+int urnn_selective_scan_backward(const void *u, const void *delta, const void *Bmat, const void *Cmat, const void *z, const void *dout,
+                                 const long *strides, const float *A, const float *skip, const float *delta_bias, const int *lengths,
+                                 const float *dstate_out, const void *record, size_t record_bytes, void *du, void *ddelta, void *dB,
+                                 void *dC, void *dz, float *dA, float *dskip, float *ddelta_bias, float *dstate, void *workspace,
+                                 size_t workspace_bytes, int dtype, int B, int L, int D, int G, int N, int softplus, int accumulate,
+                                 void *stream);
 /* One token: u, delta, z, y (B,D), B, C (B,G,N); strides: the batch strides of u, delta, B, C, z; state_out may be state. */
 int urnn_selective_scan_step(const void *u, const void *delta, const void *Bmat, const void *Cmat, const void *z, const long *strides,
                              const float *A, const float *skip, const float *delta_bias, const float *state, void *y, float *state_out,

@@ -210,6 +210,79 @@ def test_selective_scan_step_continues_a_prompt(B, dim, N, G, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("B,L,dim,N,G,lengths,opts", SCAN)
+def test_selective_scan_backward(B, L, dim, N, G, lengths, opts, dtype):
+    c, n = scan_case(B, L, dim, N, G, dtype, 3 * L + dim, lengths=lengths, **opts)
+    g = rng(17)
+    dout, dso = make(g, B, L, dim, dtype=dtype), make(g, B, dim, N)
+    if lengths is not None:
+        poison(dout, [min(max(v, 0), L) for v in lengths])
+    ref = seq_ref.selective_scan(**c, lengths=lengths, dout=dout, dstate_out=dso)
+    ws = ops.selective_scan_workspace(c["u"], c["A"])
+    ops.selective_scan(**c, lengths=n, ws=ws)
+    held = ws.clone()
+    args = {k: v for k, v in c.items() if k != "state"}
+    got = train_ops.selective_scan_backward(**args, dout=dout, fwd_ws=ws, lengths=n, dstate_out=dso, want_dstate=True)
+    k = 2 * scan_k(c)
+    wide = {"dA", "dD", "ddelta_bias", "dstate"}
+    for name in ("dz", "dC", "du", "dB", "ddelta", "dA", "dD", "ddelta_bias", "dstate"):
+        if {"dz": c["z"], "dD": c["D"], "ddelta_bias": c["delta_bias"]}.get(name, 0) is None:
+            assert got[name] is None
+            continue
+        seq_ref.check(got[name], ref[name], k + (B * L if name in wide else 0), torch.float32 if name in wide else dtype, name)
+    assert torch.equal(ws, held)                                # the record is only read: a second backward gives the same bits
+    grads = {name: got[name].clone() for name in ("dA", "dD", "ddelta_bias") if got[name] is not None}
+    more = train_ops.selective_scan_backward(**args, dout=dout, fwd_ws=ws, lengths=n, dstate_out=dso, grads=grads, accumulate=True)
+    for name in ("du", "ddelta", "dB", "dC"):
+        assert torch.equal(more[name], got[name]), name
+    for name in ("dA", "dD", "ddelta_bias"):
+        assert got[name] is None or torch.equal(more[name], 2 * got[name]), name
+    assert more["dstate"] is None
+
+
+@gpu
+def test_selective_scan_backward_many_sequences():
+    """More sequences than blocks along the batch: one block sums several."""
+    c, n = scan_case(1100, 3, 130, 4, 1, torch.float32, 8, lengths=[3, 0, 1, 2] * 275)
+    dout = make(rng(4), 1100, 3, 130)
+    ref = seq_ref.selective_scan(**c, lengths=n.tolist(), dout=dout)
+    ws = ops.selective_scan_workspace(c["u"], c["A"])
+    ops.selective_scan(**c, lengths=n, ws=ws)
+    got = train_ops.selective_scan_backward(**{k: v for k, v in c.items() if k != "state"}, dout=dout, fwd_ws=ws, lengths=n)
+    for name in ("du", "dB", "dC", "ddelta", "dz"):
+        seq_ref.check(got[name], ref[name], 2 * scan_k(c), torch.float32, name)
+    for name in ("dA", "dD", "ddelta_bias"):                    # a block's chain of 3 x 2 tokens, then double
+        seq_ref.check(got[name], ref[name], 2 * scan_k(c), torch.float32, name)
+
+
+@gpu
+def test_selective_scan_gradients_against_differences():
+    """The sum of every gradient along a direction, against central differences of the float64 forward.  h = 1e-5: the forward's values
+    are O(10), so that rounding leaves 1e-15 * 10 / 1e-5 = 1e-9 and the third derivative about h^2; the kernels add 1e-5 of the scale."""
+    c, _ = scan_case(2, 37, 20, 8, 2, torch.float32, 21)
+    g = rng(2)
+    dout, dso = make(g, 2, 37, 20), make(g, 2, 20, 8)
+    ws = ops.selective_scan_workspace(c["u"], c["A"])
+    ops.selective_scan(**c, ws=ws)
+    got = train_ops.selective_scan_backward(**{k: v for k, v in c.items() if k != "state"}, dout=dout, fwd_ws=ws, dstate_out=dso, want_dstate=True)
+    names = {"u": "du", "delta": "ddelta", "A": "dA", "B": "dB", "C": "dC", "D": "dD", "z": "dz", "delta_bias": "ddelta_bias", "state": "dstate"}
+
+    def f(shift):
+        moved = {k: (v.double().cpu() + shift.get(k, 0.0)) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+        r = seq_ref.selective_scan(**moved)
+        return ((r["y"][0] * dout.double().cpu()).sum() + (r["state"][0] * dso.double().cpu()).sum()).item()
+
+    h = 1e-5
+    for k, dk in names.items():
+        v = torch.randn(c[k].shape, generator=g, dtype=torch.float64)
+        want = (f({k: h * v}) - f({k: -h * v})) / (2 * h)
+        have = (got[dk].double().cpu() * v).sum().item()
+        scale = (got[dk].double().cpu() * v).abs().sum().item()
+        assert abs(have - want) <= 1e-5 * scale, (k, have, want)
+
+
+@gpu
 def test_selective_scan_strides_and_ungrouped_rows():
     """u and z as halves of one projection, delta, B and C as parts of another, (batch, L, N) B and C."""
     g = rng(1)
@@ -223,6 +296,16 @@ def test_selective_scan_strides_and_ungrouped_rows():
     assert torch.equal(y, y2) and torch.equal(st, st2)
     ref = seq_ref.selective_scan(**c)
     seq_ref.check(y, ref["y"], scan_k(c), torch.bfloat16, "y")
+    dout = make(g, B, L, dim + 5, dtype=torch.bfloat16)[..., 5:]
+    ws = ops.selective_scan_workspace(c["u"], c["A"])
+    ops.selective_scan(**c, ws=ws)
+    ref = seq_ref.selective_scan(**c, dout=dout)
+    a = train_ops.selective_scan_backward(**{k: v for k, v in c.items() if k != "state"}, dout=dout, fwd_ws=ws)
+    b = train_ops.selective_scan_backward(**{k: v for k, v in flat.items() if k != "state"}, dout=dout.contiguous(), fwd_ws=ws)
+    assert a["dB"].shape == (B, L, N)
+    for k in ("du", "ddelta", "dz", "dB", "dC", "dA", "dD"):
+        assert torch.equal(a[k], b[k]), k
+    seq_ref.check(a["du"], ref["du"], 2 * scan_k(c), torch.bfloat16, "du")
     one = {k: c[k][:, 0] for k in ("u", "delta", "B", "C", "z")}
     a, ha = ops.selective_scan_step(**{**c, **one})
     b, hb = ops.selective_scan_step(**{**c, **{k: v.contiguous() for k, v in one.items()}})
@@ -382,6 +465,14 @@ def test_refusals_selective_scan():
     refused("out overlaps an input", ops.selective_scan, **c, out=c["u"])
     refused("out must be contiguous", ops.selective_scan, **c, out=torch.zeros(2, 8, 5).transpose(1, 2))
     refused("state_out overlaps an input", ops.selective_scan, **c, want_state=True, state_out=c["state"])
+    back = {k: v for k, v in c.items() if k != "state"}
+    ws = torch.zeros(1 << 16, dtype=torch.uint8)
+    refused("no CPU path", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws)
+    refused("fwd_ws is None", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=None)
+    refused("dout has shape", train_ops.selective_scan_backward, **back, dout=c["u"][:, :2], fwd_ws=ws)
+    refused("dstate_out is torch.bfloat16", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, dstate_out=c["state"].bfloat16())
+    refused("accumulate needs", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, accumulate=True, grads={"dA": c["A"]})
+    refused("dA has shape", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, grads={"dA": c["A"][:4]})
     refused("state is None", ops.selective_scan_step, **{**step, "state": None})
     refused("state_out is torch.bfloat16", ops.selective_scan_step, **step, state_out=c["state"].bfloat16())
 

@@ -1628,7 +1628,7 @@ struct ScanWork { size_t keep, sum, S, total; };
 static ScanWork scan_work(int B, int L, int D, int N, int keep)
 {
     int CL;
-    const size_t np = urnn_scan_np(N), chunks = urnn_scan_chunks(B, L, D, &CL), segs = (L + URNN_SCAN_CK - 1) / URNN_SCAN_CK;
+    const size_t np = urnn_scan_np(N), chunks = urnn_scan_chunks(B, L, D, &CL), ck = urnn_scan_ck((int)np), segs = (L + ck - 1) / ck;
     ScanWork w;
     w.keep = 0;
     w.sum = keep ? align_up((size_t)B * segs * D * np * sizeof(float), 256) : 0;
@@ -1667,6 +1667,64 @@ extern "C" int urnn_selective_scan(const void *u, const void *delta, const void 
     p.batch = B; p.L = L; p.dim = D; p.N = N; p.G = G; p.softplus = softplus;
     p.chunks = urnn_scan_chunks(B, L, D, &p.CL);
     CHECK_HIP(urnn_launch_scan(p, dtype, (hipStream_t)stream), "selective_scan");
+    return URNN_OK;
+}
+
+// Backward workspace: [sums of steps][chunk hand-overs][dB, dC of the channel blocks][dA][dskip][ddelta_bias of the parts]
+struct ScanBackWork { size_t sum, S, dB, dC, dA, dD, db, total; int chunks, CL, slots; };
+static ScanBackWork scan_back_work(int B, int L, int D, int G, int N)
+{
+    ScanBackWork w;
+    w.chunks = urnn_scan_backward_chunks(B, L, D, N, &w.CL, &w.slots);
+    const size_t np = urnn_scan_np(N), cb = 64 * urnn_scan_ed((int)np), gcbs = (D / G + cb - 1) / cb, parts = (size_t)w.slots * w.chunks;
+    const size_t rows = align_up(gcbs * B * L * G * N * sizeof(float), 256), cross = w.chunks > 1 ? w.chunks : 0;
+    w.sum = 0;
+    w.S = align_up((size_t)B * cross * D * sizeof(float), 256);
+    w.dB = w.S + align_up((size_t)B * cross * D * np * sizeof(float), 256);
+    w.dC = w.dB + rows;
+    w.dA = w.dC + rows;
+    w.dD = w.dA + align_up(parts * D * N * sizeof(float), 256);
+    w.db = w.dD + align_up(parts * D * sizeof(float), 256);
+    w.total = w.db + align_up(parts * D * sizeof(float), 256);
+    return w;
+}
+
+extern "C" size_t urnn_selective_scan_backward_workspace_bytes(int B, int L, int D, int G, int N)
+{
+    if (B < 1 || L < 1 || D < 1 || G < 1 || D % G || N < 1 || N > URNN_SEQ_MAX_STATES) return 0;
+    return scan_back_work(B, L, D, G, N).total;
+}
+
+extern "C" int urnn_selective_scan_backward(const void *u, const void *delta, const void *Bmat, const void *Cmat, const void *z, const void *dout,
+                                            const long *strides, const float *A, const float *skip, const float *delta_bias, const int *lengths,
+                                            const float *dstate_out, const void *record, size_t record_bytes, void *du, void *ddelta, void *dB,
+                                            void *dC, void *dz, float *dA, float *dskip, float *ddelta_bias, float *dstate, void *workspace,
+                                            size_t workspace_bytes, int dtype, int B, int L, int D, int G, int N, int softplus, int accumulate,
+                                            void *stream)
+{
+    const int rc = scan_args("urnn_selective_scan_backward", dtype, B, L, D, G, N);
+    if (rc) return rc;
+    if (!u || !delta || !Bmat || !Cmat || !dout || !strides || !A || !record || !du || !ddelta || !dB || !dC || !dA || !workspace || (z && !dz))
+        return fail(URNN_ENULL, "urnn_selective_scan_backward: NULL argument");
+    if (!aligned16(workspace) || !aligned16(record)) return fail(URNN_EALIGN, "urnn_selective_scan_backward: workspace / record not 16-byte aligned");
+    const ScanWork f = scan_work(B, L, D, N, 1);
+    if (record_bytes < f.total) return fail(URNN_EWORKSPACE, "urnn_selective_scan_backward: the record is too small for a forward with keep");
+    const ScanBackWork w = scan_back_work(B, L, D, G, N);
+    if (workspace_bytes < w.total) return fail(URNN_EWORKSPACE, "urnn_selective_scan_backward: workspace too small");
+    char *base = reinterpret_cast<char *>(workspace);
+    ScanParams p = {};
+    p.u = u; p.delta = delta; p.B = Bmat; p.C = Cmat; p.z = z; p.dout = dout;
+    p.su = {strides[0], strides[1]}; p.sd = {strides[2], strides[3]}; p.sB = {strides[4], strides[5]}; p.sC = {strides[6], strides[7]};
+    p.sz = {strides[8], strides[9]}; p.so = {strides[10], strides[11]};
+    p.A = A; p.D = skip; p.bias = delta_bias; p.lengths = lengths; p.dstate_out = dstate_out;
+    p.keep = const_cast<float *>(reinterpret_cast<const float *>(record)) + f.keep / sizeof(float);
+    p.sum = reinterpret_cast<float *>(base + w.sum); p.S = reinterpret_cast<float *>(base + w.S);
+    p.dBp = reinterpret_cast<float *>(base + w.dB); p.dCp = reinterpret_cast<float *>(base + w.dC);
+    p.dAp = reinterpret_cast<float *>(base + w.dA); p.dDp = reinterpret_cast<float *>(base + w.dD); p.dbp = reinterpret_cast<float *>(base + w.db);
+    p.du = du; p.ddelta = ddelta; p.dz = dz; p.dstate = dstate;
+    p.batch = B; p.L = L; p.dim = D; p.N = N; p.G = G; p.softplus = softplus;
+    p.chunks = w.chunks; p.CL = w.CL; p.slots = w.slots;
+    CHECK_HIP(urnn_launch_scan_backward(p, dtype, dA, dskip, ddelta_bias, dB, dC, accumulate, (hipStream_t)stream), "selective_scan_backward");
     return URNN_OK;
 }
 

@@ -17,56 +17,12 @@
 // from its true state.  The first pass costs all exponentials once more (7 of the full pass's ~11 issue slots per state).
 #include "urnn_seq.h"
 
-template <int E>
-__device__ __forceinline__ void load_states(const float *row, int q, int N, bool vec, float (&v)[E])
-{
-    constexpr int W = E < 4 ? E : 4;
-#pragma unroll
-    for (int e = 0; e < E; e += W) {
-        const int n = q * E + e;
-        if (vec) {                                   // N % W == 0: a group of W states is inside or outside as a whole
-            Pack<float, W> t = {};
-            if (n < N) t = *reinterpret_cast<const Pack<float, W> *>(row + n);
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[e + i] = t.v[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[e + i] = n + i < N ? row[n + i] : 0.0f;
-        }
-    }
-}
-
-template <int E>
-__device__ __forceinline__ void store_states(float *row, int q, int N, bool vec, const float (&v)[E])
-{
-    constexpr int W = E < 4 ? E : 4;
-#pragma unroll
-    for (int e = 0; e < E; e += W) {
-        const int n = q * E + e;
-        if (vec) {
-            Pack<float, W> t;
-#pragma unroll
-            for (int i = 0; i < W; ++i) t.v[i] = v[e + i];
-            if (n < N) *reinterpret_cast<Pack<float, W> *>(row + n) = t;
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (n + i < N) row[n + i] = v[e + i];
-        }
-    }
-}
-
-__device__ __forceinline__ bool states_vec(const void *a, int N, int W)
-{
-    return N % W == 0 && (reinterpret_cast<uintptr_t>(a) & (W * sizeof(float) - 1)) == 0;
-}
-
 enum { SCAN_STATES = 0, SCAN_FULL = 1 };
 
 template <typename T, int NP, int MODE>
 __global__ __launch_bounds__(256) void scan_kernel(const ScanParams p)
 {
-    constexpr int E = NP / 4, W = E < 4 ? E : 4, TT = 32, CB = URNN_SCAN_CB, R = TT * CB / 256, RB = TT * NP / 256 < 1 ? 1 : TT * NP / 256;
+    constexpr int E = NP / 4, W = E < 4 ? E : 4, TT = 32, CK = urnn_scan_ck(NP), CB = URNN_SCAN_CB, R = TT * CB / 256, RB = TT * NP / 256 < 1 ? 1 : TT * NP / 256;
     __shared__ alignas(16) Pack<float, 2> s_in[TT * CB];         // (step, step * u)
     __shared__ alignas(16) float s_B[TT * NP];
     __shared__ alignas(16) float s_C[MODE == SCAN_FULL ? TT * NP : 4];
@@ -166,9 +122,9 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanParams p)
             }
             return y0;
         };
-        auto checkpoint = [&](int t) {                           // the state before token t0 + t, t a multiple of URNN_SCAN_CK
+        auto checkpoint = [&](int t) {                           // the state before token t0 + t, t a multiple of CK
             if (MODE == SCAN_FULL && p.keep && sok) {
-                const long seg = (t0 + t) / URNN_SCAN_CK, segs = (p.L + URNN_SCAN_CK - 1) / URNN_SCAN_CK;
+                const long seg = (t0 + t) / CK, segs = (p.L + CK - 1) / CK;
                 float *k = p.keep + (((long)b * segs + seg) * p.dim + sch) * NP + q * E;
 #pragma unroll
                 for (int e = 0; e < E; e += W) {
@@ -181,7 +137,7 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanParams p)
         };
         int t = 0;
         for (; t + 4 <= nt; t += 4) {
-            if (t % URNN_SCAN_CK == 0) checkpoint(t);
+            if (t % CK == 0) checkpoint(t);
             float mine = 0.0f;                                   // lane q of the quad keeps token t + q
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -194,7 +150,7 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanParams p)
             if (MODE == SCAN_FULL) s_y[(t + q) * CB + sc] = mine;
         }
         for (; t < nt; ++t) {
-            if (t % URNN_SCAN_CK == 0) checkpoint(t);
+            if (t % CK == 0) checkpoint(t);
             const float yj = token(t);
             if (MODE == SCAN_FULL) {
                 const float s = quad_sum(yj);

@@ -60,6 +60,52 @@ struct SeqStride { long b, t; };
 
 enum { URNN_SEQ_MAX_STATES = 64, URNN_SEQ_MAX_TAPS = 4, URNN_SEQ_MAX_NORM = 16384 };
 
+// A quad's share of a row of N states: lane q holds states q E .. q E + E - 1, those beyond N as zeros.  vec: the row's W-wide
+// accesses are aligned and inside or outside as a whole (states_vec).
+template <int E>
+__device__ __forceinline__ void load_states(const float *row, int q, int N, bool vec, float (&v)[E])
+{
+    constexpr int W = E < 4 ? E : 4;
+#pragma unroll
+    for (int e = 0; e < E; e += W) {
+        const int n = q * E + e;
+        if (vec) {                                   // N % W == 0: a group of W states is inside or outside as a whole
+            Pack<float, W> t = {};
+            if (n < N) t = *reinterpret_cast<const Pack<float, W> *>(row + n);
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[e + i] = t.v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[e + i] = n + i < N ? row[n + i] : 0.0f;
+        }
+    }
+}
+
+template <int E>
+__device__ __forceinline__ void store_states(float *row, int q, int N, bool vec, const float (&v)[E])
+{
+    constexpr int W = E < 4 ? E : 4;
+#pragma unroll
+    for (int e = 0; e < E; e += W) {
+        const int n = q * E + e;
+        if (vec) {
+            Pack<float, W> t;
+#pragma unroll
+            for (int i = 0; i < W; ++i) t.v[i] = v[e + i];
+            if (n < N) *reinterpret_cast<Pack<float, W> *>(row + n) = t;
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (n + i < N) row[n + i] = v[e + i];
+        }
+    }
+}
+
+__device__ __forceinline__ bool states_vec(const void *a, int N, int W)
+{
+    return N % W == 0 && (reinterpret_cast<uintptr_t>(a) & (W * sizeof(float) - 1)) == 0;
+}
+
 // ---- selective scan --------------------------------------------------------------------------------------------------
 struct ScanParams {
     const void *u, *delta, *B, *C, *z, *dout;        // (B,L,D), B / C (B,L,G,N)
@@ -74,21 +120,28 @@ struct ScanParams {
     float *S;                                        // ... and the state of a chunk that starts from zero [B][chunks][D][NP]
     int batch, L, dim, N, G, chunks, CL, softplus;
     // backward
+    int slots;                                       // blocks along the batch
     const float *dstate_out;                         // (B,D,N) or NULL
     void *du, *ddelta, *dz;                          // (B,L,D) contiguous
     float *dstate;                                   // (B,D,N) or NULL
     float *dBp, *dCp;                                // per channel block: [blocks of a group][B][L][G][N]
-    float *dAp, *dDp, *dbp;                          // per (batch slot, chunk): [parts][D][NP], [parts][D], [parts][D]
+    float *dAp, *dDp, *dbp;                          // per (batch slot, chunk): [parts][D][N], [parts][D], [parts][D]
 };
 
-#define URNN_SCAN_CK 8      // tokens between two checkpoints of the state
-#define URNN_SCAN_CB 64     // channels of a block
+#define URNN_SCAN_CB 64     // channels of a forward block
+
+// Tokens between two checkpoints of the state: what the backward holds in registers of decays and states at a time, 2 CK NP / 4 (x 2
+// channels up to 16 states).
+__host__ __device__ static constexpr int urnn_scan_ck(int np) { return np == 64 ? 4 : 8; }
+__host__ __device__ static constexpr int urnn_scan_ed(int np) { return np <= 16 ? 2 : 1; }    // channels of a backward lane
 
 static inline int urnn_scan_np(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 hipError_t urnn_launch_scan(const ScanParams &p, int dtype, hipStream_t st);
 hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st);
 int urnn_scan_chunks(int B, int L, int D, int *CL);
+hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, void *dB, void *dC, int accumulate, hipStream_t st);
+int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots);
 
 // ---- short causal convolution ----------------------------------------------------------------------------------------
 struct ConvSeqParams {

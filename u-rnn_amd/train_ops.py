@@ -273,3 +273,52 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
                                          p(scale), p(g["dy"]), p(g["dgate"]), p(g["dresidual"]), *out, p(ws), ws.numel(), dt, rows, D,
                                          ops.GATE_ACTS[gate_act], float(eps), int(bool(accumulate)), ops._stream()), "urnn_norm_residual_backward")
     return g
+
+
+def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, delta_bias=None, softplus=True, lengths=None, dstate_out=None,
+                            want_dstate=False, grads=None, accumulate=False, scratch=None):
+    """Backward of ``ops.selective_scan`` given dout (batch,L,dim) and, where the returned state was used further, ``dstate_out``
+    (batch,dim,N).  ``fwd_ws``: the buffer that the forward of the SAME inputs ran with (``ws=``, untouched since; an Arena hands out the
+    forward's): it holds the states the gradients need, the initial one among them.  Returns a dict: du, ddelta, dB, dC, dz in the
+    activations' type and B's shape, dA, dD, ddelta_bias float32 (into the buffers of ``grads`` if given, added to them with ``accumulate``),
+    dstate float32 with ``want_dstate``; None where there is no such input."""
+    what = "selective_scan_backward"
+    dt = ops._seq_dtype(what, u)
+    if u.dim() != 3:
+        raise RuntimeError(f"{what}: u has shape {tuple(u.shape)}, expected (batch, L, dim)")
+    nb, L = u.shape[0], u.shape[1]
+    b_shape, c_shape = tuple(B.shape), tuple(C.shape)
+    dim, G, N, B, C = ops._scan_check(what, u, delta, A, B, C, D, z, delta_bias, (nb, L))
+    ops._seq_check(what, "dout", dout, (nb, L, dim), u.dtype)
+    ops._lengths_check(what, lengths, nb)
+    if dstate_out is not None:
+        ops._seq_check(what, "dstate_out", dstate_out, (nb, dim, N), torch.float32, contiguous=True)
+    if fwd_ws is None:
+        raise RuntimeError(f"{what}: fwd_ws is None: run the forward with ws=ops.selective_scan_workspace(u, A)")
+    shapes = {"dA": (dim, N)}
+    if D is not None:
+        shapes["dD"] = (dim,)
+    if delta_bias is not None:
+        shapes["ddelta_bias"] = (dim,)
+    g, given = _param_grads_check(what, grads, accumulate, shapes)
+    ops._seq_device(what, u, delta, A, B, C, D, z, delta_bias, dout, lengths, dstate_out, *given)
+    L_ = lib()
+    record = ops._scratch(fwd_ws, L_.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1), u.device, key="scan")
+    ops._seq_device(what, u, record)
+    _param_grads(g, shapes, u.device)
+    g.setdefault("dD", None)
+    g.setdefault("ddelta_bias", None)
+    new = lambda shape: torch.empty(shape, dtype=u.dtype, device=u.device)      # noqa: E731
+    g["du"], g["ddelta"], g["dB"], g["dC"] = new(u.shape), new(u.shape), new(b_shape), new(c_shape)
+    g["dz"] = new(u.shape) if z is not None else None
+    g["dstate"] = torch.empty((nb, dim, N), dtype=torch.float32, device=u.device) if want_dstate else None
+    ws = _seq_scratch(scratch, L_.urnn_selective_scan_backward_workspace_bytes(nb, L, dim, G, N), u.device)
+    p = ops._ptr
+    strides = (ctypes.c_long * 12)(*u.stride()[:2], *delta.stride()[:2], *B.stride()[:2], *C.stride()[:2], *(z.stride()[:2] if z is not None else (0, 0)),
+                                   *dout.stride()[:2])
+    check(L_.urnn_selective_scan_backward(p(u), p(delta), p(B), p(C), p(z), p(dout), strides, p(A), p(D), p(delta_bias), p(lengths), p(dstate_out),
+                                          p(record), record.numel(), p(g["du"]), p(g["ddelta"]), p(g["dB"]), p(g["dC"]), p(g["dz"]), p(g["dA"]),
+                                          p(g["dD"]) if D is not None else 0, p(g["ddelta_bias"]) if delta_bias is not None else 0, p(g["dstate"]),
+                                          p(ws), ws.numel(), dt, nb, L, dim, G, N, int(bool(softplus)), int(bool(accumulate)), ops._stream()),
+          "urnn_selective_scan_backward")
+    return g
