@@ -1670,8 +1670,8 @@ extern "C" int urnn_selective_scan(const void *u, const void *delta, const void 
     return URNN_OK;
 }
 
-// Backward workspace: [sums of steps][chunk hand-overs][dB, dC of the channel blocks][dA][dskip][ddelta_bias of the parts]
-struct ScanBackWork { size_t sum, S, dB, dC, dA, dD, db, total; int chunks, CL, slots; };
+// Backward workspace: [sums of steps][chunk hand-overs][dB, dC of the channel blocks][dA | dskip | ddelta_bias of the parts]
+struct ScanBackWork { size_t sum, S, dB, dC, sums, total; int chunks, CL, slots; };
 static ScanBackWork scan_back_work(int B, int L, int D, int G, int N)
 {
     ScanBackWork w;
@@ -1682,10 +1682,8 @@ static ScanBackWork scan_back_work(int B, int L, int D, int G, int N)
     w.S = align_up((size_t)B * cross * D * sizeof(float), 256);
     w.dB = w.S + align_up((size_t)B * cross * D * np * sizeof(float), 256);
     w.dC = w.dB + rows;
-    w.dA = w.dC + rows;
-    w.dD = w.dA + align_up(parts * D * N * sizeof(float), 256);
-    w.db = w.dD + align_up(parts * D * sizeof(float), 256);
-    w.total = w.db + align_up(parts * D * sizeof(float), 256);
+    w.sums = w.dC + rows;
+    w.total = w.sums + align_up(parts * D * (N + 2) * sizeof(float), 256);
     return w;
 }
 
@@ -1720,10 +1718,13 @@ extern "C" int urnn_selective_scan_backward(const void *u, const void *delta, co
     p.keep = const_cast<float *>(reinterpret_cast<const float *>(record)) + f.keep / sizeof(float);
     p.sum = reinterpret_cast<float *>(base + w.sum); p.S = reinterpret_cast<float *>(base + w.S);
     p.dBp = reinterpret_cast<float *>(base + w.dB); p.dCp = reinterpret_cast<float *>(base + w.dC);
-    p.dAp = reinterpret_cast<float *>(base + w.dA); p.dDp = reinterpret_cast<float *>(base + w.dD); p.dbp = reinterpret_cast<float *>(base + w.db);
+    p.dAp = reinterpret_cast<float *>(base + w.sums);
     p.du = du; p.ddelta = ddelta; p.dz = dz; p.dstate = dstate;
     p.batch = B; p.L = L; p.dim = D; p.N = N; p.G = G; p.softplus = softplus;
     p.chunks = w.chunks; p.CL = w.CL; p.slots = w.slots;
+    const int e = seq_elem(dtype);
+    p.wide = wide_rows(u, strides[0], strides[1], e) && wide_rows(delta, strides[2], strides[3], e) && wide_rows(z, strides[8], strides[9], e) &&
+             wide_rows(dout, strides[10], strides[11], e) && (long)D / G * e % 16 == 0 && aligned16(du) && aligned16(ddelta) && (!z || aligned16(dz));
     CHECK_HIP(urnn_launch_scan_backward(p, dtype, dA, dskip, ddelta_bias, dB, dC, accumulate, (hipStream_t)stream), "selective_scan_backward");
     return URNN_OK;
 }

@@ -246,25 +246,41 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(cons
     put(2, cs);
 }
 
-// out[i] (+)= sum over parts of src[part * stride + i], in double: 64 columns and four lanes of parts per block.
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float *__restrict__ src, long stride, int parts, long n, float *out, int accumulate)
+// 16 columns and 64 lanes of parts to a block, eight loads of a lane in flight: the sums are short and there are few of them.
+struct SumOut { float *p[3]; long end[3]; };
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float *__restrict__ src, int parts, long n, SumOut out, int accumulate)
 {
-    __shared__ double s[4][64];
-    const long i = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int r = threadIdx.x >> 6;
+    __shared__ double s[64][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const long i = (long)blockIdx.x * 16 + c;
     double a = 0.0;
-    if (i < n)
-        for (int t = r; t < parts; t += 4) a += (double)src[t * stride + i];
-    s[r][threadIdx.x & 63] = a;
-    __syncthreads();
+    if (i < n) {
+        int t = r;
+        for (; t + 7 * 64 < parts; t += 8 * 64) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = src[(long)(t + 64 * k) * n + i];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) a += (double)v[k];
+        }
+        for (; t < parts; t += 64) a += (double)src[(long)t * n + i];
+    }
+    s[r][c] = a;
+    for (int w = 32; w >= 1; w >>= 1) {
+        __syncthreads();
+        if (r < w) s[r][c] += s[r + w][c];
+    }
     if (r || i >= n) return;
-    const int l = threadIdx.x;
-    const float v = (float)((s[0][l] + s[1][l]) + (s[2][l] + s[3][l]));
-    out[i] = accumulate ? out[i] + v : v;
+    const int k = i < out.end[0] ? 0 : i < out.end[1] ? 1 : 2;
+    if (!out.p[k]) return;
+    float *o = out.p[k] + (i - (k ? out.end[k - 1] : 0));
+    *o = (accumulate ? *o : 0.0f) + (float)s[0][c];
 }
-hipError_t urnn_launch_sum_parts(const float *src, long stride, int parts, long n, float *out, int accumulate, hipStream_t st)
+hipError_t urnn_launch_sum_parts(const float *src, int parts, const long (&n)[3], float *const (&out)[3], int accumulate, hipStream_t st)
 {
-    sum_parts_kernel<<<dim3((unsigned)((n + 63) / 64)), 256, 0, st>>>(src, stride, parts, n, out, accumulate);
+    const long all = n[0] + n[1] + n[2];
+    const SumOut o = {{out[0], out[1], out[2]}, {n[0], n[0] + n[1], all}};
+    sum_parts_kernel<<<dim3((unsigned)((all + 15) / 16)), 1024, 0, st>>>(src, parts, all, o, accumulate);
     return hipGetLastError();
 }
 
@@ -308,7 +324,7 @@ hipError_t urnn_launch_norm_backward(const NormParams &p, int dtype, bool wide, 
 {
     hipError_t e = by_type(p, dtype, wide, true, st);
     float *const outs[3] = {dpre, dpost, dscale};
-    for (int k = 0; k < 3 && e == hipSuccess; ++k)
-        if (outs[k]) e = urnn_launch_sum_parts(p.partial + (long)k * p.dim, 3l * p.dim, p.parts, p.dim, outs[k], accumulate, st);
+    const long sizes[3] = {p.dim, p.dim, p.dim};
+    if (e == hipSuccess) e = urnn_launch_sum_parts(p.partial, p.parts, sizes, outs, accumulate, st);
     return e;
 }

@@ -1,197 +1,160 @@
-// urnn_scan.hip -- selective state space scan, forward:
+// urnn_scan.hip -- selective state space scan, forward and single token:
 //   step_t = softplus(delta_t + bias)                      (or delta_t + bias)
 //   h_t[n] = exp(step_t A[n]) h_(t-1)[n] + step_t u_t B_t[n]
 //   y_t    = (sum_n C_t[n] h_t[n] + D u_t) * silu(z_t)
 // per channel; B and C are shared by the channels of a group.
 //
-// Mapping.  A channel's NP (padded) states lie on the four lanes of a quad, E = NP / 4 in each lane's registers, so that the state
-// never leaves them along the whole sequence; a wave holds 16 channels, a block of four waves 64.  Tokens pass in tiles of 32: the
-// block turns a tile's inputs into fp32 (step, step * u) pairs and fp32 rows of B and C in LDS with whole-line loads (64 channels of
-// a token are adjacent), then every wave walks the tile's tokens: per token one 8-byte and 2 E 4-byte LDS reads per lane, and per
-// state one exponential (quarter rate) and four fp32 operations.  y is summed over the quad with two DPP adds, and gate, skip and
-// store are done for the whole tile again.  The inputs of the next tile are in flight while a tile is walked.
+// Mapping.  A lane is a channel: all of its states stay in registers along the sequence, the sum over states needs no other lane, and
+// the elementwise work (softplus, gate, conversions) is done once.  A wave is 64 adjacent channels of one sequence -- whole 128-byte
+// lines of a 16-bit row per access -- and a block of its own, so that nothing waits for another wave.  B and C rows pass through
+// LDS as fp32, 16 tokens at a time, and are read by all lanes at once; inputs of the next four tokens and the next tile's rows are in
+// flight meanwhile.  What bounds it is the vector unit: per state one exponential (measured: the time of 1.6 to 2 fp32 operations) and
+// four fp32 operations, per token and channel about 45 more.
 //
-// Few long sequences do not fill the chip with B * D / 64 blocks: the time axis is cut into chunks (urnn_scan_chunks).  The recurrence
+// Few long sequences do not fill the chip with B * D / 64 waves: the time axis is cut into chunks (urnn_scan_chunks).  The recurrence
 // is linear, h_end = P h_begin + S with S the state of a chunk that starts from zero and P = exp(A * sum of its steps): one pass
 // leaves (S, sum of steps) of every chunk, a short kernel carries the states over the chunks, and the full pass starts each chunk
-// from its true state.  The first pass costs all exponentials once more (7 of the full pass's ~11 issue slots per state).
+// from its true state.  The first pass costs the exponentials once more.  The same kernel, run from the last token to the first, gives
+// the backward its chunk summaries.
 #include "urnn_seq.h"
 
-enum { SCAN_STATES = 0, SCAN_FULL = 1 };
+#include <type_traits>
 
 template <typename T, int NP, int MODE>
-__global__ __launch_bounds__(256) void scan_kernel(const ScanParams p)
+__global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
 {
-    constexpr int E = NP / 4, W = E < 4 ? E : 4, TT = 32, CK = urnn_scan_ck(NP), CB = URNN_SCAN_CB, R = TT * CB / 256, RB = TT * NP / 256 < 1 ? 1 : TT * NP / 256;
-    __shared__ alignas(16) Pack<float, 2> s_in[TT * CB];         // (step, step * u)
-    __shared__ alignas(16) float s_B[TT * NP];
-    __shared__ alignas(16) float s_C[MODE == SCAN_FULL ? TT * NP : 4];
-    __shared__ float s_y[MODE == SCAN_FULL ? TT * CB : 1];
-    const int tid = threadIdx.x, lane = tid & 63, q = lane & 3;
+    constexpr int TT = 16, TPI = 64 / NP, RB = TT / TPI, CK = urnn_scan_ck(NP), CB = URNN_SCAN_CB, G4 = 4;
+    constexpr bool FULL = MODE == SCAN_FULL, BACK = MODE == SCAN_BACK;
+    __shared__ alignas(16) float s_B[TT * NP];                   // BACK: the rows of C
+    __shared__ alignas(16) float s_C[FULL ? TT * NP : 4];
+    const int lane = threadIdx.x;
     const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
-    const int walked = MODE == SCAN_STATES ? p.chunks - 1 : p.chunks;           // nothing reads the last chunk's summary
-    const int chunk = blockIdx.x / (cbs * p.G) % walked, b = blockIdx.x / (cbs * p.G) / walked;
+    const int walked = FULL ? p.chunks : p.chunks - 1;           // nothing reads the summary of the last chunk (BACK: the first)
+    const int chunk = (BACK ? 1 : 0) + blockIdx.x / (cbs * p.G) % walked, b = blockIdx.x / (cbs * p.G) / walked;
     const int len = seq_len(p.lengths, b, p.L);
-    const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L;
-    const long te = tfull < len ? tfull : len;
-    const T *u = reinterpret_cast<const T *>(p.u) + b * p.su.b, *dl = reinterpret_cast<const T *>(p.delta) + b * p.sd.b;
-    const T *z = p.z ? reinterpret_cast<const T *>(p.z) + b * p.sz.b : nullptr;
-    const T *Bp = reinterpret_cast<const T *>(p.B) + b * p.sB.b + (long)g * p.N, *Cp = reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N;
-    T *y = reinterpret_cast<T *>(p.y) + (long)b * p.L * p.dim;
+    const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L, te = tfull < len ? tfull : len;
+    const int n = te > tb ? (int)(te - tb) : 0;                  // tokens to walk; token i is first + dir i
+    const long first = BACK ? te - 1 : tb, dir = BACK ? -1 : 1;
+    const bool ok = c0 + lane < cend;
+    const int ch = ok ? c0 + lane : c0;                          // lanes beyond the group repeat its block's first channel
+    // u; BACK: dout
+    const T *u = BACK ? reinterpret_cast<const T *>(p.dout) + b * p.so.b + ch : reinterpret_cast<const T *>(p.u) + b * p.su.b + ch;
+    const T *dl = reinterpret_cast<const T *>(p.delta) + b * p.sd.b + ch;
+    const bool gated = MODE != SCAN_STATES && p.z != nullptr;
+    const T *z = gated ? reinterpret_cast<const T *>(p.z) + b * p.sz.b + ch : dl;
+    const long ut = BACK ? p.so.t : p.su.t, zt = gated ? p.sz.t : p.sd.t;
+    const int rt = lane / NP, rn = lane % NP;                    // rows: token rt, state rn of every TPI tokens
+    const T *Bp = reinterpret_cast<const T *>(BACK ? p.C : p.B) + b * (BACK ? p.sC.b : p.sB.b) + (long)g * p.N + (rn < p.N ? rn : 0);
+    const T *Cp = reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N + (rn < p.N ? rn : 0);
+    const long Bt = BACK ? p.sC.t : p.sB.t;
+    T *y = reinterpret_cast<T *>(p.y) + (long)b * p.L * p.dim + ch;
+    const float bias = p.bias ? p.bias[ch] : 0.0f, skip = p.D ? p.D[ch] : 0.0f;
+    const bool sp = p.softplus != 0;
 
-    // the elementwise role: channel lc of the block, tokens lt + 4 i of a tile
-    const int lc = tid & 63, lt = tid >> 6, ech = c0 + lc;
-    const bool eok = ech < cend;
-    const float bias = p.bias && eok ? p.bias[ech] : 0.0f, skip = p.D && eok ? p.D[ech] : 0.0f;
-    // the scan role: channel sch, states q E .. q E + E - 1
-    const int sc = tid >> 2, sch = c0 + sc;
-    const bool sok = sch < cend;
-    const int rch = sok ? sch : c0;
-    const bool vA = states_vec(p.A, p.N, W);
-    float A2[E], h[E];
-    load_states<E>(p.A + (long)rch * p.N, q, p.N, vA, A2);
+    float A2[NP], h[NP];
+    load_states<NP>(p.A + (long)ch * p.N, 0, p.N, states_vec(p.A, p.N, 4), A2);
 #pragma unroll
-    for (int e = 0; e < E; ++e) { A2[e] *= URNN_LOG2E; h[e] = 0.0f; }
-    if (MODE == SCAN_FULL && chunk > 0) {
-        const float *s = p.S + (((long)b * p.chunks + chunk - 1) * p.dim + rch) * NP + q * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[e] = s[e];
-    } else if (p.state && chunk == 0) {
-        load_states<E>(p.state + ((long)b * p.dim + rch) * p.N, q, p.N, states_vec(p.state, p.N, W), h);
-    }
-    float total = 0.0f;                                          // STATES: this thread's share of the chunk's sum of steps
+    for (int k = 0; k < NP; ++k) { A2[k] *= URNN_LOG2E; h[k] = 0.0f; }
+    if (FULL && chunk > 0) load_states<NP>(p.S + (((long)b * p.chunks + chunk - 1) * p.dim + ch) * NP, 0, NP, true, h);
+    else if (!BACK && p.state && chunk == 0) load_states<NP>(p.state + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state, p.N, 4), h);
+    float total = 0.0f;                                          // summaries: the chunk's sum of steps
 
-    T ru[R] = {}, rd[R] = {}, rz[R] = {}, rB[RB] = {}, rC[RB] = {};
-    auto fetch = [&](long t0) {
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const long t = t0 + lt + 4 * i;
-            if (eok && t < te) {
-                ru[i] = u[t * p.su.t + ech];
-                rd[i] = dl[t * p.sd.t + ech];
-                if (MODE == SCAN_FULL && z) rz[i] = z[t * p.sz.t + ech];
-            }
-        }
+    T rB[RB], rC[RB], fu[G4], fd[G4], fz[G4];
+    auto fetch_rows = [&](int i0) {
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
-            const int k = tid + 256 * i, n = k % NP;
-            const long t = t0 + k / NP;
-            rB[i] = rC[i] = T(0.0f);
-            if (k < TT * NP && n < p.N && t < te) {
-                rB[i] = Bp[t * p.sB.t + n];
-                if (MODE == SCAN_FULL) rC[i] = Cp[t * p.sC.t + n];
-            }
+            int k = i0 + i * TPI + rt;
+            k = k < n ? k : n - 1;
+            rB[i] = Bp[(first + dir * k) * Bt];
+            if (FULL) rC[i] = Cp[(first + dir * k) * p.sC.t];
         }
     };
-    if (tb < te) fetch(tb);
-    for (long t0 = tb; t0 < te; t0 += TT) {
-        const int nt = te - t0 < TT ? (int)(te - t0) : TT;
-        T cu[R], cz[R];
+    auto fetch_tokens = [&](int i0) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const float raw = to_f(rd[i]) + bias, step = p.softplus ? softplus_f(raw) : raw, uf = to_f(ru[i]);
-            s_in[(lt + 4 * i) * CB + lc] = {{step, step * uf}};
-            if (MODE == SCAN_STATES && lt + 4 * i < nt) total += step;
-            cu[i] = ru[i];
-            cz[i] = rz[i];
+        for (int j = 0; j < G4; ++j) {
+            const int k = i0 + j < n ? i0 + j : n - 1;
+            const long t = first + dir * k;
+            fu[j] = u[t * ut];
+            fd[j] = dl[t * p.sd.t];
+            if (MODE != SCAN_STATES) fz[j] = z[t * zt];
         }
+    };
+    if (n > 0) {
+        fetch_rows(0);
+        fetch_tokens(0);
+    }
+    for (int i0 = 0; i0 < n; i0 += TT) {
+        const int nt = n - i0 < TT ? n - i0 : TT;
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
-            const int k = tid + 256 * i;
-            if (k < TT * NP) {
-                s_B[k] = to_f(rB[i]);
-                if (MODE == SCAN_FULL) s_C[k] = to_f(rC[i]);
+            s_B[(i * TPI) * NP + lane] = rn < p.N ? to_f(rB[i]) : 0.0f;
+            if (FULL) s_C[(i * TPI) * NP + lane] = rn < p.N ? to_f(rC[i]) : 0.0f;
+        }
+        __syncthreads();
+        if (i0 + TT < n) fetch_rows(i0 + TT);
+        for (int i = 0; i < nt; i += G4) {
+            float st[G4], in[G4], gate[G4], uf[G4];
+#pragma unroll
+            for (int j = 0; j < G4; ++j) {
+                const float raw = to_f(fd[j]) + bias, s = softplus_f(raw);
+                st[j] = sp ? s : raw;
+                uf[j] = to_f(fu[j]);
+                const float sl = MODE == SCAN_STATES ? 1.0f : silu_f(to_f(fz[j]));
+                gate[j] = gated ? sl : 1.0f;
+                in[j] = uf[j] * (BACK ? gate[j] : st[j]);        // step u, or d
+            }
+            if (i0 + i + G4 < n) fetch_tokens(i0 + i + G4);
+            if (FULL && p.keep && i % CK == 0 && ok) {           // the state before token tb + i0 + i
+                const int blk = 64 * urnn_scan_ed(NP), cl = ch - g * Dg, cbeg = cl / blk * blk, w = Dg - cbeg < blk ? Dg - cbeg : blk;
+                const long seg = (tb + i0 + i) / CK, segs = (p.L + CK - 1) / CK;
+                store_states<NP>(p.keep + (((long)b * segs + seg) * p.dim + g * Dg + cbeg + keep_rank(cl - cbeg, w, urnn_scan_v(NP))) * NP, 0, NP, true, h);
+            }
+            auto token = [&](int j) {
+                const float *rowB = s_B + (i + j) * NP, *rowC = s_C + (FULL ? (i + j) * NP : 0);
+                float y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+                for (int k = 0; k < NP; k += 4) {
+                    const Pack<float, 4> Bv = *reinterpret_cast<const Pack<float, 4> *>(rowB + k);
+                    Pack<float, 4> Cv;
+                    if (FULL) Cv = *reinterpret_cast<const Pack<float, 4> *>(rowC + k);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = __builtin_amdgcn_exp2f(st[j] * A2[k + e]);
+                        if (BACK) h[k + e] = a * fmaf(in[j], Bv.v[e], h[k + e]);
+                        else h[k + e] = fmaf(a, h[k + e], in[j] * Bv.v[e]);
+                        if (FULL) {
+                            if (e & 1) y1 = fmaf(Cv.v[e], h[k + e], y1);
+                            else y0 = fmaf(Cv.v[e], h[k + e], y0);
+                        }
+                    }
+                }
+                if (FULL) {
+                    const float v = fmaf(skip, uf[j], y0 + y1) * gate[j];
+                    if (ok) y[(tb + i0 + i + j) * p.dim] = from_f<T>(v);
+                } else {
+                    total += st[j];
+                }
+            };
+            if (i + G4 <= nt) {
+#pragma unroll
+                for (int j = 0; j < G4; ++j) token(j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < G4; ++j)
+                    if (i + j < nt) token(j);
             }
         }
         __syncthreads();
-        if (t0 + TT < te) fetch(t0 + TT);
-        auto token = [&](int t) -> float {
-            const Pack<float, 2> in = s_in[t * CB + sc];
-            float y0 = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; e += W) {
-                const Pack<float, W> Bv = *reinterpret_cast<const Pack<float, W> *>(s_B + t * NP + q * E + e);
-                Pack<float, W> Cv;
-                if (MODE == SCAN_FULL) Cv = *reinterpret_cast<const Pack<float, W> *>(s_C + t * NP + q * E + e);
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    h[e + i] = fmaf(__builtin_amdgcn_exp2f(in.v[0] * A2[e + i]), h[e + i], in.v[1] * Bv.v[i]);
-                    if (MODE == SCAN_FULL) y0 = fmaf(Cv.v[i], h[e + i], y0);
-                }
-            }
-            return y0;
-        };
-        auto checkpoint = [&](int t) {                           // the state before token t0 + t, t a multiple of CK
-            if (MODE == SCAN_FULL && p.keep && sok) {
-                const long seg = (t0 + t) / CK, segs = (p.L + CK - 1) / CK;
-                float *k = p.keep + (((long)b * segs + seg) * p.dim + sch) * NP + q * E;
-#pragma unroll
-                for (int e = 0; e < E; e += W) {
-                    Pack<float, W> v;
-#pragma unroll
-                    for (int i = 0; i < W; ++i) v.v[i] = h[e + i];
-                    *reinterpret_cast<Pack<float, W> *>(k + e) = v;
-                }
-            }
-        };
-        int t = 0;
-        for (; t + 4 <= nt; t += 4) {
-            if (t % CK == 0) checkpoint(t);
-            float mine = 0.0f;                                   // lane q of the quad keeps token t + q
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float yj = token(t + j);
-                if (MODE == SCAN_FULL) {
-                    yj = quad_sum(yj);
-                    mine = q == j ? yj : mine;
-                }
-            }
-            if (MODE == SCAN_FULL) s_y[(t + q) * CB + sc] = mine;
-        }
-        for (; t < nt; ++t) {
-            if (t % CK == 0) checkpoint(t);
-            const float yj = token(t);
-            if (MODE == SCAN_FULL) {
-                const float s = quad_sum(yj);
-                if (q == 0) s_y[t * CB + sc] = s;
-            }
-        }
-        __syncthreads();
-        if (MODE == SCAN_FULL && eok) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const int tt = lt + 4 * i;
-                if (tt < nt) {
-                    float v = fmaf(skip, to_f(cu[i]), s_y[tt * CB + lc]);
-                    if (z) v *= silu_f(to_f(cz[i]));
-                    y[(t0 + tt) * p.dim + ech] = from_f<T>(v);
-                }
-            }
-        }
     }
-    if (MODE == SCAN_FULL) {
-        const long z0 = te > tb ? te : tb;                       // rows behind the sequence are zeros
-        if (eok)
-            for (long t = z0 + lt; t < tfull; t += 4) y[t * p.dim + ech] = from_f<T>(0.0f);
+    if (FULL) {
+        for (long t = tb + n; ok && t < tfull; ++t) y[t * p.dim] = from_f<T>(0.0f);      // rows behind the sequence are zeros
         const int last = len > 0 ? (len - 1) / p.CL : 0;         // the chunk that holds the sequence's last token
-        if (p.state_out && sok && chunk == last)
-            store_states<E>(p.state_out + ((long)b * p.dim + sch) * p.N, q, p.N, states_vec(p.state_out, p.N, W), h);
-    } else {
-        __syncthreads();
-        s_in[tid].v[0] = total;
-        __syncthreads();
-        if (tid < CB && eok) {
-            float t = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t += s_in[tid + CB * i].v[0];
-            p.sum[((long)b * p.chunks + chunk) * p.dim + ech] = t;
-        }
-        if (sok) {
-            float *s = p.S + (((long)b * p.chunks + chunk) * p.dim + sch) * NP + q * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) s[e] = h[e];
-        }
+        if (p.state_out && ok && chunk == last)
+            store_states<NP>(p.state_out + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state_out, p.N, 4), h);
+    } else if (ok) {
+        p.sum[((long)b * p.chunks + chunk) * p.dim + ch] = total;
+        store_states<NP>(p.S + (((long)b * p.chunks + chunk) * p.dim + ch) * NP, 0, NP, true, h);
     }
 }
 
@@ -229,29 +192,34 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
 
 int urnn_scan_chunks(int B, int L, int D, int *CL)
 {
-    const long blocks = (long)B * ((D + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
-    long want = blocks >= 512 ? 1 : (1024 + blocks - 1) / blocks;
+    const long waves = (long)B * ((D + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
+    long want = waves >= 640 ? 1 : (2048 + waves - 1) / waves;
     const long most = (L + 63) / 64;
     if (want > most) want = most;
     if (want < 1) want = 1;
     long cl = (L + want - 1) / want;
-    cl = (cl + 31) / 32 * 32;
-    if (cl < 32) cl = 32;
+    cl = (cl + 15) / 16 * 16;
     *CL = (int)cl;
-    const int chunks = (int)((L + cl - 1) / cl);
-    return chunks < 1 ? 1 : chunks;
+    return (int)((L + cl - 1) / cl);
+}
+
+template <typename T, int NP, int MODE>
+static void launch_pass(const ScanParams &p, hipStream_t st)
+{
+    const int Dg = p.dim / p.G, cbs = p.G * ((Dg + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
+    const int walked = MODE == SCAN_FULL ? p.chunks : p.chunks - 1;
+    scan_kernel<T, NP, MODE><<<dim3((unsigned)(cbs * walked * p.batch)), 64, 0, st>>>(p);
 }
 
 template <typename T, int NP>
 static hipError_t launch_scan(const ScanParams &p, hipStream_t st)
 {
-    const int Dg = p.dim / p.G, cbs = p.G * ((Dg + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
     if (p.chunks > 1) {
-        scan_kernel<T, NP, SCAN_STATES><<<dim3((unsigned)(cbs * (p.chunks - 1) * p.batch)), 256, 0, st>>>(p);
+        launch_pass<T, NP, SCAN_STATES>(p, st);
         const long count = (long)p.batch * p.dim * NP;
         scan_carry_kernel<NP><<<dim3((unsigned)((count + 255) / 256)), 256, 0, st>>>(p.A, p.sum, p.S, p.dim, p.N, p.chunks, count);
     }
-    scan_kernel<T, NP, SCAN_FULL><<<dim3((unsigned)(cbs * p.chunks * p.batch)), 256, 0, st>>>(p);
+    launch_pass<T, NP, SCAN_FULL>(p, st);
     return hipGetLastError();
 }
 
@@ -301,21 +269,28 @@ static hipError_t launch_step(const ScanParams &p, hipStream_t st)
 }
 
 template <typename T>
-static hipError_t by_states(const ScanParams &p, bool step, hipStream_t st)
+static hipError_t by_states(const ScanParams &p, int what, hipStream_t st)
 {
+    auto go = [&](auto np) {
+        constexpr int NP = decltype(np)::value;
+        if (what == SCAN_STEP) return launch_step<T, NP>(p, st);
+        if (what == SCAN_BACK) { launch_pass<T, NP, SCAN_BACK>(p, st); return hipGetLastError(); }
+        return launch_scan<T, NP>(p, st);
+    };
     switch (urnn_scan_np(p.N)) {
-    case 4: return step ? launch_step<T, 4>(p, st) : launch_scan<T, 4>(p, st);
-    case 8: return step ? launch_step<T, 8>(p, st) : launch_scan<T, 8>(p, st);
-    case 16: return step ? launch_step<T, 16>(p, st) : launch_scan<T, 16>(p, st);
-    case 32: return step ? launch_step<T, 32>(p, st) : launch_scan<T, 32>(p, st);
-    default: return step ? launch_step<T, 64>(p, st) : launch_scan<T, 64>(p, st);
+    case 4: return go(std::integral_constant<int, 4>());
+    case 8: return go(std::integral_constant<int, 8>());
+    case 16: return go(std::integral_constant<int, 16>());
+    case 32: return go(std::integral_constant<int, 32>());
+    default: return go(std::integral_constant<int, 64>());
     }
 }
 
-static hipError_t by_type(const ScanParams &p, int dtype, bool step, hipStream_t st)
+static hipError_t by_type(const ScanParams &p, int dtype, int what, hipStream_t st)
 {
-    return dtype == URNN_F32 ? by_states<float>(p, step, st) : dtype == URNN_BF16 ? by_states<bf16_t>(p, step, st) : by_states<f16_t>(p, step, st);
+    return dtype == URNN_F32 ? by_states<float>(p, what, st) : dtype == URNN_BF16 ? by_states<bf16_t>(p, what, st) : by_states<f16_t>(p, what, st);
 }
 
-hipError_t urnn_launch_scan(const ScanParams &p, int dtype, hipStream_t st) { return by_type(p, dtype, false, st); }
-hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st) { return by_type(p, dtype, true, st); }
+hipError_t urnn_launch_scan(const ScanParams &p, int dtype, hipStream_t st) { return by_type(p, dtype, SCAN_FULL, st); }
+hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st) { return by_type(p, dtype, SCAN_STEP, st); }
+hipError_t urnn_launch_scan_back_summaries(const ScanParams &p, int dtype, hipStream_t st) { return by_type(p, dtype, SCAN_BACK, st); }

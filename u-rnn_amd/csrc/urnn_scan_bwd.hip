@@ -19,6 +19,8 @@
 // comes from its right (k' = a_first (..)), and the sum of its steps; a short kernel carries it over the chunks.
 #include "urnn_seq.h"
 
+#include <type_traits>
+
 // Sum v[i] over the 16 quads of the wave (lanes with equal lane & 3).  2 E values; result r[m] (m < max(1, E / 2)) holds, in row rho of
 // 16 lanes, value 4 m + {0, 2, 1, 3}[rho] (E = 1: value rho / 2).
 __device__ __forceinline__ float add_swapped32(float a, float b)
@@ -44,100 +46,6 @@ __device__ __forceinline__ void channel_sums(const float (&v)[2 * E], float (&r)
     for (int m = 0; m < (E < 2 ? 1 : E / 2); ++m) {
         r[m] += dpp_move<0x128>(r[m]);               // row_ror:8
         r[m] += dpp_move<0x124>(r[m]);               // row_ror:4
-    }
-}
-
-// What a chunk hands to the left from a zero right: h <- a_t (h + C_t d_t) from its last token to its first.
-template <typename T, int NP>
-__global__ __launch_bounds__(256) void scan_back_states_kernel(const ScanParams p)
-{
-    constexpr int E = NP / 4, W = E < 4 ? E : 4, TT = 32, CB = 64, R = TT * CB / 256, RB = TT * NP / 256 < 1 ? 1 : TT * NP / 256;
-    __shared__ alignas(16) Pack<float, 2> s_in[TT * CB];         // (step, d)
-    __shared__ alignas(16) float s_C[TT * NP];
-    const int tid = threadIdx.x, q = tid & 3;
-    const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
-    const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
-    const int walked = p.chunks - 1;                             // the first chunk hands nothing on
-    const int chunk = 1 + blockIdx.x / (cbs * p.G) % walked, b = blockIdx.x / (cbs * p.G) / walked;
-    const int len = seq_len(p.lengths, b, p.L);
-    const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L, te = tfull < len ? tfull : len;
-    const T *dl = reinterpret_cast<const T *>(p.delta) + b * p.sd.b, *dout = reinterpret_cast<const T *>(p.dout) + b * p.so.b;
-    const T *z = p.z ? reinterpret_cast<const T *>(p.z) + b * p.sz.b : nullptr;
-    const T *Cp = reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N;
-    const int lc = tid & 63, lt = tid >> 6, ech = c0 + lc;
-    const bool eok = ech < cend;
-    const float bias = p.bias && eok ? p.bias[ech] : 0.0f;
-    const int sc = tid >> 2, sch = c0 + sc;
-    const bool sok = sch < cend;
-    float A2[E], h[E];
-    load_states<E>(p.A + (long)(sok ? sch : c0) * p.N, q, p.N, states_vec(p.A, p.N, W), A2);
-#pragma unroll
-    for (int e = 0; e < E; ++e) { A2[e] *= URNN_LOG2E; h[e] = 0.0f; }
-    float total = 0.0f;
-    T rd[R] = {}, ro[R] = {}, rz[R] = {}, rC[RB] = {};
-    auto fetch = [&](long t0) {
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const long t = t0 + lt + 4 * i;
-            if (eok && t < te) {
-                rd[i] = dl[t * p.sd.t + ech];
-                ro[i] = dout[t * p.so.t + ech];
-                if (z) rz[i] = z[t * p.sz.t + ech];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < RB; ++i) {
-            const int k = tid + 256 * i, n = k % NP;
-            const long t = t0 + k / NP;
-            rC[i] = T(0.0f);
-            if (k < TT * NP && n < p.N && t < te) rC[i] = Cp[t * p.sC.t + n];
-        }
-    };
-    if (tb < te) {
-        long t0 = tb + (te - 1 - tb) / TT * TT;
-        fetch(t0);
-        for (; t0 >= tb; t0 -= TT) {
-            const int nt = te - t0 < TT ? (int)(te - t0) : TT;
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const float raw = to_f(rd[i]) + bias, step = p.softplus ? softplus_f(raw) : raw;
-                const float d = to_f(ro[i]) * (z ? silu_f(to_f(rz[i])) : 1.0f);
-                s_in[(lt + 4 * i) * CB + lc] = {{step, d}};
-                if (lt + 4 * i < nt) total += step;
-            }
-#pragma unroll
-            for (int i = 0; i < RB; ++i) {
-                const int k = tid + 256 * i;
-                if (k < TT * NP) s_C[k] = to_f(rC[i]);
-            }
-            __syncthreads();
-            if (t0 - TT >= tb) fetch(t0 - TT);
-#pragma unroll 4
-            for (int t = nt - 1; t >= 0; --t) {
-                const Pack<float, 2> in = s_in[t * CB + sc];
-#pragma unroll
-                for (int e = 0; e < E; e += W) {
-                    const Pack<float, W> Cv = *reinterpret_cast<const Pack<float, W> *>(s_C + t * NP + q * E + e);
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-                        h[e + i] = __builtin_amdgcn_exp2f(in.v[0] * A2[e + i]) * fmaf(Cv.v[i], in.v[1], h[e + i]);
-                }
-            }
-            __syncthreads();
-        }
-    }
-    s_in[tid].v[0] = total;
-    __syncthreads();
-    if (tid < CB && eok) {
-        float t = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t += s_in[tid + CB * i].v[0];
-        p.sum[((long)b * p.chunks + chunk) * p.dim + ech] = t;
-    }
-    if (sok) {
-        float *s = p.S + (((long)b * p.chunks + chunk) * p.dim + sch) * NP + q * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s[e] = h[e];
     }
 }
 
@@ -172,12 +80,62 @@ __global__ __launch_bounds__(256) void scan_back_carry_kernel(const float *__res
     }
 }
 
+// V adjacent channels of a token as they lie in memory: they wait in registers for a whole tile, two 16-bit values to a register.
+template <typename T, int V> struct Raw {
+    unsigned w[V * sizeof(T) / 4];
+    __device__ __forceinline__ float get(int i) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return to_f(__builtin_bit_cast(T, (unsigned short)(w[i / 2] >> (16 * (i & 1)))));
+    }
+    // channels from `valid` on as zeros; wide: rows start on 16 bytes and all V are there
+    __device__ __forceinline__ void load(const T *src, int valid, bool wide)
+    {
+        if (wide) {
+            constexpr int W = V * sizeof(T) / 4 < 4 ? V * sizeof(T) / 4 : 4;
+#pragma unroll
+            for (int k = 0; k < (int)(V * sizeof(T) / 4); k += W) {
+                const Pack<unsigned, W> t = *reinterpret_cast<const Pack<unsigned, W> *>(reinterpret_cast<const unsigned *>(src) + k);
+#pragma unroll
+                for (int i = 0; i < W; ++i) w[k + i] = t.v[i];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < (int)(V * sizeof(T) / 4); ++k) w[k] = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < valid) {
+                    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(src[i]);
+                    else w[i / 2] |= (unsigned)__builtin_bit_cast(unsigned short, src[i]) << (16 * (i & 1));
+                }
+        }
+    }
+};
+template <typename T, int V>
+__device__ __forceinline__ void store_channels(T *dst, int valid, bool wide, const float (&v)[V])
+{
+    constexpr int W = V * sizeof(T) < 16 ? V : 16 / sizeof(T);
+    if (wide) {
+#pragma unroll
+        for (int k = 0; k < V; k += W) {
+            Pack<T, W> t;
+#pragma unroll
+            for (int i = 0; i < W; ++i) t.v[i] = from_f<T>(v[k + i]);
+            *reinterpret_cast<Pack<T, W> *>(dst + k) = t;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < valid) dst[i] = from_f<T>(v[i]);
+    }
+}
+
 template <typename T, int NP>
 __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams p)
 {
-    constexpr int E = NP / 4, W = E < 4 ? E : 4, ED = urnn_scan_ed(NP), CK = urnn_scan_ck(NP), CB = 64 * ED, TT = 16;
-    constexpr int R = TT * CB / 256, LT = 256 / CB, RB = TT * NP / 256 < 1 ? 1 : TT * NP / 256;
-    __shared__ alignas(16) Pack<float, 4> s_io[TT * CB];         // in: (step, step u, d, -); out: (sum w A log2 e, sum k B, sum C h, -)
+    constexpr int E = NP / 4, W = E < 4 ? E : 4, ED = urnn_scan_ed(NP), CK = urnn_scan_ck(NP), CB = 64 * ED, TT = urnn_scan_tt(NP);
+    constexpr int V = urnn_scan_v(NP), CG = CB / V, RB = TT * NP / 256 < 1 ? 1 : TT * NP / 256;
+    __shared__ alignas(16) Pack<float, 4> s_io[TT * CB];         // in: (step, step u, d, -); out: (sum w A log2 e, sum k B, sum C h, step)
     __shared__ alignas(16) float s_B[TT * NP], s_C[TT * NP];
     __shared__ float s_bc[4 * TT * 2 * NP];                      // [wave][token][dB | dC]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane & 3;
@@ -185,31 +143,49 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
     const int chunk = blockIdx.x / (cbs * p.G) % p.chunks, slot = blockIdx.x / (cbs * p.G) / p.chunks;
     const long segs = (p.L + CK - 1) / CK;
+    const int width = cend - c0 < CB ? cend - c0 : CB;
+    const bool sp = p.softplus != 0;
 
-    const int lc = tid % CB, lt = tid / CB, ech = c0 + lc;       // elementwise: channel lc, tokens lt + LT i
-    const bool eok = ech < cend;
-    const float bias = p.bias && eok ? p.bias[ech] : 0.0f, skip = p.D && eok ? p.D[ech] : 0.0f;
-    int sc[ED], sch[ED];                                         // scan: channels sc[k], states q E ..
+    // elementwise: token lt of a tile, channels c0 + V lg ..  Channel V lg + i has its slot at i CG + lg of the token's row, so that the
+    // threads of a token write side by side.
+    const int lg = tid % CG, lt = tid / CG;
+    const int evalid = width - V * lg;                           // channels there, of V
+    const bool eok = evalid > 0, ewide = p.wide && evalid >= V;
+    const int ech = c0 + (eok ? V * lg : 0);
+    float bias[V], skip[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = p.bias && i < evalid ? p.bias[ech + i] : 0.0f;
+        skip[i] = p.D && i < evalid ? p.D[ech + i] : 0.0f;
+    }
+    // scan: slots sc[k] of a row, states q E ..
+    int sc[ED], sch[ED], srank[ED];
     bool sok[ED];
     float A2[ED][E], dA[ED][E];
 #pragma unroll
     for (int k = 0; k < ED; ++k) {
         sc[k] = wave * 16 * ED + 16 * k + (lane >> 2);
-        sok[k] = c0 + sc[k] < cend;
-        sch[k] = sok[k] ? c0 + sc[k] : c0;
+        const int c = sc[k] % CG * V + sc[k] / CG;               // the slot's channel
+        sok[k] = c < width;
+        sch[k] = c0 + (sok[k] ? c : 0);
+        srank[k] = c0 + keep_rank(sok[k] ? c : 0, width, V);
         load_states<E>(p.A + (long)sch[k] * p.N, q, p.N, states_vec(p.A, p.N, W), A2[k]);
 #pragma unroll
-        for (int e = 0; e < E; ++e) { A2[k][e] *= URNN_LOG2E; dA[k][e] = 0.0f; }
+        for (int e = 0; e < E; ++e) {
+            A2[k][e] *= sok[k] ? URNN_LOG2E : 0.0f;
+            A2[k][e] = A2[k][e] < -3.0e38f ? -3.0e38f : A2[k][e];            // 0 * A2 stays 0: a step of 0 keeps the state
+            dA[k][e] = 0.0f;
+        }
     }
-    float dD = 0.0f, dbias = 0.0f;
+    float dD[V] = {}, dbias[V] = {};
 
     for (int b = slot; b < p.batch; b += p.slots) {
-        const int len = seq_len(p.lengths, b, p.L);
+        const int len = __builtin_amdgcn_readfirstlane(seq_len(p.lengths, b, p.L));
         const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L, te = tfull < len ? tfull : len;
-        const T *u = reinterpret_cast<const T *>(p.u) + b * p.su.b, *dl = reinterpret_cast<const T *>(p.delta) + b * p.sd.b;
-        const T *z = p.z ? reinterpret_cast<const T *>(p.z) + b * p.sz.b : nullptr, *dout = reinterpret_cast<const T *>(p.dout) + b * p.so.b;
+        const T *u = reinterpret_cast<const T *>(p.u) + b * p.su.b + ech, *dl = reinterpret_cast<const T *>(p.delta) + b * p.sd.b + ech;
+        const T *z = p.z ? reinterpret_cast<const T *>(p.z) + b * p.sz.b + ech : nullptr, *dout = reinterpret_cast<const T *>(p.dout) + b * p.so.b + ech;
         const T *Bp = reinterpret_cast<const T *>(p.B) + b * p.sB.b + (long)g * p.N, *Cp = reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N;
-        const long base = (long)b * p.L * p.dim;
+        const long base = (long)b * p.L * p.dim + ech;
         T *du = reinterpret_cast<T *>(p.du) + base, *ddl = reinterpret_cast<T *>(p.ddelta) + base, *dz = reinterpret_cast<T *>(p.dz) + base;
         // partial rows of this channel block: [cb in group][b][t][g][n]
         const long prow = ((long)(cb % cbs) * p.batch + b) * p.L;
@@ -221,46 +197,39 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
         for (int k = 0; k < ED; ++k) {
 #pragma unroll
             for (int e = 0; e < E; ++e) carry[k][e] = ck[k][e] = 0.0f;
-            if (chunk + 1 < p.chunks) {
-                const float *s = p.S + (((long)b * p.chunks + chunk + 1) * p.dim + sch[k]) * NP + q * E;
+            if (sok[k]) {
+                if (chunk + 1 < p.chunks) {
+                    const float *s = p.S + (((long)b * p.chunks + chunk + 1) * p.dim + sch[k]) * NP + q * E;
 #pragma unroll
-                for (int e = 0; e < E; ++e) carry[k][e] = s[e];
-            } else if (p.dstate_out) {
-                load_states<E>(p.dstate_out + ((long)b * p.dim + sch[k]) * p.N, q, p.N, states_vec(p.dstate_out, p.N, W), carry[k]);
+                    for (int e = 0; e < E; ++e) carry[k][e] = s[e];
+                } else if (p.dstate_out) {
+                    load_states<E>(p.dstate_out + ((long)b * p.dim + sch[k]) * p.N, q, p.N, states_vec(p.dstate_out, p.N, W), carry[k]);
+                }
             }
         }
         auto load_ck = [&](long seg) {
 #pragma unroll
-            for (int k = 0; k < ED; ++k) {
-                const float *s = p.keep + (((long)b * segs + seg) * p.dim + sch[k]) * NP + q * E;
-#pragma unroll
-                for (int e = 0; e < E; e += W) {
-                    const Pack<float, W> v = *reinterpret_cast<const Pack<float, W> *>(s + e);
-#pragma unroll
-                    for (int i = 0; i < W; ++i) ck[k][e + i] = v.v[i];
-                }
-            }
+            for (int k = 0; k < ED; ++k)
+                if (sok[k]) load_states<E>(p.keep + (((long)b * segs + seg) * p.dim + srank[k]) * NP, q, NP, true, ck[k]);
         };
-        T ru[R] = {}, rd[R] = {}, rz[R] = {}, ro[R] = {}, rB[RB] = {}, rC[RB] = {};
+        Raw<T, V> ru = {}, rd = {}, rz = {}, ro = {};
+        T rB[RB] = {}, rC[RB] = {};
         auto fetch = [&](long t0) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const long t = t0 + lt + LT * i;
-                if (eok && t < te) {
-                    ru[i] = u[t * p.su.t + ech];
-                    rd[i] = dl[t * p.sd.t + ech];
-                    ro[i] = dout[t * p.so.t + ech];
-                    if (z) rz[i] = z[t * p.sz.t + ech];
-                }
+            const long t = t0 + lt;
+            if (eok && t < te) {
+                ru.load(u + t * p.su.t, evalid, ewide);
+                rd.load(dl + t * p.sd.t, evalid, ewide);
+                ro.load(dout + t * p.so.t, evalid, ewide);
+                if (z) rz.load(z + t * p.sz.t, evalid, ewide);
             }
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
                 const int k = tid + 256 * i, n = k % NP;
-                const long t = t0 + k / NP;
+                const long tr = t0 + k / NP;
                 rB[i] = rC[i] = T(0.0f);
-                if (k < TT * NP && n < p.N && t < te) {
-                    rB[i] = Bp[t * p.sB.t + n];
-                    rC[i] = Cp[t * p.sC.t + n];
+                if (k < TT * NP && n < p.N && tr < te) {
+                    rB[i] = Bp[tr * p.sB.t + n];
+                    rC[i] = Cp[tr * p.sC.t + n];
                 }
             }
         };
@@ -270,13 +239,13 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
             fetch(t0);
             for (; t0 >= tb; t0 -= TT) {
                 const int nt = te - t0 < TT ? (int)(te - t0) : TT;
-                T cu[R], cd[R], cz[R], co[R];
+                const Raw<T, V> cu = ru, cd = rd, cz = rz, co = ro;
+                const bool here = eok && lt < nt;                // tokens behind the sequence: steps of zero, which change nothing
 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const float raw = to_f(rd[i]) + bias, step = p.softplus ? softplus_f(raw) : raw, uf = to_f(ru[i]);
-                    const float d = to_f(ro[i]) * (z ? silu_f(to_f(rz[i])) : 1.0f);
-                    s_io[(lt + LT * i) * CB + lc] = {{step, step * uf, d, 0.0f}};
-                    cu[i] = ru[i]; cd[i] = rd[i]; cz[i] = rz[i]; co[i] = ro[i];
+                for (int i = 0; i < V; ++i) {
+                    const float raw = cd.get(i) + bias[i], s = softplus_f(raw), step = here ? (sp ? s : raw) : 0.0f;
+                    const float d = co.get(i) * (z ? silu_f(cz.get(i)) : 1.0f);
+                    s_io[lt * CB + i * CG + lg] = {{step, here ? step * cu.get(i) : 0.0f, here ? d : 0.0f, 0.0f}};
                 }
 #pragma unroll
                 for (int i = 0; i < RB; ++i) {
@@ -287,7 +256,6 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                 if (t0 - TT >= tb) fetch(t0 - TT);
 
                 for (int s0 = (nt - 1) / CK * CK; s0 >= 0; s0 -= CK) {
-                    const int ns = nt - s0 < CK ? nt - s0 : CK;
                     float a[CK][ED][E], ah[CK][ED][E], h[ED][E];
 #pragma unroll
                     for (int k = 0; k < ED; ++k)
@@ -296,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                     if (t0 + s0 > tb) load_ck((t0 + s0) / CK - 1);
 #pragma unroll
                     for (int j = 0; j < CK; ++j) {
-                        if (j < ns) {
+                        {
                             const int t = s0 + j;
                             float Bv[E];
 #pragma unroll
@@ -307,7 +275,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                             }
 #pragma unroll
                             for (int k = 0; k < ED; ++k) {
-                                const Pack<float, 4> in = s_io[t * CB + sc[k]];
+                                const Pack<float, 2> in = *reinterpret_cast<const Pack<float, 2> *>(s_io + t * CB + sc[k]);
 #pragma unroll
                                 for (int e = 0; e < E; ++e) {
                                     a[j][k][e] = __builtin_amdgcn_exp2f(in.v[0] * A2[k][e]);
@@ -319,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                     }
 #pragma unroll
                     for (int j = CK - 1; j >= 0; --j) {
-                        if (j < ns) {
+                        {
                             const int t = s0 + j;
                             float Bv[E], Cv[E], v[2 * E] = {};               // v: dB's terms, then dC's
 #pragma unroll
@@ -340,14 +308,14 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                                     SG = fmaf(kk, Bv[e], SG);
                                     SY = fmaf(Cv[e], hj, SY);
                                     dA[k][e] = fmaf(w, in.v[0], dA[k][e]);
-                                    v[e] = sok[k] ? fmaf(kk, in.v[1], v[e]) : v[e];
-                                    v[E + e] = sok[k] ? fmaf(hj, in.v[2], v[E + e]) : v[E + e];
+                                    v[e] = fmaf(kk, in.v[1], v[e]);
+                                    v[E + e] = fmaf(hj, in.v[2], v[E + e]);
                                     carry[k][e] = a[j][k][e] * kk;
                                 }
                                 SW = quad_sum(SW);
                                 SG = quad_sum(SG);
-                                if (z) SY = quad_sum(SY);
-                                if (q == 0) s_io[t * CB + sc[k]] = {{SW, SG, SY, 0.0f}};
+                                SY = quad_sum(SY);
+                                if (q == 0) s_io[t * CB + sc[k]] = {{SW, SG, SY, in.v[0]}};
                             }
                             float r[E < 2 ? 1 : E / 2];
                             channel_sums<E>(v, r);
@@ -370,27 +338,28 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                     }
                 }
                 __syncthreads();
-                if (eok) {
+                if (eok && lt < nt) {
+                    float odz[V], odd[V], odu[V];
 #pragma unroll
-                    for (int i = 0; i < R; ++i) {
-                        const int tt = lt + LT * i;
-                        if (tt < nt) {
-                            const Pack<float, 4> r = s_io[tt * CB + lc];
-                            const float raw = to_f(cd[i]) + bias, step = p.softplus ? softplus_f(raw) : raw, uf = to_f(cu[i]), of = to_f(co[i]);
-                            float d = of;
-                            const long at = (t0 + tt) * p.dim + ech;
-                            if (z) {
-                                const float zf = to_f(cz[i]), sg = sigmoid_f(zf);
-                                d = of * zf * sg;
-                                dz[at] = from_f<T>(of * fmaf(skip, uf, r.v[2]) * sg * fmaf(zf, 1.0f - sg, 1.0f));
-                            }
-                            const float dstep = fmaf(r.v[0], URNN_LN2, r.v[1] * uf), dd = p.softplus ? dstep * sigmoid_f(raw) : dstep;
-                            ddl[at] = from_f<T>(dd);
-                            du[at] = from_f<T>(fmaf(r.v[1], step, d * skip));
-                            dD = fmaf(d, uf, dD);
-                            dbias += dd;
+                    for (int i = 0; i < V; ++i) {
+                        const Pack<float, 4> r = s_io[lt * CB + i * CG + lg];
+                        const float raw = cd.get(i) + bias[i], uf = cu.get(i), of = co.get(i);
+                        float d = of;
+                        if (z) {
+                            const float zf = cz.get(i), sg = sigmoid_f(zf);
+                            d = of * zf * sg;
+                            odz[i] = of * fmaf(skip[i], uf, r.v[2]) * sg * fmaf(zf, 1.0f - sg, 1.0f);
                         }
+                        const float dstep = fmaf(r.v[0], URNN_LN2, r.v[1] * uf), dd = dstep * (sp ? sigmoid_f(raw) : 1.0f);
+                        odd[i] = dd;
+                        odu[i] = fmaf(r.v[1], r.v[3], d * skip[i]);
+                        dD[i] = fmaf(d, uf, dD[i]);
+                        dbias[i] += dd;
                     }
+                    const long at = (t0 + lt) * p.dim;
+                    store_channels<T, V>(ddl + at, evalid, ewide, odd);
+                    store_channels<T, V>(du + at, evalid, ewide, odu);
+                    if (z) store_channels<T, V>(dz + at, evalid, ewide, odz);
                 }
                 for (int k = tid; k < nt * 2 * NP; k += 256) {
                     const int t = k / (2 * NP), w = k % (2 * NP), n = w % NP;
@@ -404,10 +373,11 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
             }
         }
         const long z0 = te > tb ? te : tb;                       // rows behind the sequence are zeros
-        for (long t = z0 + lt; eok && t < tfull; t += LT) {
-            const long at = t * p.dim + ech;
-            du[at] = ddl[at] = from_f<T>(0.0f);
-            if (z) dz[at] = from_f<T>(0.0f);
+        const float none[V] = {};
+        for (long t = z0 + lt; eok && t < tfull; t += TT) {
+            store_channels<T, V>(du + t * p.dim, evalid, ewide, none);
+            store_channels<T, V>(ddl + t * p.dim, evalid, ewide, none);
+            if (z) store_channels<T, V>(dz + t * p.dim, evalid, ewide, none);
         }
         for (long k = z0 * NP + tid; k < tfull * NP; k += 256) {
             const long t = k / NP;
@@ -419,20 +389,23 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
             for (int k = 0; k < ED; ++k)
                 if (sok[k]) store_states<E>(p.dstate + ((long)b * p.dim + sch[k]) * p.N, q, p.N, states_vec(p.dstate, p.N, W), carry[k]);
         }
-        __syncthreads();                                         // the next sequence's tile overwrites s_B, s_C and s_bc
+        __syncthreads();                                         // the next sequence's tile overwrites s_io, s_B, s_C and s_bc
     }
-    const long part = (long)slot * p.chunks + chunk;
+    float *sums = p.dAp + ((long)slot * p.chunks + chunk) * p.dim * (p.N + 2);      // this part's dA, dD, ddelta_bias
 #pragma unroll
     for (int k = 0; k < ED; ++k)
-        if (sok[k]) store_states<E>(p.dAp + (part * p.dim + sch[k]) * p.N, q, p.N, states_vec(p.dAp, p.N, W), dA[k]);
-    s_io[tid] = {{dD, dbias, 0.0f, 0.0f}};
-    __syncthreads();
-    if (tid < CB && eok) {
-        float x = 0.0f, y = 0.0f;
+        if (sok[k]) store_states<E>(sums + (long)sch[k] * p.N, q, p.N, states_vec(sums, p.N, W), dA[k]);
 #pragma unroll
-        for (int i = 0; i < LT; ++i) { x += s_io[tid + CB * i].v[0]; y += s_io[tid + CB * i].v[1]; }
-        p.dDp[part * p.dim + ech] = x;
-        p.dbp[part * p.dim + ech] = y;
+    for (int i = 0; i < V; ++i) s_io[lt * CB + i * CG + lg] = {{dD[i], dbias[i], 0.0f, 0.0f}};
+    __syncthreads();
+    if (tid < CB) {
+        float x = 0.0f, y = 0.0f;
+        for (int t = 0; t < TT; ++t) { x += s_io[t * CB + tid].v[0]; y += s_io[t * CB + tid].v[1]; }
+        const int c = tid % CG * V + tid / CG;
+        if (c < width) {
+            sums[(long)p.dim * p.N + c0 + c] = x;
+            sums[(long)p.dim * (p.N + 1) + c0 + c] = y;
+        }
     }
 }
 
@@ -461,7 +434,7 @@ int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots)
     *CL = (int)(cl < 32 ? 32 : cl);
     const int chunks = (L + *CL - 1) / *CL;
     long s = B;                                                  // several sequences to a block once there are enough blocks
-    while (s > 1 && s * cbs * chunks > 2048) s = (s + 1) / 2;
+    while (s > 1 && s * cbs * chunks > 1024) s = (s + 1) / 2;
     *slots = (int)s;
     return chunks;
 }
@@ -471,8 +444,8 @@ static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, flo
 {
     const int Dg = p.dim / p.G, CB = 64 * urnn_scan_ed(NP), gcbs = (Dg + CB - 1) / CB;
     if (p.chunks > 1) {
-        const int cbs = p.G * ((Dg + 63) / 64);
-        scan_back_states_kernel<T, NP><<<dim3((unsigned)(cbs * (p.chunks - 1) * p.batch)), 256, 0, st>>>(p);
+        const hipError_t e = urnn_launch_scan_back_summaries(p, sizeof(T) == 4 ? URNN_F32 : std::is_same<T, bf16_t>::value ? URNN_BF16 : URNN_F16, st);
+        if (e != hipSuccess) return e;
         const long count = (long)p.batch * p.dim * NP;
         scan_back_carry_kernel<NP><<<dim3((unsigned)((count + 255) / 256)), 256, 0, st>>>(p.A, p.sum, p.S, p.dstate_out, p.dim, p.N, p.chunks, count);
     }
@@ -480,10 +453,9 @@ static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, flo
     const long n = (long)p.batch * p.L * p.G * p.N;
     scan_fold_rows_kernel<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(p.dBp, p.dCp, gcbs, n, reinterpret_cast<T *>(dB), reinterpret_cast<T *>(dC));
     hipError_t e = hipGetLastError();
-    const int parts = p.slots * p.chunks;
-    if (e == hipSuccess) e = urnn_launch_sum_parts(p.dAp, (long)p.dim * p.N, parts, (long)p.dim * p.N, dA, accumulate, st);
-    if (e == hipSuccess && dD) e = urnn_launch_sum_parts(p.dDp, p.dim, parts, p.dim, dD, accumulate, st);
-    if (e == hipSuccess && dbias) e = urnn_launch_sum_parts(p.dbp, p.dim, parts, p.dim, dbias, accumulate, st);
+    float *const outs[3] = {dA, dD, dbias};
+    const long sizes[3] = {(long)p.dim * p.N, p.dim, p.dim};
+    if (e == hipSuccess) e = urnn_launch_sum_parts(p.dAp, p.slots * p.chunks, sizes, outs, accumulate, st);
     return e;
 }
 

@@ -121,23 +121,33 @@ struct ScanParams {
     int batch, L, dim, N, G, chunks, CL, softplus;
     // backward
     int slots;                                       // blocks along the batch
+    int wide;                                        // all (B,L,D) rows start on 16 bytes
     const float *dstate_out;                         // (B,D,N) or NULL
     void *du, *ddelta, *dz;                          // (B,L,D) contiguous
     float *dstate;                                   // (B,D,N) or NULL
     float *dBp, *dCp;                                // per channel block: [blocks of a group][B][L][G][N]
-    float *dAp, *dDp, *dbp;                          // per (batch slot, chunk): [parts][D][N], [parts][D], [parts][D]
+    float *dAp;                                      // per (batch slot, chunk): [parts][D N | D | D], sums for dA, dD, ddelta_bias
 };
 
-#define URNN_SCAN_CB 64     // channels of a forward block
+#define URNN_SCAN_CB 64     // channels of a forward wave
+enum { SCAN_STATES = 0, SCAN_FULL = 1, SCAN_BACK = 2, SCAN_STEP = 3 };
 
 // Tokens between two checkpoints of the state: what the backward holds in registers of decays and states at a time, 2 CK NP / 4 (x 2
 // channels up to 16 states).
 __host__ __device__ static constexpr int urnn_scan_ck(int np) { return np == 64 ? 4 : 8; }
-__host__ __device__ static constexpr int urnn_scan_ed(int np) { return np <= 16 ? 2 : 1; }    // channels of a backward lane
+__host__ __device__ static constexpr int urnn_scan_ed(int) { return 1; }    // channels of a backward lane
 
 static inline int urnn_scan_np(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
+// Place of channel c among the w channels of a backward block, in the record of checkpoints: the block's thread for channels V i ..
+// V i + V - 1 spreads them over its LDS rows so that neighbours of a row are V channels apart, and reads a row's states side by side.
+__host__ __device__ static inline int keep_rank(int c, int w, int V) { return w % V == 0 ? c % V * (w / V) + c / V : c; }
+// Tokens of a backward tile, and so the channels of a thread of 256
+__host__ __device__ static constexpr int urnn_scan_tt(int) { return 16; }
+__host__ __device__ static constexpr int urnn_scan_v(int np) { return urnn_scan_tt(np) * 64 * urnn_scan_ed(np) / 256; }
+
 hipError_t urnn_launch_scan(const ScanParams &p, int dtype, hipStream_t st);
+hipError_t urnn_launch_scan_back_summaries(const ScanParams &p, int dtype, hipStream_t st);
 hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st);
 int urnn_scan_chunks(int B, int L, int D, int *CL);
 hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, void *dB, void *dC, int accumulate, hipStream_t st);
@@ -182,5 +192,5 @@ hipError_t urnn_launch_norm(const NormParams &p, int dtype, bool wide, hipStream
 hipError_t urnn_launch_norm_backward(const NormParams &p, int dtype, bool wide, float *dpre, float *dpost, float *dscale, int accumulate, hipStream_t st);
 int urnn_norm_parts(long rows, int D);
 
-// out[i] (+)= sum over parts of src[part][i], in ascending order of parts within fixed groups (bit-reproducible)
-hipError_t urnn_launch_sum_parts(const float *src, long stride, int parts, long n, float *out, int accumulate, hipStream_t st);
+// src [parts][n[0] + n[1] + n[2]] -> out[k] (+)= the sums over parts of its columns; out[k] may be NULL.  In double, in a fixed order.
+hipError_t urnn_launch_sum_parts(const float *src, int parts, const long (&n)[3], float *const (&out)[3], int accumulate, hipStream_t st);
