@@ -32,23 +32,26 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
     const int walked = FULL ? p.chunks : p.chunks - 1;           // nothing reads the summary of the last chunk (BACK: the first)
     const int chunk = (BACK ? 1 : 0) + blockIdx.x / (cbs * p.G) % walked, b = blockIdx.x / (cbs * p.G) / walked;
-    const int len = seq_len(p.lengths, b, p.L);
+    const int len = __builtin_amdgcn_readfirstlane(seq_len(p.lengths, b, p.L));
     const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L, te = tfull < len ? tfull : len;
     const int n = te > tb ? (int)(te - tb) : 0;                  // tokens to walk; token i is first + dir i
     const long first = BACK ? te - 1 : tb, dir = BACK ? -1 : 1;
-    const bool ok = c0 + lane < cend;
-    const int ch = ok ? c0 + lane : c0;                          // lanes beyond the group repeat its block's first channel
-    // u; BACK: dout
-    const T *u = BACK ? reinterpret_cast<const T *>(p.dout) + b * p.so.b + ch : reinterpret_cast<const T *>(p.u) + b * p.su.b + ch;
-    const T *dl = reinterpret_cast<const T *>(p.delta) + b * p.sd.b + ch;
+    // Lanes beyond the group repeat its block's first channel, bit for bit: what they store is what that lane stores.
+    const int ch = c0 + lane < cend ? c0 + lane : c0;
+    // Every stream is a uniform running pointer, to the next token to fetch, and the lane's byte offset in a row.
     const bool gated = MODE != SCAN_STATES && p.z != nullptr;
-    const T *z = gated ? reinterpret_cast<const T *>(p.z) + b * p.sz.b + ch : dl;
-    const long ut = BACK ? p.so.t : p.su.t, zt = gated ? p.sz.t : p.sd.t;
-    const int rt = lane / NP, rn = lane % NP;                    // rows: token rt, state rn of every TPI tokens
-    const T *Bp = reinterpret_cast<const T *>(BACK ? p.C : p.B) + b * (BACK ? p.sC.b : p.sB.b) + (long)g * p.N + (rn < p.N ? rn : 0);
-    const T *Cp = reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N + (rn < p.N ? rn : 0);
-    const long Bt = BACK ? p.sC.t : p.sB.t;
-    T *y = reinterpret_cast<T *>(p.y) + (long)b * p.L * p.dim + ch;
+    const unsigned chb = ch * (unsigned)sizeof(T);
+    const long ut = (BACK ? -p.so.t : p.su.t) * (long)sizeof(T), dt = dir * p.sd.t * (long)sizeof(T), zt = gated ? dir * p.sz.t * (long)sizeof(T) : dt;
+    const char *pu = reinterpret_cast<const char *>(BACK ? p.dout : p.u) + ((BACK ? b * p.so.b + first * p.so.t : b * p.su.b + first * p.su.t)) * (long)sizeof(T);
+    const char *pd = reinterpret_cast<const char *>(p.delta) + (b * p.sd.b + first * p.sd.t) * (long)sizeof(T);
+    const char *pz = gated ? reinterpret_cast<const char *>(p.z) + (b * p.sz.b + first * p.sz.t) * (long)sizeof(T) : pd;
+    char *py = reinterpret_cast<char *>(p.y) + ((long)b * p.L + tb) * p.dim * (long)sizeof(T);
+    const long yt = (long)p.dim * sizeof(T);
+    // rows of B and C (BACK: C alone): lane's token rt and state rn of every TPI tokens
+    const int rt = lane / NP, rn = lane % NP;
+    const long Bt = BACK ? -p.sC.t : p.sB.t, Ct = p.sC.t;
+    const T *rowB = reinterpret_cast<const T *>(BACK ? p.C : p.B) + (BACK ? b * p.sC.b + first * p.sC.t : b * p.sB.b + first * p.sB.t) + (long)g * p.N + (rn < p.N ? rn : 0);
+    const T *rowC = reinterpret_cast<const T *>(p.C) + b * p.sC.b + first * p.sC.t + (long)g * p.N + (rn < p.N ? rn : 0);
     const float bias = p.bias ? p.bias[ch] : 0.0f, skip = p.D ? p.D[ch] : 0.0f;
     const bool sp = p.softplus != 0;
 
@@ -62,27 +65,45 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
 
     T rB[RB], rC[RB], fu[G4], fd[G4], fz[G4];
     auto fetch_rows = [&](int i0) {
+        if (i0 + TT <= n) {
 #pragma unroll
-        for (int i = 0; i < RB; ++i) {
-            int k = i0 + i * TPI + rt;
-            k = k < n ? k : n - 1;
-            rB[i] = Bp[(first + dir * k) * Bt];
-            if (FULL) rC[i] = Cp[(first + dir * k) * p.sC.t];
+            for (int i = 0; i < RB; ++i) {
+                rB[i] = rowB[(i0 + i * TPI + rt) * Bt];
+                if (FULL) rC[i] = rowC[(i0 + i * TPI + rt) * Ct];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                const int k = i0 + i * TPI + rt < n ? i0 + i * TPI + rt : n - 1;
+                rB[i] = rowB[k * Bt];
+                if (FULL) rC[i] = rowC[k * Ct];
+            }
         }
     };
-    auto fetch_tokens = [&](int i0) {
+    auto fetch_tokens = [&](int left) {                          // the next min(G4, left) tokens; the last again where there are fewer
+        if (left >= G4) {
 #pragma unroll
-        for (int j = 0; j < G4; ++j) {
-            const int k = i0 + j < n ? i0 + j : n - 1;
-            const long t = first + dir * k;
-            fu[j] = u[t * ut];
-            fd[j] = dl[t * p.sd.t];
-            if (MODE != SCAN_STATES) fz[j] = z[t * zt];
+            for (int j = 0; j < G4; ++j) {
+                fu[j] = *reinterpret_cast<const T *>(pu + chb);
+                fd[j] = *reinterpret_cast<const T *>(pd + chb);
+                if (MODE != SCAN_STATES) fz[j] = *reinterpret_cast<const T *>(pz + chb);
+                pu += ut;
+                pd += dt;
+                pz += zt;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < G4; ++j) {
+                const long k = j < left ? j : left - 1;
+                fu[j] = *reinterpret_cast<const T *>(pu + k * ut + chb);
+                fd[j] = *reinterpret_cast<const T *>(pd + k * dt + chb);
+                if (MODE != SCAN_STATES) fz[j] = *reinterpret_cast<const T *>(pz + k * zt + chb);
+            }
         }
     };
     if (n > 0) {
         fetch_rows(0);
-        fetch_tokens(0);
+        fetch_tokens(n);
     }
     for (int i0 = 0; i0 < n; i0 += TT) {
         const int nt = n - i0 < TT ? n - i0 : TT;
@@ -104,20 +125,20 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
                 gate[j] = gated ? sl : 1.0f;
                 in[j] = uf[j] * (BACK ? gate[j] : st[j]);        // step u, or d
             }
-            if (i0 + i + G4 < n) fetch_tokens(i0 + i + G4);
-            if (FULL && p.keep && i % CK == 0 && ok) {           // the state before token tb + i0 + i
+            if (i0 + i + G4 < n) fetch_tokens(n - (i0 + i + G4));
+            if (FULL && p.keep && i % CK == 0) {           // the state before token tb + i0 + i
                 const int blk = 64 * urnn_scan_ed(NP), cl = ch - g * Dg, cbeg = cl / blk * blk, w = Dg - cbeg < blk ? Dg - cbeg : blk;
                 const long seg = (tb + i0 + i) / CK, segs = (p.L + CK - 1) / CK;
                 store_states<NP>(p.keep + (((long)b * segs + seg) * p.dim + g * Dg + cbeg + keep_rank(cl - cbeg, w, urnn_scan_v(NP))) * NP, 0, NP, true, h);
             }
             auto token = [&](int j) {
-                const float *rowB = s_B + (i + j) * NP, *rowC = s_C + (FULL ? (i + j) * NP : 0);
+                const float *sb = s_B + (i + j) * NP, *sc = s_C + (FULL ? (i + j) * NP : 0);
                 float y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
                 for (int k = 0; k < NP; k += 4) {
-                    const Pack<float, 4> Bv = *reinterpret_cast<const Pack<float, 4> *>(rowB + k);
+                    const Pack<float, 4> Bv = *reinterpret_cast<const Pack<float, 4> *>(sb + k);
                     Pack<float, 4> Cv;
-                    if (FULL) Cv = *reinterpret_cast<const Pack<float, 4> *>(rowC + k);
+                    if (FULL) Cv = *reinterpret_cast<const Pack<float, 4> *>(sc + k);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float a = __builtin_amdgcn_exp2f(st[j] * A2[k + e]);
@@ -131,7 +152,8 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
                 }
                 if (FULL) {
                     const float v = fmaf(skip, uf[j], y0 + y1) * gate[j];
-                    if (ok) y[(tb + i0 + i + j) * p.dim] = from_f<T>(v);
+                    *reinterpret_cast<T *>(py + chb) = from_f<T>(v);
+                    py += yt;
                 } else {
                     total += st[j];
                 }
@@ -148,11 +170,11 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
         __syncthreads();
     }
     if (FULL) {
-        for (long t = tb + n; ok && t < tfull; ++t) y[t * p.dim] = from_f<T>(0.0f);      // rows behind the sequence are zeros
+        for (long t = tb + n; t < tfull; ++t, py += yt) *reinterpret_cast<T *>(py + chb) = from_f<T>(0.0f);      // rows behind the sequence are zeros
         const int last = len > 0 ? (len - 1) / p.CL : 0;         // the chunk that holds the sequence's last token
-        if (p.state_out && ok && chunk == last)
+        if (p.state_out && chunk == last)
             store_states<NP>(p.state_out + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state_out, p.N, 4), h);
-    } else if (ok) {
+    } else {
         p.sum[((long)b * p.chunks + chunk) * p.dim + ch] = total;
         store_states<NP>(p.S + (((long)b * p.chunks + chunk) * p.dim + ch) * NP, 0, NP, true, h);
     }

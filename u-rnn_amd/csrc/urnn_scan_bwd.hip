@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
             for (int e = 0; e < E; ++e) carry[k][e] = ck[k][e] = 0.0f;
             if (sok[k]) {
                 if (chunk + 1 < p.chunks) {
-                    const float *s = p.S + (((long)b * p.chunks + chunk + 1) * p.dim + sch[k]) * NP + q * E;
+                    const float *s = p.S + (((long)b * p.chunks + chunk + 1) * p.pieces * p.dim + sch[k]) * NP + q * E;
 #pragma unroll
                     for (int e = 0; e < E; ++e) carry[k][e] = s[e];
                 } else if (p.dstate_out) {
@@ -421,7 +421,9 @@ __global__ __launch_bounds__(256) void scan_fold_rows_kernel(const float *__rest
     dC[i] = from_f<T>(y);
 }
 
-int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots)
+// Chunks of the time axis, blocks along the batch, and the pieces that a chunk's summary is made of (the summaries are waves of 64
+// channels, which a block of the main pass has four of: they need more chunks to fill the chip).
+int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, int *pieces)
 {
     const int CB = 64 * urnn_scan_ed(urnn_scan_np(N));
     const long cbs = (D + CB - 1) / CB, blocks = (long)B * cbs;
@@ -430,9 +432,12 @@ int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots)
     if (want > most) want = most;
     if (want < 1) want = 1;
     long cl = (L + want - 1) / want;
-    cl = (cl + 31) / 32 * 32;
-    *CL = (int)(cl < 32 ? 32 : cl);
-    const int chunks = (L + *CL - 1) / *CL;
+    cl = (cl + 63) / 64 * 64;
+    *CL = (int)cl;
+    const int chunks = (int)((L + cl - 1) / cl);
+    int m = 1;
+    while (m < 8 && cl % (32 * m) == 0 && cl / (2 * m) >= 64 && blocks * chunks * m < 2048) m *= 2;
+    *pieces = m;
     long s = B;                                                  // several sequences to a block once there are enough blocks
     while (s > 1 && s * cbs * chunks > 1024) s = (s + 1) / 2;
     *slots = (int)s;
@@ -444,10 +449,13 @@ static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, flo
 {
     const int Dg = p.dim / p.G, CB = 64 * urnn_scan_ed(NP), gcbs = (Dg + CB - 1) / CB;
     if (p.chunks > 1) {
-        const hipError_t e = urnn_launch_scan_back_summaries(p, sizeof(T) == 4 ? URNN_F32 : std::is_same<T, bf16_t>::value ? URNN_BF16 : URNN_F16, st);
+        ScanParams ps = p;
+        ps.chunks = p.chunks * p.pieces;
+        ps.CL = p.CL / p.pieces;
+        const hipError_t e = urnn_launch_scan_back_summaries(ps, sizeof(T) == 4 ? URNN_F32 : std::is_same<T, bf16_t>::value ? URNN_BF16 : URNN_F16, st);
         if (e != hipSuccess) return e;
         const long count = (long)p.batch * p.dim * NP;
-        scan_back_carry_kernel<NP><<<dim3((unsigned)((count + 255) / 256)), 256, 0, st>>>(p.A, p.sum, p.S, p.dstate_out, p.dim, p.N, p.chunks, count);
+        scan_back_carry_kernel<NP><<<dim3((unsigned)((count + 255) / 256)), 256, 0, st>>>(p.A, p.sum, p.S, p.dstate_out, p.dim, p.N, ps.chunks, count);
     }
     scan_backward_kernel<T, NP><<<dim3((unsigned)(gcbs * p.G * p.chunks * p.slots)), 256, 0, st>>>(p);
     const long n = (long)p.batch * p.L * p.G * p.N;

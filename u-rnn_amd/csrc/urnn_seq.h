@@ -120,7 +120,7 @@ struct ScanParams {
     float *S;                                        // ... and the state of a chunk that starts from zero [B][chunks][D][NP]
     int batch, L, dim, N, G, chunks, CL, softplus;
     // backward
-    int slots;                                       // blocks along the batch
+    int slots, pieces;                               // blocks along the batch; summaries of a chunk
     int wide;                                        // all (B,L,D) rows start on 16 bytes
     const float *dstate_out;                         // (B,D,N) or NULL
     void *du, *ddelta, *dz;                          // (B,L,D) contiguous
@@ -151,7 +151,7 @@ hipError_t urnn_launch_scan_back_summaries(const ScanParams &p, int dtype, hipSt
 hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st);
 int urnn_scan_chunks(int B, int L, int D, int *CL);
 hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, void *dB, void *dC, int accumulate, hipStream_t st);
-int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots);
+int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, int *pieces);
 
 // ---- short causal convolution ----------------------------------------------------------------------------------------
 struct ConvSeqParams {
