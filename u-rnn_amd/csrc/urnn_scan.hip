@@ -6,10 +6,12 @@
 //
 // Mapping.  A lane is a channel: all of its states stay in registers along the sequence, the sum over states needs no other lane, and
 // the elementwise work (softplus, gate, conversions) is done once.  A wave is 64 adjacent channels of one sequence -- whole 128-byte
-// lines of a 16-bit row per access -- and a block of its own, so that nothing waits for another wave.  B and C rows pass through
-// LDS as fp32, 16 tokens at a time, and are read by all lanes at once; inputs of the next four tokens and the next tile's rows are in
-// flight meanwhile.  What bounds it is the vector unit: per state one exponential (measured: the time of 1.6 to 2 fp32 operations) and
-// four fp32 operations, per token and channel about 45 more.
+// lines of a 16-bit row per access -- and a block of its own, so that nothing waits for another wave and LDS is not used.  A row of B
+// lies across the lanes, a state to a lane; the outer product with the lanes' inputs, B_t[n] (step u), is added to the decayed states by
+// v_mfma_f32_4x4x1 (fp32 as the vector unit's; four states of 64 channels in 8 cycles of the otherwise idle matrix pipe), which
+// broadcasts four values of the row; the sum with C takes the row's values by DPP row_newbcast inside the fma.  Inputs of the next four
+// tokens are in flight meanwhile.  What bounds it is the vector unit: per state one exponential (measured: the time of 1.6 to 2 fp32
+// operations) and three fp32 operations, per token and channel about 45 more.
 //
 // Few long sequences do not fill the chip with B * D / 64 waves: the time axis is cut into chunks (urnn_scan_chunks).  The recurrence
 // is linear, h_end = P h_begin + S with S the state of a chunk that starts from zero and P = exp(A * sum of its steps): one pass
@@ -20,13 +22,25 @@
 
 #include <type_traits>
 
-template <typename T, int NP, int MODE>
-__global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
+// h[k] = (decayed h[k]) + outer product of x (one per lane) with the row's values 4 k .. 4 k + 3: v_mfma_f32_4x4x1, sixteen blocks of four
+// states by four lanes.  The rows of four tokens lie across the lanes of v, NP values after one another; the instruction broadcasts
+// four of them, of token J, to all blocks.
+template <int J, int K, int NP>
+__device__ __forceinline__ void add_outer(const float (&v)[NP < 16 ? 1 : NP / 16], float x, f32x4 (&h)[NP / 4])
 {
-    constexpr int TT = 16, TPI = 64 / NP, RB = TT / TPI, CK = urnn_scan_ck(NP), CB = URNN_SCAN_CB, G4 = 4;
+    if constexpr (K < NP / 4) {
+        constexpr int at = J * NP + 4 * K;
+        h[K] = __builtin_amdgcn_mfma_f32_4x4x1f32(v[at / 64], x, h[K], 4, at % 64 / 4, 0);
+        add_outer<J, K + 1, NP>(v, x, h);
+    }
+}
+
+template <typename T, int NP, int MODE>
+__global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
+{
+    constexpr int CK = urnn_scan_ck(NP), CB = URNN_SCAN_CB, G4 = 4, RV = NP < 16 ? 1 : NP / 16, TPV = NP < 16 ? 4 : 64 / NP;
     constexpr bool FULL = MODE == SCAN_FULL, BACK = MODE == SCAN_BACK;
-    __shared__ alignas(16) float s_B[TT * NP];                   // BACK: the rows of C
-    __shared__ alignas(16) float s_C[FULL ? TT * NP : 4];
+    __shared__ alignas(16) float s_C[FULL ? G4 * NP : 4];
     const int lane = threadIdx.x;
     const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
@@ -38,50 +52,45 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
     const long first = BACK ? te - 1 : tb, dir = BACK ? -1 : 1;
     // Lanes beyond the group repeat its block's first channel, bit for bit: what they store is what that lane stores.
     const int ch = c0 + lane < cend ? c0 + lane : c0;
-    // Every stream is a uniform running pointer, to the next token to fetch, and the lane's byte offset in a row.
+    // Every stream is a uniform running pointer, to the next token to fetch, and the lane's byte offset in a row.  The rows of B and C of
+    // four tokens come as RV values to a lane: value lane + 64 r is state (lane + 64 r) % NP of token (lane + 64 r) / NP.
     const bool gated = MODE != SCAN_STATES && p.z != nullptr;
     const unsigned chb = ch * (unsigned)sizeof(T);
+    const int rn = lane % NP, rt = lane / NP;
+    const bool okr = rn < p.N && rt < G4;
     const long ut = (BACK ? -p.so.t : p.su.t) * (long)sizeof(T), dt = dir * p.sd.t * (long)sizeof(T), zt = gated ? dir * p.sz.t * (long)sizeof(T) : dt;
-    const char *pu = reinterpret_cast<const char *>(BACK ? p.dout : p.u) + ((BACK ? b * p.so.b + first * p.so.t : b * p.su.b + first * p.su.t)) * (long)sizeof(T);
+    const long Bt = p.sB.t * (long)sizeof(T), Ct = dir * p.sC.t * (long)sizeof(T), yt = (long)p.dim * sizeof(T);
+    const char *pu = reinterpret_cast<const char *>(BACK ? p.dout : p.u) + (BACK ? b * p.so.b + first * p.so.t : b * p.su.b + first * p.su.t) * (long)sizeof(T);
     const char *pd = reinterpret_cast<const char *>(p.delta) + (b * p.sd.b + first * p.sd.t) * (long)sizeof(T);
     const char *pz = gated ? reinterpret_cast<const char *>(p.z) + (b * p.sz.b + first * p.sz.t) * (long)sizeof(T) : pd;
+    const char *pB = reinterpret_cast<const char *>(p.B) + (b * p.sB.b + first * p.sB.t + (long)g * p.N) * (long)sizeof(T);
+    const char *pC = reinterpret_cast<const char *>(p.C) + (b * p.sC.b + first * p.sC.t + (long)g * p.N) * (long)sizeof(T);
     char *py = reinterpret_cast<char *>(p.y) + ((long)b * p.L + tb) * p.dim * (long)sizeof(T);
-    const long yt = (long)p.dim * sizeof(T);
-    // rows of B and C (BACK: C alone): lane's token rt and state rn of every TPI tokens
-    const int rt = lane / NP, rn = lane % NP;
-    const long Bt = BACK ? -p.sC.t : p.sB.t, Ct = p.sC.t;
-    const T *rowB = reinterpret_cast<const T *>(BACK ? p.C : p.B) + (BACK ? b * p.sC.b + first * p.sC.t : b * p.sB.b + first * p.sB.t) + (long)g * p.N + (rn < p.N ? rn : 0);
-    const T *rowC = reinterpret_cast<const T *>(p.C) + b * p.sC.b + first * p.sC.t + (long)g * p.N + (rn < p.N ? rn : 0);
     const float bias = p.bias ? p.bias[ch] : 0.0f, skip = p.D ? p.D[ch] : 0.0f;
     const bool sp = p.softplus != 0;
 
-    float A2[NP], h[NP];
+    float A2[NP], h0[NP];
+    f32x4 h[NP / 4];
     load_states<NP>(p.A + (long)ch * p.N, 0, p.N, states_vec(p.A, p.N, 4), A2);
 #pragma unroll
-    for (int k = 0; k < NP; ++k) { A2[k] *= URNN_LOG2E; h[k] = 0.0f; }
-    if (FULL && chunk > 0) load_states<NP>(p.S + (((long)b * p.chunks + chunk - 1) * p.dim + ch) * NP, 0, NP, true, h);
-    else if (!BACK && p.state && chunk == 0) load_states<NP>(p.state + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state, p.N, 4), h);
+    for (int k = 0; k < NP; ++k) { A2[k] *= URNN_LOG2E; h0[k] = 0.0f; }
+    if (FULL && chunk > 0) load_states<NP>(p.S + (((long)b * p.chunks + chunk - 1) * p.dim + ch) * NP, 0, NP, true, h0);
+    else if (!BACK && p.state && chunk == 0) load_states<NP>(p.state + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state, p.N, 4), h0);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) h[k / 4][k % 4] = h0[k];
     float total = 0.0f;                                          // summaries: the chunk's sum of steps
 
-    T rB[RB], rC[RB], fu[G4], fd[G4], fz[G4];
-    auto fetch_rows = [&](int i0) {
-        if (i0 + TT <= n) {
-#pragma unroll
-            for (int i = 0; i < RB; ++i) {
-                rB[i] = rowB[(i0 + i * TPI + rt) * Bt];
-                if (FULL) rC[i] = rowC[(i0 + i * TPI + rt) * Ct];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < RB; ++i) {
-                const int k = i0 + i * TPI + rt < n ? i0 + i * TPI + rt : n - 1;
-                rB[i] = rowB[k * Bt];
-                if (FULL) rC[i] = rowC[k * Ct];
-            }
-        }
-    };
+    const long offr = (okr ? rn : 0) * (long)sizeof(T), offB = (okr ? rt : 0) * Bt + offr, offC = (okr ? rt : 0) * Ct + offr;
+    T fu[G4], fd[G4], fz[G4], fB[RV], fC[RV];
     auto fetch_tokens = [&](int left) {                          // the next min(G4, left) tokens; the last again where there are fewer
         if (left >= G4) {
+#pragma unroll
+            for (int r = 0; r < RV; ++r) {
+                if (!BACK) fB[r] = *reinterpret_cast<const T *>(pB + r * TPV * Bt + offB);
+                if (MODE != SCAN_STATES) fC[r] = *reinterpret_cast<const T *>(pC + r * TPV * Ct + offC);
+            }
+            pB += G4 * Bt;
+            pC += G4 * Ct;
 #pragma unroll
             for (int j = 0; j < G4; ++j) {
                 fu[j] = *reinterpret_cast<const T *>(pu + chb);
@@ -93,6 +102,12 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
             }
         } else {
 #pragma unroll
+            for (int r = 0; r < RV; ++r) {
+                const int t = okr ? r * TPV + rt : 0, k = t < left ? t : left - 1;
+                if (!BACK) fB[r] = *reinterpret_cast<const T *>(pB + k * Bt + offr);
+                if (MODE != SCAN_STATES) fC[r] = *reinterpret_cast<const T *>(pC + k * Ct + offr);
+            }
+#pragma unroll
             for (int j = 0; j < G4; ++j) {
                 const long k = j < left ? j : left - 1;
                 fu[j] = *reinterpret_cast<const T *>(pu + k * ut + chb);
@@ -101,82 +116,76 @@ __global__ __launch_bounds__(64) void scan_kernel(const ScanParams p)
             }
         }
     };
-    if (n > 0) {
-        fetch_rows(0);
-        fetch_tokens(n);
-    }
-    for (int i0 = 0; i0 < n; i0 += TT) {
-        const int nt = n - i0 < TT ? n - i0 : TT;
+    if (n > 0) fetch_tokens(n);
+    for (int i = 0; i < n; i += G4) {
+        float st[G4], in[G4], gate[G4], uf[G4], row[RV];         // row: B's; BACK: C's
 #pragma unroll
-        for (int i = 0; i < RB; ++i) {
-            s_B[(i * TPI) * NP + lane] = rn < p.N ? to_f(rB[i]) : 0.0f;
-            if (FULL) s_C[(i * TPI) * NP + lane] = rn < p.N ? to_f(rC[i]) : 0.0f;
+        for (int r = 0; r < RV; ++r) {
+            row[r] = okr ? to_f(BACK ? fC[r] : fB[r]) : 0.0f;
+            if (FULL && rt < G4) s_C[lane + 64 * r] = okr ? to_f(fC[r]) : 0.0f;
         }
-        __syncthreads();
-        if (i0 + TT < n) fetch_rows(i0 + TT);
-        for (int i = 0; i < nt; i += G4) {
-            float st[G4], in[G4], gate[G4], uf[G4];
+        if (FULL) __syncthreads();                               // one wave: orders the rows' writes before their reads
 #pragma unroll
-            for (int j = 0; j < G4; ++j) {
-                const float raw = to_f(fd[j]) + bias, s = softplus_f(raw);
-                st[j] = sp ? s : raw;
-                uf[j] = to_f(fu[j]);
-                const float sl = MODE == SCAN_STATES ? 1.0f : silu_f(to_f(fz[j]));
-                gate[j] = gated ? sl : 1.0f;
-                in[j] = uf[j] * (BACK ? gate[j] : st[j]);        // step u, or d
-            }
-            if (i0 + i + G4 < n) fetch_tokens(n - (i0 + i + G4));
-            if (FULL && p.keep && i % CK == 0) {           // the state before token tb + i0 + i
-                const int blk = 64 * urnn_scan_ed(NP), cl = ch - g * Dg, cbeg = cl / blk * blk, w = Dg - cbeg < blk ? Dg - cbeg : blk;
-                const long seg = (tb + i0 + i) / CK, segs = (p.L + CK - 1) / CK;
-                store_states<NP>(p.keep + (((long)b * segs + seg) * p.dim + g * Dg + cbeg + keep_rank(cl - cbeg, w, urnn_scan_v(NP))) * NP, 0, NP, true, h);
-            }
-            auto token = [&](int j) {
-                const float *sb = s_B + (i + j) * NP, *sc = s_C + (FULL ? (i + j) * NP : 0);
+        for (int j = 0; j < G4; ++j) {
+            const float raw = to_f(fd[j]) + bias, s = softplus_f(raw);
+            st[j] = sp ? s : raw;
+            uf[j] = to_f(fu[j]);
+            const float sl = MODE == SCAN_STATES ? 1.0f : silu_f(to_f(fz[j]));
+            gate[j] = gated ? sl : 1.0f;
+            in[j] = uf[j] * (BACK ? gate[j] : st[j]);            // step u, or d
+        }
+        if (i + G4 < n) fetch_tokens(n - (i + G4));
+        if (FULL && p.keep && i % CK == 0) {                     // the state before token tb + i
+            const int blk = 64 * urnn_scan_ed(NP), cl = ch - g * Dg, cbeg = cl / blk * blk, w = Dg - cbeg < blk ? Dg - cbeg : blk;
+            const long seg = (tb + i) / CK, segs = (p.L + CK - 1) / CK;
+            f32x4 *k = reinterpret_cast<f32x4 *>(p.keep + (((long)b * segs + seg) * p.dim + g * Dg + cbeg + keep_rank(cl - cbeg, w, urnn_scan_v(NP))) * NP);
+#pragma unroll
+            for (int e = 0; e < NP / 4; ++e) k[e] = h[e];
+        }
+        auto token = [&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            if (BACK) add_outer<j, 0, NP>(row, in[j], h);        // h <- a (h + C d), otherwise h <- a h + B (step u)
+#pragma unroll
+            for (int k = 0; k < NP; ++k) h[k / 4][k % 4] *= __builtin_amdgcn_exp2f(st[j] * A2[k]);
+            if (!BACK) add_outer<j, 0, NP>(row, in[j], h);
+            if (FULL) {
                 float y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
-                for (int k = 0; k < NP; k += 4) {
-                    const Pack<float, 4> Bv = *reinterpret_cast<const Pack<float, 4> *>(sb + k);
-                    Pack<float, 4> Cv;
-                    if (FULL) Cv = *reinterpret_cast<const Pack<float, 4> *>(sc + k);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float a = __builtin_amdgcn_exp2f(st[j] * A2[k + e]);
-                        if (BACK) h[k + e] = a * fmaf(in[j], Bv.v[e], h[k + e]);
-                        else h[k + e] = fmaf(a, h[k + e], in[j] * Bv.v[e]);
-                        if (FULL) {
-                            if (e & 1) y1 = fmaf(Cv.v[e], h[k + e], y1);
-                            else y0 = fmaf(Cv.v[e], h[k + e], y0);
-                        }
-                    }
+                for (int k = 0; k < NP / 4; ++k) {
+                    const f32x4 c = *reinterpret_cast<const f32x4 *>(s_C + j * NP + 4 * k);
+                    y0 = fmaf(c[0], h[k][0], y0);
+                    y1 = fmaf(c[1], h[k][1], y1);
+                    y0 = fmaf(c[2], h[k][2], y0);
+                    y1 = fmaf(c[3], h[k][3], y1);
                 }
-                if (FULL) {
-                    const float v = fmaf(skip, uf[j], y0 + y1) * gate[j];
-                    *reinterpret_cast<T *>(py + chb) = from_f<T>(v);
-                    py += yt;
-                } else {
-                    total += st[j];
-                }
-            };
-            if (i + G4 <= nt) {
-#pragma unroll
-                for (int j = 0; j < G4; ++j) token(j);
+                const float v = fmaf(skip, uf[j], y0 + y1) * gate[j];
+                *reinterpret_cast<T *>(py + chb) = from_f<T>(v);
+                py += yt;
             } else {
-#pragma unroll
-                for (int j = 0; j < G4; ++j)
-                    if (i + j < nt) token(j);
+                total += st[j];
             }
+        };
+        if (i + G4 <= n) {
+            token(std::integral_constant<int, 0>());
+            token(std::integral_constant<int, 1>());
+            token(std::integral_constant<int, 2>());
+            token(std::integral_constant<int, 3>());
+        } else {
+            token(std::integral_constant<int, 0>());
+            if (i + 1 < n) token(std::integral_constant<int, 1>());
+            if (i + 2 < n) token(std::integral_constant<int, 2>());
         }
-        __syncthreads();
     }
+#pragma unroll
+    for (int k = 0; k < NP; ++k) h0[k] = h[k / 4][k % 4];
     if (FULL) {
         for (long t = tb + n; t < tfull; ++t, py += yt) *reinterpret_cast<T *>(py + chb) = from_f<T>(0.0f);      // rows behind the sequence are zeros
         const int last = len > 0 ? (len - 1) / p.CL : 0;         // the chunk that holds the sequence's last token
         if (p.state_out && chunk == last)
-            store_states<NP>(p.state_out + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state_out, p.N, 4), h);
+            store_states<NP>(p.state_out + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state_out, p.N, 4), h0);
     } else {
         p.sum[((long)b * p.chunks + chunk) * p.dim + ch] = total;
-        store_states<NP>(p.S + (((long)b * p.chunks + chunk) * p.dim + ch) * NP, 0, NP, true, h);
+        store_states<NP>(p.S + (((long)b * p.chunks + chunk) * p.dim + ch) * NP, 0, NP, true, h0);
     }
 }
 
@@ -194,7 +203,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
     float *s = S + b * chunks * dim * NP + r;
     const float *w = sum + b * chunks * dim + d;
     float h = s[0];
-    constexpr int U = 8;
+    constexpr int U = 16;
     for (int c0 = 1; c0 < chunks; c0 += U) {
         float sv[U], wv[U];
 #pragma unroll
@@ -215,7 +224,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
 int urnn_scan_chunks(int B, int L, int D, int *CL)
 {
     const long waves = (long)B * ((D + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
-    long want = waves >= 640 ? 1 : (2048 + waves - 1) / waves;
+    long want = waves >= 640 ? 1 : (3000 + waves - 1) / waves;
     const long most = (L + 63) / 64;
     if (want > most) want = most;
     if (want < 1) want = 1;

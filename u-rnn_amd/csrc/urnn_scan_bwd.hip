@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void scan_back_carry_kernel(const float *__res
     float *s = S + b * chunks * dim * NP + r;
     const float *w = sum + b * chunks * dim + d;
     float k = dstate_out && n < N ? dstate_out[(b * dim + d) * N + n] : 0.0f;
-    constexpr int U = 8;
+    constexpr int U = 16;
     for (int c0 = chunks - 1; c0 >= 1; c0 -= U) {
         float sv[U], wv[U];
 #pragma unroll
