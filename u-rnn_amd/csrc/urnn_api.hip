@@ -1677,7 +1677,7 @@ static ScanBackWork scan_back_work(int B, int L, int D, int G, int N)
     ScanBackWork w;
     w.chunks = urnn_scan_backward_chunks(B, L, D, N, &w.CL, &w.slots, &w.pieces);
     const size_t np = urnn_scan_np(N), cb = 64 * urnn_scan_ed((int)np), gcbs = (D / G + cb - 1) / cb, parts = (size_t)w.slots * w.chunks;
-    const size_t rows = align_up(gcbs * B * L * G * N * sizeof(float), 256), cross = w.chunks > 1 ? (size_t)w.chunks * w.pieces : 0;
+    const size_t rows = gcbs > 1 ? align_up(gcbs * B * L * G * N * sizeof(float), 256) : 0, cross = w.chunks > 1 ? (size_t)w.chunks * w.pieces : 0;
     w.sum = 0;
     w.S = align_up((size_t)B * cross * D * sizeof(float), 256);
     w.dB = w.S + align_up((size_t)B * cross * D * np * sizeof(float), 256);
@@ -1707,6 +1707,9 @@ extern "C" int urnn_selective_scan_backward(const void *u, const void *delta, co
     if (!aligned16(workspace) || !aligned16(record)) return fail(URNN_EALIGN, "urnn_selective_scan_backward: workspace / record not 16-byte aligned");
     const ScanWork f = scan_work(B, L, D, N, 1);
     if (record_bytes < f.total) return fail(URNN_EWORKSPACE, "urnn_selective_scan_backward: the record is too small for a forward with keep");
+    for (int k = 1; L > 1 && k < 12; k += 2)                     // the kernel's offsets within a segment of eight tokens are of 32 bits
+        if (strides[k] < 0 || (k != 9 || z ? ((double)strides[k] * 7 + D + 64) * seq_elem(dtype) : 0.0) >= 4294967296.0)
+            return fail(URNN_EINVAL, "urnn_selective_scan_backward: a token stride of %ld elements is beyond 4 GB in eight tokens", strides[k]);
     const ScanBackWork w = scan_back_work(B, L, D, G, N);
     if (workspace_bytes < w.total) return fail(URNN_EWORKSPACE, "urnn_selective_scan_backward: workspace too small");
     char *base = reinterpret_cast<char *>(workspace);
@@ -1719,13 +1722,13 @@ extern "C" int urnn_selective_scan_backward(const void *u, const void *delta, co
     p.sum = reinterpret_cast<float *>(base + w.sum); p.S = reinterpret_cast<float *>(base + w.S);
     p.dBp = reinterpret_cast<float *>(base + w.dB); p.dCp = reinterpret_cast<float *>(base + w.dC);
     p.dAp = reinterpret_cast<float *>(base + w.sums);
-    p.du = du; p.ddelta = ddelta; p.dz = dz; p.dstate = dstate;
+    p.du = du; p.ddelta = ddelta; p.dz = dz; p.dstate = dstate; p.dB = dB; p.dC = dC; p.direct = w.dB == w.dC;
     p.batch = B; p.L = L; p.dim = D; p.N = N; p.G = G; p.softplus = softplus;
     p.chunks = w.chunks; p.CL = w.CL; p.slots = w.slots; p.pieces = w.pieces;
     const int e = seq_elem(dtype);
     p.wide = wide_rows(u, strides[0], strides[1], e) && wide_rows(delta, strides[2], strides[3], e) && wide_rows(z, strides[8], strides[9], e) &&
              wide_rows(dout, strides[10], strides[11], e) && (long)D / G * e % 16 == 0 && aligned16(du) && aligned16(ddelta) && (!z || aligned16(dz));
-    CHECK_HIP(urnn_launch_scan_backward(p, dtype, dA, dskip, ddelta_bias, dB, dC, accumulate, (hipStream_t)stream), "selective_scan_backward");
+    CHECK_HIP(urnn_launch_scan_backward(p, dtype, dA, dskip, ddelta_bias, accumulate, (hipStream_t)stream), "selective_scan_backward");
     return URNN_OK;
 }
 

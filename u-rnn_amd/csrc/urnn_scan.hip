@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
         }
         if (i + G4 < n) fetch_tokens(n - (i + G4));
         if (FULL && p.keep && i % CK == 0) {                     // the state before token tb + i
-            const int blk = 64 * urnn_scan_ed(NP), cl = ch - g * Dg, cbeg = cl / blk * blk, w = Dg - cbeg < blk ? Dg - cbeg : blk;
+            const int blk = 16 * urnn_scan_ed(NP), cl = ch - g * Dg, cbeg = cl / blk * blk, w = Dg - cbeg < blk ? Dg - cbeg : blk;
             const long seg = (tb + i) / CK, segs = (p.L + CK - 1) / CK;
             f32x4 *k = reinterpret_cast<f32x4 *>(p.keep + (((long)b * segs + seg) * p.dim + g * Dg + cbeg + keep_rank(cl - cbeg, w, urnn_scan_v(NP))) * NP);
 #pragma unroll

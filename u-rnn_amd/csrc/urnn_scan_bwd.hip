@@ -44,8 +44,8 @@ __device__ __forceinline__ void channel_sums(const float (&v)[2 * E], float (&r)
     for (int m = 0; m < E / 2; ++m) r[m] = add_swapped16(s[2 * m], s[2 * m + 1]);
 #pragma unroll
     for (int m = 0; m < (E < 2 ? 1 : E / 2); ++m) {
-        r[m] += dpp_move<0x128>(r[m]);               // row_ror:8
-        r[m] += dpp_move<0x124>(r[m]);               // row_ror:4
+        r[m] += dpp_all<0x128>(r[m]);                // row_ror:8
+        r[m] += dpp_all<0x124>(r[m]);                // row_ror:4
     }
 }
 
@@ -82,26 +82,28 @@ __global__ __launch_bounds__(256) void scan_back_carry_kernel(const float *__res
 
 // V adjacent channels of a token as they lie in memory: they wait in registers for a whole tile, two 16-bit values to a register.
 template <typename T, int V> struct Raw {
-    unsigned w[V * sizeof(T) / 4];
+    static constexpr int WORDS = V * sizeof(T) < 4 ? 1 : V * sizeof(T) / 4;
+    unsigned w[WORDS];
     __device__ __forceinline__ float get(int i) const
     {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
         else return to_f(__builtin_bit_cast(T, (unsigned short)(w[i / 2] >> (16 * (i & 1)))));
     }
-    // channels from `valid` on as zeros; wide: rows start on 16 bytes and all V are there
-    __device__ __forceinline__ void load(const T *src, int valid, bool wide)
+    // channels from `valid` on as zeros; WIDE: rows start on 16 bytes and all V are there
+    template <bool WIDE> __device__ __forceinline__ void load(const void *from, int valid)
     {
-        if (wide) {
-            constexpr int W = V * sizeof(T) / 4 < 4 ? V * sizeof(T) / 4 : 4;
+        const T *src = reinterpret_cast<const T *>(from);
+        if constexpr (WIDE && V * sizeof(T) >= 4) {
+            constexpr int W = WORDS < 4 ? WORDS : 4;
 #pragma unroll
-            for (int k = 0; k < (int)(V * sizeof(T) / 4); k += W) {
+            for (int k = 0; k < WORDS; k += W) {
                 const Pack<unsigned, W> t = *reinterpret_cast<const Pack<unsigned, W> *>(reinterpret_cast<const unsigned *>(src) + k);
 #pragma unroll
                 for (int i = 0; i < W; ++i) w[k + i] = t.v[i];
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < (int)(V * sizeof(T) / 4); ++k) w[k] = 0;
+            for (int k = 0; k < WORDS; ++k) w[k] = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (i < valid) {
@@ -111,11 +113,12 @@ template <typename T, int V> struct Raw {
         }
     }
 };
-template <typename T, int V>
-__device__ __forceinline__ void store_channels(T *dst, int valid, bool wide, const float (&v)[V])
+template <typename T, int V, bool WIDE>
+__device__ __forceinline__ void store_channels(void *to, int valid, const float (&v)[V])
 {
+    T *dst = reinterpret_cast<T *>(to);
     constexpr int W = V * sizeof(T) < 16 ? V : 16 / sizeof(T);
-    if (wide) {
+    if constexpr (WIDE) {
 #pragma unroll
         for (int k = 0; k < V; k += W) {
             Pack<T, W> t;
@@ -130,45 +133,71 @@ __device__ __forceinline__ void store_channels(T *dst, int valid, bool wide, con
     }
 }
 
-template <typename T, int NP>
+// A wave's LDS is its own: its operations are done in order, this keeps the compiler's in order as well.
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int NP, bool WIDE>
 __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams p)
 {
-    constexpr int E = NP / 4, W = E < 4 ? E : 4, ED = urnn_scan_ed(NP), CK = urnn_scan_ck(NP), CB = 64 * ED, TT = urnn_scan_tt(NP);
-    constexpr int V = urnn_scan_v(NP), CG = CB / V, RB = TT * NP / 256 < 1 ? 1 : TT * NP / 256;
-    __shared__ alignas(16) Pack<float, 4> s_io[TT * CB];         // in: (step, step u, d, -); out: (sum w A log2 e, sum k B, sum C h, step)
-    __shared__ alignas(16) float s_B[TT * NP], s_C[TT * NP];
-    __shared__ float s_bc[4 * TT * 2 * NP];                      // [wave][token][dB | dC]
+    constexpr int E = NP / 4, W = E < 4 ? E : 4, ED = urnn_scan_ed(NP), CK = urnn_scan_ck(NP), CW = 16 * ED, CB = 4 * CW;
+    constexpr int HT = CK / 2;                                   // tokens whose decays and states are in registers at a time
+    constexpr int V = urnn_scan_v(NP), CG = CW / V, RB = CK * NP < 64 ? 1 : CK * NP / 64;
+    static_assert(CG * CK == 64, "a wave's lanes are the tokens of a segment by groups of V channels");
+    __shared__ alignas(16) Pack<float, 4> s_io[4][CK * CW];      // in: (step, step u, d, -); out: (sum w A log2 e, sum k B, sum C h, step)
+    __shared__ alignas(16) float s_row[4][2][CK * NP];           // B, C
+    __shared__ float s_bc[2][4][CK][2 * NP];                     // [turn][wave][token][dB | dC]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane & 3;
     const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
     const int chunk = blockIdx.x / (cbs * p.G) % p.chunks, slot = blockIdx.x / (cbs * p.G) / p.chunks;
-    const long segs = (p.L + CK - 1) / CK;
-    const int width = cend - c0 < CB ? cend - c0 : CB;
+    const int segs = (p.L + CK - 1) / CK;
+    const int w0 = c0 + wave * CW;                               // the wave's first channel
+    const int width = cend - w0 < CW ? (cend > w0 ? cend - w0 : 0) : CW;
     const bool sp = p.softplus != 0;
+    Pack<float, 4> *const io = s_io[wave];
+    float *const rowB = s_row[wave][0], *const rowC = s_row[wave][1];
 
-    // elementwise: token lt of a tile, channels c0 + V lg ..  Channel V lg + i has its slot at i CG + lg of the token's row, so that the
-    // threads of a token write side by side.
-    const int lg = tid % CG, lt = tid / CG;
+    // elementwise: token lt of a segment, channels w0 + V lg ..  Channel V lg + i has its slot at i CG + lg of the token's row, so that
+    // the threads of a token write side by side.
+    const int lg = lane % CG, lt = lane / CG;
     const int evalid = width - V * lg;                           // channels there, of V
-    const bool eok = evalid > 0, ewide = p.wide && evalid >= V;
-    const int ech = c0 + (eok ? V * lg : 0);
-    float bias[V], skip[V];
+    const bool eok = evalid > 0;
+    const int ech = eok ? w0 + V * lg : c0;
+    // the lane's bias and skip, and its sums for their gradients: in LDS, where they cost no registers in between
+    typedef Pack<float, V> Chan;
+    __shared__ alignas(16) Chan s_par[4][4][64];
+    Chan *const par = &s_par[wave][0][lane];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        bias[i] = p.bias && i < evalid ? p.bias[ech + i] : 0.0f;
-        skip[i] = p.D && i < evalid ? p.D[ech + i] : 0.0f;
+        par[0].v[i] = p.bias && i < evalid ? p.bias[ech + i] : 0.0f;
+        par[64].v[i] = p.D && i < evalid ? p.D[ech + i] : 0.0f;
+        par[128].v[i] = par[192].v[i] = 0.0f;
     }
+    const bool gated = p.z != nullptr;
+    // Addresses: a uniform pointer to a segment's first token, and the lane's byte offset from there in 32 bits (the host checks that
+    // CK tokens are within 4 GB).
+    constexpr long TS = sizeof(T);
+    const unsigned cho = ech * (unsigned)TS, ou = lt * (unsigned)(p.su.t * TS) + cho, od = lt * (unsigned)(p.sd.t * TS) + cho;
+    const unsigned oo = lt * (unsigned)(p.so.t * TS) + cho, oz = gated ? lt * (unsigned)(p.sz.t * TS) + cho : 0;
+    const unsigned oy = lt * (unsigned)(p.dim * TS) + cho;
+    const int rn = lane % NP, rt = lane / NP;                    // rows of B, C: values lane + 64 i, token rt + 64 / NP i, state rn
+    const bool rok = rn < p.N && rt < CK;
+    const unsigned oB = (rok ? rt : 0) * (unsigned)(p.sB.t * TS) + (rok ? rn : 0) * (unsigned)TS, oC = (rok ? rt : 0) * (unsigned)(p.sC.t * TS) + (rok ? rn : 0) * (unsigned)TS;
     // scan: slots sc[k] of a row, states q E ..
     int sc[ED], sch[ED], srank[ED];
     bool sok[ED];
     float A2[ED][E], dA[ED][E];
 #pragma unroll
     for (int k = 0; k < ED; ++k) {
-        sc[k] = wave * 16 * ED + 16 * k + (lane >> 2);
+        sc[k] = 16 * k + (lane >> 2);
         const int c = sc[k] % CG * V + sc[k] / CG;               // the slot's channel
         sok[k] = c < width;
-        sch[k] = c0 + (sok[k] ? c : 0);
-        srank[k] = c0 + keep_rank(sok[k] ? c : 0, width, V);
+        sch[k] = sok[k] ? w0 + c : c0;
+        srank[k] = sok[k] ? w0 + keep_rank(c, width, V) : c0;
         load_states<E>(p.A + (long)sch[k] * p.N, q, p.N, states_vec(p.A, p.N, W), A2[k]);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -177,234 +206,277 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
             dA[k][e] = 0.0f;
         }
     }
-    float dD[V] = {}, dbias[V] = {};
+
+    const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L;
+    auto end_of = [&](int b) -> long {                           // behind the last token of sequence b in this chunk; tb: none
+        const int len = __builtin_amdgcn_readfirstlane(seq_len(p.lengths, b, p.L));
+        return tfull < len ? tfull : (len > tb ? len : tb);
+    };
+    // what is fetched ahead: a segment's inputs and the state before it
+    Raw<T, V> ru = {}, rd = {}, rz = {}, ro = {};
+    T rB[RB] = {}, rC[RB] = {};
+    float ck[ED][E] = {};
+    const char *qu, *qd, *qz, *qo, *qB, *qC;                     // the segment to fetch next
+    const float *qk = nullptr;
+    int qn = 0;                                                  // its tokens
+    auto fetch = [&]() {
+        if (eok && lt < qn) {
+            ru.template load<WIDE>(qu + ou, evalid);
+            rd.template load<WIDE>(qd + od, evalid);
+            ro.template load<WIDE>(qo + oo, evalid);
+            if (gated) rz.template load<WIDE>(qz + oz, evalid);
+        }
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+            rB[i] = rC[i] = T(0.0f);
+            if (rok && rt + 64 / NP * i < qn) {
+                rB[i] = *reinterpret_cast<const T *>(qB + 64 / NP * i * p.sB.t * TS + oB);
+                rC[i] = *reinterpret_cast<const T *>(qC + 64 / NP * i * p.sC.t * TS + oC);
+            }
+        }
+        qn = CK;                                                 // the ones before are whole
+        qu -= CK * p.su.t * TS;
+        qd -= CK * p.sd.t * TS;
+        qo -= CK * p.so.t * TS;
+        qz -= CK * p.sz.t * TS;
+        qB -= CK * p.sB.t * TS;
+        qC -= CK * p.sC.t * TS;
+    };
+    auto fetch_states = [&]() {
+#pragma unroll
+        for (int k = 0; k < ED; ++k)
+            if (sok[k]) load_states<E>(qk + (long)srank[k] * NP, q, NP, true, ck[k]);
+        qk -= (long)p.dim * NP;
+    };
+    // the last segment of the next sequence that has one
+    auto fetch_sequence = [&](int b) {
+        for (; b < p.batch; b += p.slots) {
+            const long te = end_of(b);
+            if (te > tb) {
+                const long t0 = tb + (te - 1 - tb) / CK * CK;
+                qn = (int)(te - t0);
+                qu = reinterpret_cast<const char *>(p.u) + (b * p.su.b + t0 * p.su.t) * TS;
+                qd = reinterpret_cast<const char *>(p.delta) + (b * p.sd.b + t0 * p.sd.t) * TS;
+                qo = reinterpret_cast<const char *>(p.dout) + (b * p.so.b + t0 * p.so.t) * TS;
+                qz = gated ? reinterpret_cast<const char *>(p.z) + (b * p.sz.b + t0 * p.sz.t) * TS : qu;
+                qB = reinterpret_cast<const char *>(p.B) + (b * p.sB.b + t0 * p.sB.t + (long)g * p.N) * TS;
+                qC = reinterpret_cast<const char *>(p.C) + (b * p.sC.b + t0 * p.sC.t + (long)g * p.N) * TS;
+                qk = p.keep + ((long)b * segs + t0 / CK) * p.dim * NP;
+                fetch();
+                return;
+            }
+        }
+        qk = nullptr;                                            // no further segment
+    };
+    fetch_sequence(slot);
+    if (qk) fetch_states();
+    int turn = 0;
 
     for (int b = slot; b < p.batch; b += p.slots) {
-        const int len = __builtin_amdgcn_readfirstlane(seq_len(p.lengths, b, p.L));
-        const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L, te = tfull < len ? tfull : len;
-        const T *u = reinterpret_cast<const T *>(p.u) + b * p.su.b + ech, *dl = reinterpret_cast<const T *>(p.delta) + b * p.sd.b + ech;
-        const T *z = p.z ? reinterpret_cast<const T *>(p.z) + b * p.sz.b + ech : nullptr, *dout = reinterpret_cast<const T *>(p.dout) + b * p.so.b + ech;
-        const T *Bp = reinterpret_cast<const T *>(p.B) + b * p.sB.b + (long)g * p.N, *Cp = reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N;
-        const long base = (long)b * p.L * p.dim + ech;
-        T *du = reinterpret_cast<T *>(p.du) + base, *ddl = reinterpret_cast<T *>(p.ddelta) + base, *dz = reinterpret_cast<T *>(p.dz) + base;
-        // partial rows of this channel block: [cb in group][b][t][g][n]
-        const long prow = ((long)(cb % cbs) * p.batch + b) * p.L;
-        float *dBp = p.dBp + (prow * p.G + g) * p.N, *dCp = p.dCp + (prow * p.G + g) * p.N;
-        const long pt = (long)p.G * p.N;
-
-        float carry[ED][E], ck[ED][E];
+        const long te = end_of(b);
+        // rows of dB and dC: this channel block's partial ones, or the results where the group is one block
+        const long prow = p.direct ? (long)b * p.L : ((long)(cb % cbs) * p.batch + b) * p.L;
+        auto put_bc = [&](int which, long t, int n, float v) {
+            const long at = ((prow + t) * p.G + g) * p.N + n;
+            if (p.direct) reinterpret_cast<T *>(which ? p.dC : p.dB)[at] = from_f<T>(v);
+            else (which ? p.dCp : p.dBp)[at] = v;
+        };
+        float carry[ED][E];
 #pragma unroll
         for (int k = 0; k < ED; ++k) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) carry[k][e] = ck[k][e] = 0.0f;
+            for (int e = 0; e < E; ++e) carry[k][e] = 0.0f;
             if (sok[k]) {
                 if (chunk + 1 < p.chunks) {
-                    const float *s = p.S + (((long)b * p.chunks + chunk + 1) * p.pieces * p.dim + sch[k]) * NP + q * E;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) carry[k][e] = s[e];
+                    load_states<E>(p.S + (((long)b * p.chunks + chunk + 1) * p.pieces * p.dim + sch[k]) * NP, q, NP, true, carry[k]);
                 } else if (p.dstate_out) {
                     load_states<E>(p.dstate_out + ((long)b * p.dim + sch[k]) * p.N, q, p.N, states_vec(p.dstate_out, p.N, W), carry[k]);
                 }
             }
         }
-        auto load_ck = [&](long seg) {
+        for (long t0 = tb + (te - 1 - tb) / CK * CK; t0 >= tb && t0 < te; t0 -= CK, turn ^= 1) {
+            const int nt = te - t0 < CK ? (int)(te - t0) : CK;
+            const Raw<T, V> cu = ru, cd = rd, cz = rz, co = ro;
+            const bool here = eok && lt < nt;                    // tokens behind the sequence: steps of zero, which change nothing
+            const Chan bias = par[0];
 #pragma unroll
-            for (int k = 0; k < ED; ++k)
-                if (sok[k]) load_states<E>(p.keep + (((long)b * segs + seg) * p.dim + srank[k]) * NP, q, NP, true, ck[k]);
-        };
-        Raw<T, V> ru = {}, rd = {}, rz = {}, ro = {};
-        T rB[RB] = {}, rC[RB] = {};
-        auto fetch = [&](long t0) {
-            const long t = t0 + lt;
-            if (eok && t < te) {
-                ru.load(u + t * p.su.t, evalid, ewide);
-                rd.load(dl + t * p.sd.t, evalid, ewide);
-                ro.load(dout + t * p.so.t, evalid, ewide);
-                if (z) rz.load(z + t * p.sz.t, evalid, ewide);
+            for (int i = 0; i < V; ++i) {
+                const float raw = cd.get(i) + bias.v[i], s = softplus_f(raw), step = here ? (sp ? s : raw) : 0.0f;
+                const float d = co.get(i) * (gated ? silu_f(cz.get(i)) : 1.0f);
+                io[lt * CW + i * CG + lg] = {{step, here ? step * cu.get(i) : 0.0f, here ? d : 0.0f, 0.0f}};
             }
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
-                const int k = tid + 256 * i, n = k % NP;
-                const long tr = t0 + k / NP;
-                rB[i] = rC[i] = T(0.0f);
-                if (k < TT * NP && n < p.N && tr < te) {
-                    rB[i] = Bp[tr * p.sB.t + n];
-                    rC[i] = Cp[tr * p.sC.t + n];
+                if (lane + 64 * i < CK * NP) {
+                    rowB[lane + 64 * i] = to_f(rB[i]);
+                    rowC[lane + 64 * i] = to_f(rC[i]);
                 }
             }
-        };
-        if (tb < te) {
-            long t0 = tb + (te - 1 - tb) / TT * TT;
-            load_ck((te - 1) / CK);
-            fetch(t0);
-            for (; t0 >= tb; t0 -= TT) {
-                const int nt = te - t0 < TT ? (int)(te - t0) : TT;
-                const Raw<T, V> cu = ru, cd = rd, cz = rz, co = ro;
-                const bool here = eok && lt < nt;                // tokens behind the sequence: steps of zero, which change nothing
+            wave_fence();
+            if (t0 - CK >= tb) fetch();
+            else fetch_sequence(b + p.slots);
+
+            float a[HT][ED][E], ah[HT][ED][E], h[ED][E];
+            auto forward = [&](int j0) {                         // HT tokens from j0 on: h, and what the way back needs of them
+#pragma unroll
+                for (int j = 0; j < HT; ++j) {
+                    float Bv[E];
+#pragma unroll
+                    for (int e = 0; e < E; e += W) {
+                        const Pack<float, W> v = *reinterpret_cast<const Pack<float, W> *>(rowB + (j0 + j) * NP + q * E + e);
+#pragma unroll
+                        for (int i = 0; i < W; ++i) Bv[e + i] = v.v[i];
+                    }
+#pragma unroll
+                    for (int k = 0; k < ED; ++k) {
+                        const Pack<float, 2> in = *reinterpret_cast<const Pack<float, 2> *>(io + (j0 + j) * CW + sc[k]);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            a[j][k][e] = __builtin_amdgcn_exp2f(in.v[0] * A2[k][e]);
+                            ah[j][k][e] = a[j][k][e] * h[k][e];
+                            h[k][e] = fmaf(in.v[1], Bv[e], ah[j][k][e]);
+                        }
+                    }
+                }
+            };
+            auto from_checkpoint = [&]() {
+#pragma unroll
+                for (int k = 0; k < ED; ++k)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) h[k][e] = ck[k][e];
+            };
+            auto backward = [&](int j0) {
+#pragma unroll
+                for (int j = HT - 1; j >= 0; --j) {
+                    float Bv[E], Cv[E], v[2 * E] = {};           // v: dB's terms, then dC's
+#pragma unroll
+                    for (int e = 0; e < E; e += W) {
+                        const Pack<float, W> vb = *reinterpret_cast<const Pack<float, W> *>(rowB + (j0 + j) * NP + q * E + e);
+                        const Pack<float, W> vc = *reinterpret_cast<const Pack<float, W> *>(rowC + (j0 + j) * NP + q * E + e);
+#pragma unroll
+                        for (int i = 0; i < W; ++i) { Bv[e + i] = vb.v[i]; Cv[e + i] = vc.v[i]; }
+                    }
+#pragma unroll
+                    for (int k = 0; k < ED; ++k) {
+                        const Pack<float, 4> in = io[(j0 + j) * CW + sc[k]];
+                        float SW = 0.0f, SG = 0.0f, SY = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const float kk = fmaf(Cv[e], in.v[2], carry[k][e]), hj = fmaf(in.v[1], Bv[e], ah[j][k][e]), w = kk * ah[j][k][e];
+                            SW = fmaf(w, A2[k][e], SW);
+                            SG = fmaf(kk, Bv[e], SG);
+                            SY = fmaf(Cv[e], hj, SY);
+                            dA[k][e] = fmaf(w, in.v[0], dA[k][e]);
+                            v[e] = fmaf(kk, in.v[1], v[e]);
+                            v[E + e] = fmaf(hj, in.v[2], v[E + e]);
+                            carry[k][e] = a[j][k][e] * kk;
+                        }
+                        SW = quad_sum(SW);
+                        SG = quad_sum(SG);
+                        SY = quad_sum(SY);
+                        io[(j0 + j) * CW + sc[k]] = {{SW, SG, SY, in.v[0]}};       // the same from all four lanes
+                    }
+                    float r[E < 2 ? 1 : E / 2];
+                    channel_sums<E>(v, r);
+                    float *o = s_bc[turn][wave][j0 + j];
+                    const int rho = lane >> 4, qr = (lane >> 2) & 3;
+                    if (E == 1) {
+                        o[(lane >> 5) * NP + q] = r[0];          // every quad of a row has its sums: all of them write
+                    } else {
+                        const int in4 = ((rho & 1) << 1) | (rho >> 1);
+                        constexpr int M = E / 2 < 4 ? E / 2 : 4;
+#pragma unroll
+                        for (int m0 = 0; m0 < E / 2; m0 += M) {
+                            float val = r[m0];
+#pragma unroll
+                            for (int m = 1; m < M; ++m) val = (qr & (M - 1)) == m ? r[m0 + m] : val;
+                            const int idx = 4 * (m0 + (qr & (M - 1))) + in4;     // value: dB of state q E + idx, or dC from E on
+                            o[(idx / E) * NP + q * E + idx % E] = val;
+                        }
+                    }
+                }
+            };
+            from_checkpoint();
+            if (nt > HT) {
+                forward(0);
+                forward(HT);
+                backward(HT);
+                from_checkpoint();
+            }
+            forward(0);
+            if (qk) fetch_states();
+            backward(0);
+            wave_fence();
+            if (here) {
+                float odz[V], odd[V], odu[V];
+                const Chan bias = par[0], skip = par[64];
+                Chan dD = par[128], db = par[192];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float raw = cd.get(i) + bias[i], s = softplus_f(raw), step = here ? (sp ? s : raw) : 0.0f;
-                    const float d = co.get(i) * (z ? silu_f(cz.get(i)) : 1.0f);
-                    s_io[lt * CB + i * CG + lg] = {{step, here ? step * cu.get(i) : 0.0f, here ? d : 0.0f, 0.0f}};
-                }
-#pragma unroll
-                for (int i = 0; i < RB; ++i) {
-                    const int k = tid + 256 * i;
-                    if (k < TT * NP) { s_B[k] = to_f(rB[i]); s_C[k] = to_f(rC[i]); }
-                }
-                __syncthreads();
-                if (t0 - TT >= tb) fetch(t0 - TT);
-
-                for (int s0 = (nt - 1) / CK * CK; s0 >= 0; s0 -= CK) {
-                    float a[CK][ED][E], ah[CK][ED][E], h[ED][E];
-#pragma unroll
-                    for (int k = 0; k < ED; ++k)
-#pragma unroll
-                        for (int e = 0; e < E; ++e) h[k][e] = ck[k][e];
-                    if (t0 + s0 > tb) load_ck((t0 + s0) / CK - 1);
-#pragma unroll
-                    for (int j = 0; j < CK; ++j) {
-                        {
-                            const int t = s0 + j;
-                            float Bv[E];
-#pragma unroll
-                            for (int e = 0; e < E; e += W) {
-                                const Pack<float, W> v = *reinterpret_cast<const Pack<float, W> *>(s_B + t * NP + q * E + e);
-#pragma unroll
-                                for (int i = 0; i < W; ++i) Bv[e + i] = v.v[i];
-                            }
-#pragma unroll
-                            for (int k = 0; k < ED; ++k) {
-                                const Pack<float, 2> in = *reinterpret_cast<const Pack<float, 2> *>(s_io + t * CB + sc[k]);
-#pragma unroll
-                                for (int e = 0; e < E; ++e) {
-                                    a[j][k][e] = __builtin_amdgcn_exp2f(in.v[0] * A2[k][e]);
-                                    ah[j][k][e] = a[j][k][e] * h[k][e];
-                                    h[k][e] = fmaf(in.v[1], Bv[e], ah[j][k][e]);
-                                }
-                            }
-                        }
+                    const Pack<float, 4> r = io[lt * CW + i * CG + lg];
+                    const float raw = cd.get(i) + bias.v[i], uf = cu.get(i), of = co.get(i);
+                    float d = of;
+                    if (gated) {
+                        const float zf = cz.get(i), sg = sigmoid_f(zf);
+                        d = of * zf * sg;
+                        odz[i] = of * fmaf(skip.v[i], uf, r.v[2]) * sg * fmaf(zf, 1.0f - sg, 1.0f);
                     }
-#pragma unroll
-                    for (int j = CK - 1; j >= 0; --j) {
-                        {
-                            const int t = s0 + j;
-                            float Bv[E], Cv[E], v[2 * E] = {};               // v: dB's terms, then dC's
-#pragma unroll
-                            for (int e = 0; e < E; e += W) {
-                                const Pack<float, W> vb = *reinterpret_cast<const Pack<float, W> *>(s_B + t * NP + q * E + e);
-                                const Pack<float, W> vc = *reinterpret_cast<const Pack<float, W> *>(s_C + t * NP + q * E + e);
-#pragma unroll
-                                for (int i = 0; i < W; ++i) { Bv[e + i] = vb.v[i]; Cv[e + i] = vc.v[i]; }
-                            }
-#pragma unroll
-                            for (int k = 0; k < ED; ++k) {
-                                const Pack<float, 4> in = s_io[t * CB + sc[k]];
-                                float SW = 0.0f, SG = 0.0f, SY = 0.0f;
-#pragma unroll
-                                for (int e = 0; e < E; ++e) {
-                                    const float kk = fmaf(Cv[e], in.v[2], carry[k][e]), hj = fmaf(in.v[1], Bv[e], ah[j][k][e]), w = kk * ah[j][k][e];
-                                    SW = fmaf(w, A2[k][e], SW);
-                                    SG = fmaf(kk, Bv[e], SG);
-                                    SY = fmaf(Cv[e], hj, SY);
-                                    dA[k][e] = fmaf(w, in.v[0], dA[k][e]);
-                                    v[e] = fmaf(kk, in.v[1], v[e]);
-                                    v[E + e] = fmaf(hj, in.v[2], v[E + e]);
-                                    carry[k][e] = a[j][k][e] * kk;
-                                }
-                                SW = quad_sum(SW);
-                                SG = quad_sum(SG);
-                                SY = quad_sum(SY);
-                                if (q == 0) s_io[t * CB + sc[k]] = {{SW, SG, SY, in.v[0]}};
-                            }
-                            float r[E < 2 ? 1 : E / 2];
-                            channel_sums<E>(v, r);
-                            float *o = s_bc + (wave * TT + t) * 2 * NP;
-                            const int rho = lane >> 4, qr = (lane >> 2) & 3;
-                            if (E == 1) {
-                                if ((lane & 31) < 4) o[(lane >> 5) * NP + q] = r[0];
-                            } else {
-                                const int in4 = ((rho & 1) << 1) | (rho >> 1);
-#pragma unroll
-                                for (int m0 = 0; m0 < E / 2; m0 += 4) {
-                                    float val = r[m0];
-#pragma unroll
-                                    for (int m = m0 + 1; m < m0 + 4 && m < E / 2; ++m) val = qr == m - m0 ? r[m] : val;
-                                    const int idx = 4 * (m0 + qr) + in4;       // value: dB of state q E + idx, or dC from E on
-                                    if (m0 + qr < E / 2) o[(idx / E) * NP + q * E + idx % E] = val;
-                                }
-                            }
-                        }
-                    }
+                    const float dstep = fmaf(r.v[0], URNN_LN2, r.v[1] * uf), dd = dstep * (sp ? sigmoid_f(raw) : 1.0f);
+                    odd[i] = dd;
+                    odu[i] = fmaf(r.v[1], r.v[3], d * skip.v[i]);
+                    dD.v[i] = fmaf(d, uf, dD.v[i]);
+                    db.v[i] += dd;
                 }
-                __syncthreads();
-                if (eok && lt < nt) {
-                    float odz[V], odd[V], odu[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const Pack<float, 4> r = s_io[lt * CB + i * CG + lg];
-                        const float raw = cd.get(i) + bias[i], uf = cu.get(i), of = co.get(i);
-                        float d = of;
-                        if (z) {
-                            const float zf = cz.get(i), sg = sigmoid_f(zf);
-                            d = of * zf * sg;
-                            odz[i] = of * fmaf(skip[i], uf, r.v[2]) * sg * fmaf(zf, 1.0f - sg, 1.0f);
-                        }
-                        const float dstep = fmaf(r.v[0], URNN_LN2, r.v[1] * uf), dd = dstep * (sp ? sigmoid_f(raw) : 1.0f);
-                        odd[i] = dd;
-                        odu[i] = fmaf(r.v[1], r.v[3], d * skip[i]);
-                        dD[i] = fmaf(d, uf, dD[i]);
-                        dbias[i] += dd;
-                    }
-                    const long at = (t0 + lt) * p.dim;
-                    store_channels<T, V>(ddl + at, evalid, ewide, odd);
-                    store_channels<T, V>(du + at, evalid, ewide, odu);
-                    if (z) store_channels<T, V>(dz + at, evalid, ewide, odz);
-                }
-                for (int k = tid; k < nt * 2 * NP; k += 256) {
-                    const int t = k / (2 * NP), w = k % (2 * NP), n = w % NP;
-                    if (n < p.N) {
-                        float s = 0.0f;
-#pragma unroll
-                        for (int l = 0; l < 4; ++l) s += s_bc[(l * TT + t) * 2 * NP + w];
-                        (w < NP ? dBp : dCp)[(t0 + t) * pt + n] = s;
-                    }
-                }
+                par[128] = dD;
+                par[192] = db;
+                const long at = ((long)b * p.L + t0) * p.dim * TS;
+                store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.ddelta) + at + oy, evalid, odd);
+                store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.du) + at + oy, evalid, odu);
+                if (gated) store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.dz) + at + oy, evalid, odz);
+            }
+            __syncthreads();                                     // the four waves' sums are there; the next segment's go to the other turn
+            for (int k = tid; k < nt * 2 * NP; k += 256) {
+                const int t = k / (2 * NP), w = k % (2 * NP), n = w % NP;
+                if (n < p.N) put_bc(w / NP, t0 + t, n, (s_bc[turn][0][t][w] + s_bc[turn][1][t][w]) + (s_bc[turn][2][t][w] + s_bc[turn][3][t][w]));
             }
         }
-        const long z0 = te > tb ? te : tb;                       // rows behind the sequence are zeros
         const float none[V] = {};
-        for (long t = z0 + lt; eok && t < tfull; t += TT) {
-            store_channels<T, V>(du + t * p.dim, evalid, ewide, none);
-            store_channels<T, V>(ddl + t * p.dim, evalid, ewide, none);
-            if (z) store_channels<T, V>(dz + t * p.dim, evalid, ewide, none);
+        for (long t = te; t < tfull; t += CK) {                  // rows behind the sequence are zeros
+            const long at = ((long)b * p.L + t) * p.dim * TS;
+            if (eok && t + lt < tfull) {
+                store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.ddelta) + at + oy, evalid, none);
+                store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.du) + at + oy, evalid, none);
+                if (gated) store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.dz) + at + oy, evalid, none);
+            }
         }
-        for (long k = z0 * NP + tid; k < tfull * NP; k += 256) {
-            const long t = k / NP;
+        for (long k = te * NP + tid; k < tfull * NP; k += 256) {
             const int n = (int)(k % NP);
-            if (n < p.N) dBp[t * pt + n] = dCp[t * pt + n] = 0.0f;
+            if (n < p.N) {
+                put_bc(0, k / NP, n, 0.0f);
+                put_bc(1, k / NP, n, 0.0f);
+            }
         }
         if (p.dstate && chunk == 0) {
 #pragma unroll
             for (int k = 0; k < ED; ++k)
                 if (sok[k]) store_states<E>(p.dstate + ((long)b * p.dim + sch[k]) * p.N, q, p.N, states_vec(p.dstate, p.N, W), carry[k]);
         }
-        __syncthreads();                                         // the next sequence's tile overwrites s_io, s_B, s_C and s_bc
     }
     float *sums = p.dAp + ((long)slot * p.chunks + chunk) * p.dim * (p.N + 2);      // this part's dA, dD, ddelta_bias
 #pragma unroll
     for (int k = 0; k < ED; ++k)
         if (sok[k]) store_states<E>(sums + (long)sch[k] * p.N, q, p.N, states_vec(sums, p.N, W), dA[k]);
+    wave_fence();
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_io[lt * CB + i * CG + lg] = {{dD[i], dbias[i], 0.0f, 0.0f}};
-    __syncthreads();
-    if (tid < CB) {
+    for (int i = 0; i < V; ++i) io[lt * CW + i * CG + lg] = {{par[128].v[i], par[192].v[i], 0.0f, 0.0f}};
+    wave_fence();
+    if (lane < CW) {
         float x = 0.0f, y = 0.0f;
-        for (int t = 0; t < TT; ++t) { x += s_io[t * CB + tid].v[0]; y += s_io[t * CB + tid].v[1]; }
-        const int c = tid % CG * V + tid / CG;
+        for (int t = 0; t < CK; ++t) { x += io[t * CW + lane].v[0]; y += io[t * CW + lane].v[1]; }
+        const int c = lane % CG * V + lane / CG;
         if (c < width) {
-            sums[(long)p.dim * p.N + c0 + c] = x;
-            sums[(long)p.dim * (p.N + 1) + c0 + c] = y;
+            sums[(long)p.dim * p.N + w0 + c] = x;
+            sums[(long)p.dim * (p.N + 1) + w0 + c] = y;
         }
     }
 }
@@ -425,7 +497,7 @@ __global__ __launch_bounds__(256) void scan_fold_rows_kernel(const float *__rest
 // channels, which a block of the main pass has four of: they need more chunks to fill the chip).
 int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, int *pieces)
 {
-    const int CB = 64 * urnn_scan_ed(urnn_scan_np(N));
+    const int CB = 64 * urnn_scan_ed(urnn_scan_np(N));      // channels of a block
     const long cbs = (D + CB - 1) / CB, blocks = (long)B * cbs;
     long want = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
     const long most = (L + 63) / 64;
@@ -445,7 +517,7 @@ int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, i
 }
 
 template <typename T, int NP>
-static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, float *dbias, void *dB, void *dC, int accumulate, hipStream_t st)
+static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, float *dbias, int accumulate, hipStream_t st)
 {
     const int Dg = p.dim / p.G, CB = 64 * urnn_scan_ed(NP), gcbs = (Dg + CB - 1) / CB;
     if (p.chunks > 1) {
@@ -457,9 +529,11 @@ static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, flo
         const long count = (long)p.batch * p.dim * NP;
         scan_back_carry_kernel<NP><<<dim3((unsigned)((count + 255) / 256)), 256, 0, st>>>(p.A, p.sum, p.S, p.dstate_out, p.dim, p.N, ps.chunks, count);
     }
-    scan_backward_kernel<T, NP><<<dim3((unsigned)(gcbs * p.G * p.chunks * p.slots)), 256, 0, st>>>(p);
+    const dim3 grid((unsigned)(gcbs * p.G * p.chunks * p.slots));
+    if (p.wide) scan_backward_kernel<T, NP, true><<<grid, 256, 0, st>>>(p);
+    else scan_backward_kernel<T, NP, false><<<grid, 256, 0, st>>>(p);
     const long n = (long)p.batch * p.L * p.G * p.N;
-    scan_fold_rows_kernel<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(p.dBp, p.dCp, gcbs, n, reinterpret_cast<T *>(dB), reinterpret_cast<T *>(dC));
+    if (!p.direct) scan_fold_rows_kernel<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(p.dBp, p.dCp, gcbs, n, reinterpret_cast<T *>(p.dB), reinterpret_cast<T *>(p.dC));
     hipError_t e = hipGetLastError();
     float *const outs[3] = {dA, dD, dbias};
     const long sizes[3] = {(long)p.dim * p.N, p.dim, p.dim};
@@ -468,19 +542,19 @@ static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, flo
 }
 
 template <typename T>
-static hipError_t by_states(const ScanParams &p, float *dA, float *dD, float *dbias, void *dB, void *dC, int accumulate, hipStream_t st)
+static hipError_t by_states(const ScanParams &p, float *dA, float *dD, float *dbias, int accumulate, hipStream_t st)
 {
     switch (urnn_scan_np(p.N)) {
-    case 4: return launch_backward<T, 4>(p, dA, dD, dbias, dB, dC, accumulate, st);
-    case 8: return launch_backward<T, 8>(p, dA, dD, dbias, dB, dC, accumulate, st);
-    case 16: return launch_backward<T, 16>(p, dA, dD, dbias, dB, dC, accumulate, st);
-    case 32: return launch_backward<T, 32>(p, dA, dD, dbias, dB, dC, accumulate, st);
-    default: return launch_backward<T, 64>(p, dA, dD, dbias, dB, dC, accumulate, st);
+    case 4: return launch_backward<T, 4>(p, dA, dD, dbias, accumulate, st);
+    case 8: return launch_backward<T, 8>(p, dA, dD, dbias, accumulate, st);
+    case 16: return launch_backward<T, 16>(p, dA, dD, dbias, accumulate, st);
+    case 32: return launch_backward<T, 32>(p, dA, dD, dbias, accumulate, st);
+    default: return launch_backward<T, 64>(p, dA, dD, dbias, accumulate, st);
     }
 }
 
-hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, void *dB, void *dC, int accumulate, hipStream_t st)
+hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, int accumulate, hipStream_t st)
 {
-    return dtype == URNN_F32 ? by_states<float>(p, dA, dD, dbias, dB, dC, accumulate, st)
-         : dtype == URNN_BF16 ? by_states<bf16_t>(p, dA, dD, dbias, dB, dC, accumulate, st) : by_states<f16_t>(p, dA, dD, dbias, dB, dC, accumulate, st);
+    return dtype == URNN_F32 ? by_states<float>(p, dA, dD, dbias, accumulate, st)
+         : dtype == URNN_BF16 ? by_states<bf16_t>(p, dA, dD, dbias, accumulate, st) : by_states<f16_t>(p, dA, dD, dbias, accumulate, st);
 }

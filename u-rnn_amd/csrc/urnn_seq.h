@@ -39,12 +39,27 @@ __device__ __forceinline__ float softplus_f(float x)
     return fmaxf(x, 0.0f) + 2.0f * s * p;
 }
 
+// A lane's value through a DPP pattern that has a source for every lane (no value for others to keep: it folds into the addition).
+template <int CTRL>
+__device__ __forceinline__ float dpp_all(float v)
+{
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 // Sum over the four lanes of a quad, returned to all of them.
 __device__ __forceinline__ float quad_sum(float v)
 {
-    v += dpp_move<0xB1>(v);
-    v += dpp_move<0x4E>(v);
+    v += dpp_all<0xB1>(v);
+    v += dpp_all<0x4E>(v);
     return v;
+}
+
+// The kernel's parameters, read again from here on: a loop that needs a few of many then loads those it needs where it needs them,
+// instead of holding all of them in scalar registers (and spilling those to vector registers' lanes).
+template <typename P>
+__device__ __forceinline__ const P *reread(const P *p)
+{
+    asm volatile("" : "+s"(p));
+    return p;
 }
 
 // Tokens of sequence b that count: lengths clamped to [0, L], so that no length can reach outside the tensors.
@@ -125,6 +140,8 @@ struct ScanParams {
     const float *dstate_out;                         // (B,D,N) or NULL
     void *du, *ddelta, *dz;                          // (B,L,D) contiguous
     float *dstate;                                   // (B,D,N) or NULL
+    void *dB, *dC;                                   // (B,L,G,N) contiguous
+    int direct;                                      // a group is one block: dB and dC leave the main pass as they are
     float *dBp, *dCp;                                // per channel block: [blocks of a group][B][L][G][N]
     float *dAp;                                      // per (batch slot, chunk): [parts][D N | D | D], sums for dA, dD, ddelta_bias
 };
@@ -135,22 +152,21 @@ enum { SCAN_STATES = 0, SCAN_FULL = 1, SCAN_BACK = 2, SCAN_STEP = 3 };
 // Tokens between two checkpoints of the state: what the backward holds in registers of decays and states at a time, 2 CK NP / 4 (x 2
 // channels up to 16 states).
 __host__ __device__ static constexpr int urnn_scan_ck(int np) { return np == 64 ? 4 : 8; }
-__host__ __device__ static constexpr int urnn_scan_ed(int) { return 1; }    // channels of a backward lane
+__host__ __device__ static constexpr int urnn_scan_ed(int np) { return np <= 16 ? 2 : 1; }    // channels of a backward lane
 
 static inline int urnn_scan_np(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
-// Place of channel c among the w channels of a backward block, in the record of checkpoints: the block's thread for channels V i ..
-// V i + V - 1 spreads them over its LDS rows so that neighbours of a row are V channels apart, and reads a row's states side by side.
+// Channels of a thread in the backward's elementwise work: a segment's tokens by a wave's channels over 64 lanes.
+__host__ __device__ static constexpr int urnn_scan_v(int np) { return urnn_scan_ck(np) * 16 * urnn_scan_ed(np) / 64; }
+// Place of channel c among the w channels of a backward wave, in the record of checkpoints: the wave's lane for channels V i .. V i + V - 1
+// spreads them over its LDS rows so that neighbours of a row are V channels apart, and reads a row's states side by side.
 __host__ __device__ static inline int keep_rank(int c, int w, int V) { return w % V == 0 ? c % V * (w / V) + c / V : c; }
-// Tokens of a backward tile, and so the channels of a thread of 256
-__host__ __device__ static constexpr int urnn_scan_tt(int) { return 16; }
-__host__ __device__ static constexpr int urnn_scan_v(int np) { return urnn_scan_tt(np) * 64 * urnn_scan_ed(np) / 256; }
 
 hipError_t urnn_launch_scan(const ScanParams &p, int dtype, hipStream_t st);
 hipError_t urnn_launch_scan_back_summaries(const ScanParams &p, int dtype, hipStream_t st);
 hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st);
 int urnn_scan_chunks(int B, int L, int D, int *CL);
-hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, void *dB, void *dC, int accumulate, hipStream_t st);
+hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, int accumulate, hipStream_t st);
 int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, int *pieces);
 
 // ---- short causal convolution ----------------------------------------------------------------------------------------
