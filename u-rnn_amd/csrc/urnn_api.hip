@@ -1675,8 +1675,8 @@ struct ScanBackWork { size_t sum, S, dB, dC, sums, total; int chunks, CL, slots,
 static ScanBackWork scan_back_work(int B, int L, int D, int G, int N)
 {
     ScanBackWork w;
-    w.chunks = urnn_scan_backward_chunks(B, L, D, N, &w.CL, &w.slots, &w.pieces);
-    const size_t np = urnn_scan_np(N), cb = 64 * urnn_scan_ed((int)np), gcbs = (D / G + cb - 1) / cb, parts = (size_t)w.slots * w.chunks;
+    w.chunks = urnn_scan_backward_chunks(B, L, D, G, N, &w.CL, &w.slots, &w.pieces);
+    const size_t np = urnn_scan_np(N), cb = 16 * urnn_scan_ed((int)np) * urnn_scan_waves(D / G, (int)np), gcbs = (D / G + cb - 1) / cb, parts = (size_t)w.slots * w.chunks;
     const size_t rows = gcbs > 1 ? align_up(gcbs * B * L * G * N * sizeof(float), 256) : 0, cross = w.chunks > 1 ? (size_t)w.chunks * w.pieces : 0;
     w.sum = 0;
     w.S = align_up((size_t)B * cross * D * sizeof(float), 256);
@@ -1724,7 +1724,7 @@ extern "C" int urnn_selective_scan_backward(const void *u, const void *delta, co
     p.dAp = reinterpret_cast<float *>(base + w.sums);
     p.du = du; p.ddelta = ddelta; p.dz = dz; p.dstate = dstate; p.dB = dB; p.dC = dC; p.direct = w.dB == w.dC;
     p.batch = B; p.L = L; p.dim = D; p.N = N; p.G = G; p.softplus = softplus;
-    p.chunks = w.chunks; p.CL = w.CL; p.slots = w.slots; p.pieces = w.pieces;
+    p.chunks = w.chunks; p.CL = w.CL; p.slots = w.slots; p.pieces = w.pieces; p.waves = urnn_scan_waves(D / G, urnn_scan_np(N));
     const int e = seq_elem(dtype);
     p.wide = wide_rows(u, strides[0], strides[1], e) && wide_rows(delta, strides[2], strides[3], e) && wide_rows(z, strides[8], strides[9], e) &&
              wide_rows(dout, strides[10], strides[11], e) && (long)D / G * e % 16 == 0 && aligned16(du) && aligned16(ddelta) && (!z || aligned16(dz));

@@ -3,6 +3,7 @@
 //   k_t[n] = C_t[n] d_t + a_(t+1)[n] k_(t+1)[n]        (behind the last token: dstate_out)
 // per channel and state
 //   dC_t[n] = sum_channels d_t h_t[n]                  dB_t[n] = sum_channels k_t[n] step_t u_t
+//           = sum_channels d_t a_t h_(t-1)[n] + B_t[n] sum_channels d_t step_t u_t       (C . h likewise: h_t itself is not formed again)
 //   w = k_t[n] a_t[n] h_(t-1)[n]                       dA[n] = sum_tokens w step_t
 //   du_t = step_t sum_n k_t B_t + D d_t                dstep_t = sum_n w A + u_t sum_n k_t B_t,   ddelta_t = dstep_t softplus'(raw_t)
 //   dz_t = dout_t (sum_n C_t h_t + D u_t) silu'(z_t)   dD = sum d_t u_t
@@ -32,6 +33,15 @@ __device__ __forceinline__ float add_swapped16(float a, float b)
 {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Sum over G adjacent lanes (G = 8 or 16, aligned), returned to all of them.
+template <int G>
+__device__ __forceinline__ float group_sum(float v)
+{
+    v = quad_sum(v);
+    v += dpp_all<0x141>(v);                          // row_half_mirror
+    if (G == 16) v += dpp_all<0x140>(v);             // row_mirror
+    return v;
 }
 template <int E>
 __device__ __forceinline__ void channel_sums(const float (&v)[2 * E], float (&r)[E < 2 ? 1 : E / 2])
@@ -141,17 +151,19 @@ __device__ __forceinline__ void wave_fence()
 }
 
 template <typename T, int NP, bool WIDE>
-__global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams p)
+__global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(const ScanParams p)
 {
-    constexpr int E = NP / 4, W = E < 4 ? E : 4, ED = urnn_scan_ed(NP), CK = urnn_scan_ck(NP), CW = 16 * ED, CB = 4 * CW;
+    constexpr int E = NP / 4, W = E < 4 ? E : 4, ED = urnn_scan_ed(NP), CK = urnn_scan_ck(NP), CW = 16 * ED;
     constexpr int HT = CK / 2;                                   // tokens whose decays and states are in registers at a time
     constexpr int V = urnn_scan_v(NP), CG = CW / V, RB = CK * NP < 64 ? 1 : CK * NP / 64;
     static_assert(CG * CK == 64, "a wave's lanes are the tokens of a segment by groups of V channels");
     __shared__ alignas(16) Pack<float, 4> s_io[4][CK * CW];      // in: (step, step u, d, -); out: (sum w A log2 e, sum k B, sum C h, step)
     __shared__ alignas(16) float s_row[4][2][CK * NP];           // B, C
-    __shared__ float s_bc[2][4][CK][2 * NP];                     // [turn][wave][token][dB | dC]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane & 3;
-    const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
+    __shared__ float s_bc[2][4][CK][2 * NP];                     // [turn][wave][token][sum k step u | sum d a h]
+    __shared__ float s_ds[2][4][CK];                             // [turn][wave][token] sum over channels d step u
+    __shared__ float s_cb[4][CK];                                // C . B of a token
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane & 3;
+    const int CB = p.waves * CW, Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
     const int chunk = blockIdx.x / (cbs * p.G) % p.chunks, slot = blockIdx.x / (cbs * p.G) / p.chunks;
     const int segs = (p.L + CK - 1) / CK;
@@ -299,11 +311,13 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
             const Raw<T, V> cu = ru, cd = rd, cz = rz, co = ro;
             const bool here = eok && lt < nt;                    // tokens behind the sequence: steps of zero, which change nothing
             const Chan bias = par[0];
+            float ds = 0.0f, dot = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float raw = cd.get(i) + bias.v[i], s = softplus_f(raw), step = here ? (sp ? s : raw) : 0.0f;
-                const float d = co.get(i) * (gated ? silu_f(cz.get(i)) : 1.0f);
-                io[lt * CW + i * CG + lg] = {{step, here ? step * cu.get(i) : 0.0f, here ? d : 0.0f, 0.0f}};
+                const float d = here ? co.get(i) * (gated ? silu_f(cz.get(i)) : 1.0f) : 0.0f, su = here ? step * cu.get(i) : 0.0f;
+                io[lt * CW + i * CG + lg] = {{step, su, d, 0.0f}};
+                ds = fmaf(d, su, ds);
             }
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
@@ -313,6 +327,13 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                 }
             }
             wave_fence();
+#pragma unroll
+            for (int n = 0; n < NP / CG; ++n) dot = fmaf(rowB[lt * NP + n * CG + lg], rowC[lt * NP + n * CG + lg], dot);
+            if (NP < CG) dot = lg < NP ? rowB[lt * NP + lg] * rowC[lt * NP + lg] : 0.0f;
+            ds = group_sum<CG>(ds);
+            dot = group_sum<CG>(dot);
+            s_ds[turn][wave][lt] = ds;                           // the same from all lanes of a token
+            s_cb[wave][lt] = dot;
             if (t0 - CK >= tb) fetch();
             else fetch_sequence(b + p.slots);
 
@@ -362,13 +383,13 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                         float SW = 0.0f, SG = 0.0f, SY = 0.0f;
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
-                            const float kk = fmaf(Cv[e], in.v[2], carry[k][e]), hj = fmaf(in.v[1], Bv[e], ah[j][k][e]), w = kk * ah[j][k][e];
+                            const float kk = fmaf(Cv[e], in.v[2], carry[k][e]), w = kk * ah[j][k][e];
                             SW = fmaf(w, A2[k][e], SW);
                             SG = fmaf(kk, Bv[e], SG);
-                            SY = fmaf(Cv[e], hj, SY);
-                            dA[k][e] = fmaf(w, in.v[0], dA[k][e]);
+                            SY = fmaf(Cv[e], ah[j][k][e], SY);   // h = a h + step u B: the second term's sums are common to
+                            dA[k][e] = fmaf(w, in.v[0], dA[k][e]);       // all states (C . B) and to all channels (d step u)
                             v[e] = fmaf(kk, in.v[1], v[e]);
-                            v[E + e] = fmaf(hj, in.v[2], v[E + e]);
+                            v[E + e] = fmaf(ah[j][k][e], in.v[2], v[E + e]);
                             carry[k][e] = a[j][k][e] * kk;
                         }
                         SW = quad_sum(SW);
@@ -410,6 +431,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
             if (here) {
                 float odz[V], odd[V], odu[V];
                 const Chan bias = par[0], skip = par[64];
+                const float cb_t = s_cb[wave][lt];
                 Chan dD = par[128], db = par[192];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -419,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                     if (gated) {
                         const float zf = cz.get(i), sg = sigmoid_f(zf);
                         d = of * zf * sg;
-                        odz[i] = of * fmaf(skip.v[i], uf, r.v[2]) * sg * fmaf(zf, 1.0f - sg, 1.0f);
+                        odz[i] = of * fmaf(fmaf(r.v[3], cb_t, skip.v[i]), uf, r.v[2]) * sg * fmaf(zf, 1.0f - sg, 1.0f);
                     }
                     const float dstep = fmaf(r.v[0], URNN_LN2, r.v[1] * uf), dd = dstep * (sp ? sigmoid_f(raw) : 1.0f);
                     odd[i] = dd;
@@ -435,9 +457,12 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                 if (gated) store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.dz) + at + oy, evalid, odz);
             }
             __syncthreads();                                     // the four waves' sums are there; the next segment's go to the other turn
-            for (int k = tid; k < nt * 2 * NP; k += 256) {
+            for (int k = tid; k < nt * 2 * NP; k += 64 * p.waves) {
                 const int t = k / (2 * NP), w = k % (2 * NP), n = w % NP;
-                if (n < p.N) put_bc(w / NP, t0 + t, n, (s_bc[turn][0][t][w] + s_bc[turn][1][t][w]) + (s_bc[turn][2][t][w] + s_bc[turn][3][t][w]));
+                float sum = s_bc[turn][0][t][w], ds = s_ds[turn][0][t];
+                for (int l = 1; l < p.waves; ++l) { sum += s_bc[turn][l][t][w]; ds += s_ds[turn][l][t]; }
+                if (w >= NP) sum = fmaf(rowB[t * NP + n], ds, sum);
+                if (n < p.N) put_bc(w / NP, t0 + t, n, sum);
             }
         }
         const float none[V] = {};
@@ -449,7 +474,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(const ScanParams 
                 if (gated) store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.dz) + at + oy, evalid, none);
             }
         }
-        for (long k = te * NP + tid; k < tfull * NP; k += 256) {
+        for (long k = te * NP + tid; k < tfull * NP; k += 64 * p.waves) {
             const int n = (int)(k % NP);
             if (n < p.N) {
                 put_bc(0, k / NP, n, 0.0f);
@@ -495,10 +520,10 @@ __global__ __launch_bounds__(256) void scan_fold_rows_kernel(const float *__rest
 
 // Chunks of the time axis, blocks along the batch, and the pieces that a chunk's summary is made of (the summaries are waves of 64
 // channels, which a block of the main pass has four of: they need more chunks to fill the chip).
-int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, int *pieces)
+int urnn_scan_backward_chunks(int B, int L, int D, int G, int N, int *CL, int *slots, int *pieces)
 {
-    const int CB = 64 * urnn_scan_ed(urnn_scan_np(N));      // channels of a block
-    const long cbs = (D + CB - 1) / CB, blocks = (long)B * cbs;
+    const int np = urnn_scan_np(N), CB = urnn_scan_waves(D / G, np) * 16 * urnn_scan_ed(np);      // channels of a block
+    const long cbs = (long)G * ((D / G + CB - 1) / CB), blocks = (long)B * cbs;
     long want = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
     const long most = (L + 63) / 64;
     if (want > most) want = most;
@@ -519,7 +544,7 @@ int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, i
 template <typename T, int NP>
 static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, float *dbias, int accumulate, hipStream_t st)
 {
-    const int Dg = p.dim / p.G, CB = 64 * urnn_scan_ed(NP), gcbs = (Dg + CB - 1) / CB;
+    const int Dg = p.dim / p.G, CB = urnn_scan_waves(Dg, NP) * 16 * urnn_scan_ed(NP), gcbs = (Dg + CB - 1) / CB;
     if (p.chunks > 1) {
         ScanParams ps = p;
         ps.chunks = p.chunks * p.pieces;
@@ -530,8 +555,8 @@ static hipError_t launch_backward(const ScanParams &p, float *dA, float *dD, flo
         scan_back_carry_kernel<NP><<<dim3((unsigned)((count + 255) / 256)), 256, 0, st>>>(p.A, p.sum, p.S, p.dstate_out, p.dim, p.N, ps.chunks, count);
     }
     const dim3 grid((unsigned)(gcbs * p.G * p.chunks * p.slots));
-    if (p.wide) scan_backward_kernel<T, NP, true><<<grid, 256, 0, st>>>(p);
-    else scan_backward_kernel<T, NP, false><<<grid, 256, 0, st>>>(p);
+    if (p.wide) scan_backward_kernel<T, NP, true><<<grid, 64 * p.waves, 0, st>>>(p);
+    else scan_backward_kernel<T, NP, false><<<grid, 64 * p.waves, 0, st>>>(p);
     const long n = (long)p.batch * p.L * p.G * p.N;
     if (!p.direct) scan_fold_rows_kernel<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(p.dBp, p.dCp, gcbs, n, reinterpret_cast<T *>(p.dB), reinterpret_cast<T *>(p.dC));
     hipError_t e = hipGetLastError();

@@ -135,7 +135,7 @@ struct ScanParams {
     float *S;                                        // ... and the state of a chunk that starts from zero [B][chunks][D][NP]
     int batch, L, dim, N, G, chunks, CL, softplus;
     // backward
-    int slots, pieces;                               // blocks along the batch; summaries of a chunk
+    int slots, pieces, waves;                        // blocks along the batch; summaries of a chunk; waves of a block
     int wide;                                        // all (B,L,D) rows start on 16 bytes
     const float *dstate_out;                         // (B,D,N) or NULL
     void *du, *ddelta, *dz;                          // (B,L,D) contiguous
@@ -158,6 +158,12 @@ static inline int urnn_scan_np(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16
 
 // Channels of a thread in the backward's elementwise work: a segment's tokens by a wave's channels over 64 lanes.
 __host__ __device__ static constexpr int urnn_scan_v(int np) { return urnn_scan_ck(np) * 16 * urnn_scan_ed(np) / 64; }
+// Waves of a backward block: at most four, as many as the channels of a group divide into evenly (96 channels are three, not four).
+__host__ __device__ static inline int urnn_scan_waves(int Dg, int np)
+{
+    const int cw = 16 * urnn_scan_ed(np), w = (Dg + cw - 1) / cw, blocks = (w + 3) / 4;
+    return (w + blocks - 1) / blocks;
+}
 // Place of channel c among the w channels of a backward wave, in the record of checkpoints: the wave's lane for channels V i .. V i + V - 1
 // spreads them over its LDS rows so that neighbours of a row are V channels apart, and reads a row's states side by side.
 __host__ __device__ static inline int keep_rank(int c, int w, int V) { return w % V == 0 ? c % V * (w / V) + c / V : c; }
@@ -167,7 +173,7 @@ hipError_t urnn_launch_scan_back_summaries(const ScanParams &p, int dtype, hipSt
 hipError_t urnn_launch_scan_step(const ScanParams &p, int dtype, hipStream_t st);
 int urnn_scan_chunks(int B, int L, int D, int *CL);
 hipError_t urnn_launch_scan_backward(const ScanParams &p, int dtype, float *dA, float *dD, float *dbias, int accumulate, hipStream_t st);
-int urnn_scan_backward_chunks(int B, int L, int D, int N, int *CL, int *slots, int *pieces);
+int urnn_scan_backward_chunks(int B, int L, int D, int G, int N, int *CL, int *slots, int *pieces);
 
 // ---- short causal convolution ----------------------------------------------------------------------------------------
 struct ConvSeqParams {
