@@ -181,14 +181,15 @@ __global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(con
     const int ech = eok ? w0 + V * lg : c0;
     // the lane's bias and skip, and its sums for their gradients: in LDS, where they cost no registers in between
     typedef Pack<float, V> Chan;
-    __shared__ alignas(16) Chan s_par[4][4][64];
-    Chan *const par = &s_par[wave][0][lane];
+    __shared__ alignas(16) Chan s_par[4][2][CG], s_sum[4][2][64];
+    Chan *const par = &s_par[wave][0][lg], *const acc = &s_sum[wave][0][lane];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        par[0].v[i] = p.bias && i < evalid ? p.bias[ech + i] : 0.0f;
-        par[64].v[i] = p.D && i < evalid ? p.D[ech + i] : 0.0f;
-        par[128].v[i] = par[192].v[i] = 0.0f;
+        par[0].v[i] = p.bias && i < evalid ? p.bias[ech + i] : 0.0f;         // the same from all tokens' lanes
+        par[CG].v[i] = p.D && i < evalid ? p.D[ech + i] : 0.0f;
+        acc[0].v[i] = acc[64].v[i] = 0.0f;
     }
+    wave_fence();
     const bool gated = p.z != nullptr;
     // Addresses: a uniform pointer to a segment's first token, and the lane's byte offset from there in 32 bits (the host checks that
     // CK tokens are within 4 GB).
@@ -430,9 +431,9 @@ __global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(con
             wave_fence();
             if (here) {
                 float odz[V], odd[V], odu[V];
-                const Chan bias = par[0], skip = par[64];
+                const Chan bias = par[0], skip = par[CG];
                 const float cb_t = s_cb[wave][lt];
-                Chan dD = par[128], db = par[192];
+                Chan dD = acc[0], db = acc[64];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const Pack<float, 4> r = io[lt * CW + i * CG + lg];
@@ -449,8 +450,8 @@ __global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(con
                     dD.v[i] = fmaf(d, uf, dD.v[i]);
                     db.v[i] += dd;
                 }
-                par[128] = dD;
-                par[192] = db;
+                acc[0] = dD;
+                acc[64] = db;
                 const long at = ((long)b * p.L + t0) * p.dim * TS;
                 store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.ddelta) + at + oy, evalid, odd);
                 store_channels<T, V, WIDE>(reinterpret_cast<char *>(p.du) + at + oy, evalid, odu);
@@ -459,8 +460,15 @@ __global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(con
             __syncthreads();                                     // the four waves' sums are there; the next segment's go to the other turn
             for (int k = tid; k < nt * 2 * NP; k += 64 * p.waves) {
                 const int t = k / (2 * NP), w = k % (2 * NP), n = w % NP;
-                float sum = s_bc[turn][0][t][w], ds = s_ds[turn][0][t];
-                for (int l = 1; l < p.waves; ++l) { sum += s_bc[turn][l][t][w]; ds += s_ds[turn][l][t]; }
+                float sum, ds;
+                if (p.waves == 4) {
+                    sum = (s_bc[turn][0][t][w] + s_bc[turn][1][t][w]) + (s_bc[turn][2][t][w] + s_bc[turn][3][t][w]);
+                    ds = (s_ds[turn][0][t] + s_ds[turn][1][t]) + (s_ds[turn][2][t] + s_ds[turn][3][t]);
+                } else {
+                    sum = s_bc[turn][0][t][w];
+                    ds = s_ds[turn][0][t];
+                    for (int l = 1; l < p.waves; ++l) { sum += s_bc[turn][l][t][w]; ds += s_ds[turn][l][t]; }
+                }
                 if (w >= NP) sum = fmaf(rowB[t * NP + n], ds, sum);
                 if (n < p.N) put_bc(w / NP, t0 + t, n, sum);
             }
@@ -493,7 +501,7 @@ __global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(con
         if (sok[k]) store_states<E>(sums + (long)sch[k] * p.N, q, p.N, states_vec(sums, p.N, W), dA[k]);
     wave_fence();
 #pragma unroll
-    for (int i = 0; i < V; ++i) io[lt * CW + i * CG + lg] = {{par[128].v[i], par[192].v[i], 0.0f, 0.0f}};
+    for (int i = 0; i < V; ++i) io[lt * CW + i * CG + lg] = {{acc[0].v[i], acc[64].v[i], 0.0f, 0.0f}};
     wave_fence();
     if (lane < CW) {
         float x = 0.0f, y = 0.0f;
@@ -535,8 +543,11 @@ int urnn_scan_backward_chunks(int B, int L, int D, int G, int N, int *CL, int *s
     int m = 1;
     while (m < 8 && cl % (32 * m) == 0 && cl / (2 * m) >= 64 && blocks * chunks * m < 2048) m *= 2;
     *pieces = m;
-    long s = B;                                                  // several sequences to a block once there are enough blocks
-    while (s > 1 && s * cbs * chunks > 1024) s = (s + 1) / 2;
+    // several sequences to a block once there are as many blocks as fit the chip at a time
+    const long fit = np <= 8 ? 768 : 512;
+    long s = fit / (cbs * chunks);
+    if (s < 1) s = 1;
+    if (s > B) s = B;
     *slots = (int)s;
     return chunks;
 }
