@@ -466,6 +466,8 @@ def _seq_dtype(what, t):
 
 def _seq_check(what, name, t, shape, dtype, contiguous=False):
     """Shape, type and layout of an argument (no device is needed to refuse a wrong one)."""
+    if t.shape == shape and t.dtype is dtype and (t.is_contiguous() if contiguous else t.stride(-1) == 1):
+        return
     if tuple(t.shape) != shape:
         raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
     if t.dtype != dtype:
@@ -477,8 +479,19 @@ def _seq_check(what, name, t, shape, dtype, contiguous=False):
         raise RuntimeError(f"{what}: the channels of {name} must be adjacent (stride {t.stride(-1)})")
 
 
+# The current stream as the C ABI takes it, without the stream object that torch.cuda.current_stream() builds (2.7 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _seq_device(what, *tensors):
-    """All on the current device: kernels are enqueued on its current stream."""
+    """All on the current device: kernels are enqueued on its current stream.  Returns that stream."""
+    cur = tensors[0].get_device()                        # -1: a CPU tensor
+    if cur >= 0 and cur == torch.cuda.current_device():
+        for t in tensors:
+            if t is not None and t.get_device() != cur:
+                break
+        else:
+            return _raw_stream(cur)
     dev = None
     for t in tensors:
         if t is None:
@@ -552,14 +565,14 @@ def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, out=N
         _seq_out(what, "out", out, (B, L, D), x.dtype, (x, weight, bias, state, state_out))
     if state_out is not None:
         _seq_out(what, "state_out", state_out, (B, K - 1, D), x.dtype, (x, weight, bias, state))
-    _seq_device(what, x, weight, bias, state, lengths, out, state_out)
+    stream = _seq_device(what, x, weight, bias, state, lengths, out, state_out)
     if out is None:
         out = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
     if want_state and state_out is None:
         state_out = torch.empty((B, K - 1, D), dtype=x.dtype, device=x.device)
     sb, st, _ = x.stride()
     check(lib().urnn_causal_conv(_ptr(x), sb, st, _ptr(weight), _ptr(bias), _ptr(state), _ptr(lengths), _ptr(out), _ptr(state_out), dt, B, L,
-                                 D, K, 1 if silu else 0, _stream()), "urnn_causal_conv")
+                                 D, K, 1 if silu else 0, stream), "urnn_causal_conv")
     return (out, state_out) if want_state else out
 
 
@@ -577,13 +590,13 @@ def causal_conv_step(x, state, weight, bias=None, silu=True, out=None, state_out
         _seq_out(what, "out", out, (B, D), x.dtype, (x, weight, bias, state, state_out))
     if state_out is not None:
         _seq_out(what, "state_out", state_out, (B, K - 1, D), x.dtype, (x, weight, bias, state), same=(state,))
-    _seq_device(what, x, weight, bias, state, out, state_out)
+    stream = _seq_device(what, x, weight, bias, state, out, state_out)
     if out is None:
         out = torch.empty((B, D), dtype=x.dtype, device=x.device)
     if state_out is None:
         state_out = torch.empty_like(state)
     check(lib().urnn_causal_conv_step(_ptr(x), x.stride(0), _ptr(weight), _ptr(bias), _ptr(state), _ptr(out), _ptr(state_out), dt, B, D, K,
-                                      1 if silu else 0, _stream()), "urnn_causal_conv_step")
+                                      1 if silu else 0, stream), "urnn_causal_conv_step")
     return out, state_out
 
 
@@ -647,7 +660,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
         _seq_out(what, "out", out, (nb, L, dim), u.dtype, inputs + (state_out,))
     if state_out is not None:
         _seq_out(what, "state_out", state_out, (nb, dim, N), torch.float32, inputs)
-    _seq_device(what, *inputs, lengths, out, state_out)
+    stream = _seq_device(what, *inputs, lengths, out, state_out)
     Lb = lib()
     keep = ws is not None
     nbytes = Lb.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1 if keep else 0)
@@ -663,7 +676,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     strides = (ctypes.c_long * 10)(*u.stride()[:2], *delta.stride()[:2], *B.stride()[:2], *C.stride()[:2], *(z.stride()[:2] if z is not None else (0, 0)))
     check(Lb.urnn_selective_scan(_ptr(u), _ptr(delta), _ptr(B), _ptr(C), _ptr(z), strides, _ptr(A), _ptr(D), _ptr(delta_bias), _ptr(state),
                                  _ptr(lengths), _ptr(out), _ptr(state_out), _ptr(ws), nbytes if not keep else ws.numel(), 1 if keep else 0, dt, nb, L,
-                                 dim, G, N, 1 if softplus else 0, _stream()), "urnn_selective_scan")
+                                 dim, G, N, 1 if softplus else 0, stream), "urnn_selective_scan")
     return (out, state_out) if want_state else out
 
 
@@ -684,14 +697,14 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
         _seq_out(what, "out", out, (nb, dim), u.dtype, inputs + (state_out,))
     if state_out is not None:
         _seq_out(what, "state_out", state_out, (nb, dim, N), torch.float32, inputs, same=(state,))
-    _seq_device(what, *inputs, out, state_out)
+    stream = _seq_device(what, *inputs, out, state_out)
     if out is None:
         out = torch.empty((nb, dim), dtype=u.dtype, device=u.device)
     if state_out is None:
         state_out = torch.empty_like(state)
     strides = (ctypes.c_long * 5)(u.stride(0), delta.stride(0), B.stride(0), C.stride(0), z.stride(0) if z is not None else 0)
     check(lib().urnn_selective_scan_step(_ptr(u), _ptr(delta), _ptr(B), _ptr(C), _ptr(z), strides, _ptr(A), _ptr(D), _ptr(delta_bias), _ptr(state),
-                                         _ptr(out), _ptr(state_out), dt, nb, dim, G, N, 1 if softplus else 0, _stream()),
+                                         _ptr(out), _ptr(state_out), dt, nb, dim, G, N, 1 if softplus else 0, stream),
           "urnn_selective_scan_step")
     return out, state_out
 
@@ -741,12 +754,12 @@ def norm_residual(y, pre_w, residual=None, post_w=None, gate=None, scale=None, g
         _seq_out(what, "out", out, shape, y.dtype, inputs + (residual_out,), same=inputs)
     if residual_out is not None:
         _seq_out(what, "residual_out", residual_out, shape, y.dtype, inputs, same=inputs)
-    _seq_device(what, y, pre_w, residual, post_w, gate, scale, out, residual_out)
+    stream = _seq_device(what, y, pre_w, residual, post_w, gate, scale, out, residual_out)
     if out is None:
         out = torch.empty(shape, dtype=y.dtype, device=y.device)
     if residual_out is None:
         residual_out = torch.empty(shape, dtype=y.dtype, device=y.device)
     D = shape[-1]
     check(lib().urnn_norm_residual(_ptr(y), _ptr(gate), _ptr(residual), (ctypes.c_long * 3)(sy, sg, sr), _ptr(pre_w), _ptr(post_w), _ptr(scale),
-                                   _ptr(out), _ptr(residual_out), dt, y.numel() // D, D, GATE_ACTS[gate_act], float(eps), _stream()), "urnn_norm_residual")
+                                   _ptr(out), _ptr(residual_out), dt, y.numel() // D, D, GATE_ACTS[gate_act], float(eps), stream), "urnn_norm_residual")
     return out, residual_out

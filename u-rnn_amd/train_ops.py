@@ -227,7 +227,7 @@ def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, s
         ops._seq_check(what, "dstate_out", dstate_out, (B, K - 1, D), x.dtype, contiguous=True)
     shapes = {"dweight": (D, K), **({"dbias": (D,)} if bias is not None else {})}
     g, given = _param_grads_check(what, grads, accumulate, shapes)
-    ops._seq_device(what, x, weight, dout, bias, state, lengths, dstate_out, *given)
+    stream = ops._seq_device(what, x, weight, dout, bias, state, lengths, dstate_out, *given)
     L_ = lib()
     _param_grads(g, shapes, x.device)
     g.setdefault("dbias", None)
@@ -237,7 +237,7 @@ def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, s
     p = ops._ptr
     check(L_.urnn_causal_conv_backward(p(x), *x.stride()[:2], p(weight), p(bias), p(state), p(lengths), p(dout), *dout.stride()[:2], p(dstate_out),
                                        p(g["dx"]), p(g["dstate"]), p(g["dweight"]), p(g["dbias"]), p(ws), ws.numel(), dt, B, L, D, K,
-                                       int(bool(silu)), int(bool(accumulate)), ops._stream()), "urnn_causal_conv_backward")
+                                       int(bool(silu)), int(bool(accumulate)), stream), "urnn_causal_conv_backward")
     return g
 
 
@@ -258,7 +258,7 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
     params = {"dpre_w": pre_w, "dpost_w": post_w, "dscale": scale}
     shapes = {k: (D,) for k, w in params.items() if w is not None}
     g, given = _param_grads_check(what, grads, accumulate, shapes)
-    ops._seq_device(what, y, pre_w, dnormed, dresidual_out, residual, post_w, gate, scale, *given)
+    stream = ops._seq_device(what, y, pre_w, dnormed, dresidual_out, residual, post_w, gate, scale, *given)
     L_ = lib()
     _param_grads(g, shapes, y.device)
     new = lambda: torch.empty(shape, dtype=y.dtype, device=y.device)      # noqa: E731
@@ -271,7 +271,7 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
         g.setdefault(k, None)
     check(L_.urnn_norm_residual_backward(p(y), p(gate), p(residual), p(dnormed), p(dresidual_out), (ctypes.c_long * 5)(*strides), p(pre_w), p(post_w),
                                          p(scale), p(g["dy"]), p(g["dgate"]), p(g["dresidual"]), *out, p(ws), ws.numel(), dt, rows, D,
-                                         ops.GATE_ACTS[gate_act], float(eps), int(bool(accumulate)), ops._stream()), "urnn_norm_residual_backward")
+                                         ops.GATE_ACTS[gate_act], float(eps), int(bool(accumulate)), stream), "urnn_norm_residual_backward")
     return g
 
 
@@ -301,7 +301,7 @@ def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, del
     if delta_bias is not None:
         shapes["ddelta_bias"] = (dim,)
     g, given = _param_grads_check(what, grads, accumulate, shapes)
-    ops._seq_device(what, u, delta, A, B, C, D, z, delta_bias, dout, lengths, dstate_out, *given)
+    stream = ops._seq_device(what, u, delta, A, B, C, D, z, delta_bias, dout, lengths, dstate_out, *given)
     L_ = lib()
     record = ops._scratch(fwd_ws, L_.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1), u.device, key="scan")
     ops._seq_device(what, u, record)
@@ -319,6 +319,6 @@ def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, del
     check(L_.urnn_selective_scan_backward(p(u), p(delta), p(B), p(C), p(z), p(dout), strides, p(A), p(D), p(delta_bias), p(lengths), p(dstate_out),
                                           p(record), record.numel(), p(g["du"]), p(g["ddelta"]), p(g["dB"]), p(g["dC"]), p(g["dz"]), p(g["dA"]),
                                           p(g["dD"]) if D is not None else 0, p(g["ddelta_bias"]) if delta_bias is not None else 0, p(g["dstate"]),
-                                          p(ws), ws.numel(), dt, nb, L, dim, G, N, int(bool(softplus)), int(bool(accumulate)), ops._stream()),
+                                          p(ws), ws.numel(), dt, nb, L, dim, G, N, int(bool(softplus)), int(bool(accumulate)), stream),
           "urnn_selective_scan_backward")
     return g
