@@ -173,55 +173,68 @@ __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqPar
 #pragma unroll
             for (int k = 1; k < K; ++k) line(t0 - K + k, win[k]);
             // s: the token whose dp is formed; j = s - K + 1: the line entry whose gradient is complete then
-            for (long s = t0; s < te + K - 1 || (first && s < K - 1); ++s) {
-                float in[V], dyv[V];
-                line(s, in);
-                const bool live = s < len, own = s < te;         // tokens behind the chunk count for dx, not for the sums
+            const long send = te + K - 1;
+            constexpr int U = 4;                                 // tokens of x and dy in flight
+            float ahead[U][V], dahead[U][V];
+            for (long s0 = t0; s0 < send; s0 += U) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) dyv[i] = 0.0f;
-                if (live) load_v<T, V>(dy + s * p.so.t, dyv);
+                for (int a = 0; a < U; ++a) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
+                    for (int i = 0; i < V; ++i) ahead[a][i] = dahead[a][i] = 0.0f;
+                    if (s0 + a < len && s0 + a < send) {
+                        load_v<T, V>(x + (s0 + a) * p.sx.t, ahead[a]);
+                        load_v<T, V>(dy + (s0 + a) * p.so.t, dahead[a]);
+                    }
+                }
 #pragma unroll
-                    for (int k = 0; k < K - 1; ++k) { win[k][i] = win[k + 1][i]; dp[k][i] = dp[k + 1][i]; }
-                    win[K - 1][i] = in[i];
-                    float g = 0.0f;
-                    if (live) {
-                        g = dyv[i];
-                        if (p.silu) {
-                            float a = bias[i];
+                for (int a = 0; a < U; ++a) {
+                    const long s = s0 + a;
+                    if (s >= send) break;
+                    float (&in)[V] = ahead[a], (&dyv)[V] = dahead[a];
+                    const bool live = s < len, own = s < te;         // tokens behind the chunk count for dx, not for the sums
 #pragma unroll
-                            for (int k = 0; k < K; ++k) a = fmaf(w[k][i], win[k][i], a);
-                            const float sg = sigmoid_f(a);
-                            g *= sg * fmaf(a, 1.0f - sg, 1.0f);
+                    for (int i = 0; i < V; ++i) {
+#pragma unroll
+                        for (int k = 0; k < K - 1; ++k) { win[k][i] = win[k + 1][i]; dp[k][i] = dp[k + 1][i]; }
+                        win[K - 1][i] = in[i];
+                        float g = 0.0f;
+                        if (live) {
+                            g = dyv[i];
+                            if (p.silu) {
+                                float a = bias[i];
+#pragma unroll
+                                for (int k = 0; k < K; ++k) a = fmaf(w[k][i], win[k][i], a);
+                                const float sg = sigmoid_f(a);
+                                g *= sg * fmaf(a, 1.0f - sg, 1.0f);
+                            }
+                        }
+                        dp[K - 1][i] = g;
+                        if (own) {
+                            db[i] += g;
+#pragma unroll
+                            for (int k = 0; k < K; ++k) dw[k][i] = fmaf(g, win[k][i], dw[k][i]);
                         }
                     }
-                    dp[K - 1][i] = g;
-                    if (own) {
-                        db[i] += g;
+                    // dline[j] = sum_k w[k] dp[token j + (K - 1) - k], tokens j .. j + K - 1: dp[0 .. K - 1] of tokens s - K + 1 ..
+                    const long j = s - (K - 1);
+                    if (j >= te || (j < t0 && !first)) continue;
+                    float o[V];
 #pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][i] = fmaf(g, win[k][i], dw[k][i]);
+                    for (int i = 0; i < V; ++i) {
+                        float a = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < K; ++k) a = fmaf(w[k][i], dp[K - 1 - k][i], a);
+                        o[i] = a;
                     }
-                }
-                // dline[j] = sum_k w[k] dp[token j + (K - 1) - k], tokens j .. j + K - 1: dp[0 .. K - 1] of tokens s - K + 1 ..
-                const long j = s - (K - 1);
-                if (j >= te || (j < t0 && !first)) continue;
-                float o[V];
+                    if (dso && j >= (long)len - (K - 1)) {
+                        float v[V];
+                        load_v<T, V>(dso + (j - ((long)len - (K - 1))) * p.dim, v);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float a = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < K; ++k) a = fmaf(w[k][i], dp[K - 1 - k][i], a);
-                    o[i] = a;
+                        for (int i = 0; i < V; ++i) o[i] += v[i];
+                    }
+                    if (j >= 0) store_v<T, V>(dx + j * p.dim, o);
+                    else if (dst) store_v<T, V>(dst + (j + K - 1) * p.dim, o);
                 }
-                if (dso && j >= (long)len - (K - 1)) {
-                    float v[V];
-                    load_v<T, V>(dso + (j - ((long)len - (K - 1))) * p.dim, v);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) o[i] += v[i];
-                }
-                if (j >= 0) store_v<T, V>(dx + j * p.dim, o);
-                else if (dst) store_v<T, V>(dst + (j + K - 1) * p.dim, o);
             }
         }
         float zero[V] = {};
@@ -242,27 +255,9 @@ __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqPar
             float a = 0.0f;
             for (int l = 0; l < yb; ++l) a += s_sum[l * V * xb + r];
             const int i = r / xb, c = cb * xb + r % xb;
-            if (c < nv) p.partial[((long)part * (K + 1) + k) * p.dim + c * V + i] = a;
+            if (c < nv) p.partial[(long)part * (K + 1) * p.dim + (k < K ? (c * V + i) * K + k : K * p.dim + c * V + i)] = a;
         }
     }
-}
-
-// dweight (D,K), dbias (D) (+)= sum over parts of partial [parts][K + 1][D]: a block takes 64 channels of one tap, four lanes of
-// parts; double, because a tap's sum runs over every token of the batch.
-__global__ __launch_bounds__(256) void conv_seq_fold_kernel(const float *__restrict__ partial, int parts, int D, int K, float *dweight, float *dbias, int accumulate)
-{
-    __shared__ double s[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), k = blockIdx.y, r = threadIdx.x >> 6;
-    double a = 0.0;
-    if (c < D)
-        for (int t = r; t < parts; t += 4) a += (double)partial[((long)t * (K + 1) + k) * D + c];
-    s[r][threadIdx.x & 63] = a;
-    __syncthreads();
-    if (r || c >= D) return;
-    const int l = threadIdx.x;
-    const float v = (float)((s[0][l] + s[1][l]) + (s[2][l] + s[3][l]));
-    float *out = k < K ? dweight + (long)c * K + k : dbias ? dbias + c : nullptr;
-    if (out) *out = accumulate ? *out + v : v;
 }
 
 // Work split of the backward: a block takes XB channel vectors, parts x 256 / XB token lanes share the chunks.
@@ -326,6 +321,7 @@ hipError_t urnn_launch_conv_seq_backward(ConvSeqParams p, int dtype, bool wide, 
     const hipError_t e = by_type(p, dtype, wide, 2, st);
     if (e != hipSuccess) return e;
     const int parts = conv_parts(p.batch, p.L, p.dim, 64 * (!wide ? 1 : dtype == URNN_F32 ? 4 : 8));
-    conv_seq_fold_kernel<<<dim3((p.dim + 63) / 64, p.K + 1), 256, 0, st>>>(p.partial, parts, p.dim, p.K, dweight, dbias, accumulate);
-    return hipGetLastError();
+    const long sizes[3] = {(long)p.dim * p.K, p.dim, 0};
+    float *const outs[3] = {dweight, dbias, nullptr};
+    return urnn_launch_sum_parts(p.partial, parts, sizes, outs, accumulate, st);
 }

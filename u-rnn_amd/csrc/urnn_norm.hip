@@ -8,7 +8,7 @@
 //   dv = sum_rows dn hat,  dw = sum_rows dp act(g) yh,  ds = sum_rows dr p.
 //
 // Memory-bound.  A row lives in the registers of NT threads, EPT values each, so that everything is read once and both means are
-// taken on the way: NT = 16 (D <= 128), 64 (<= 1024), 256 (<= 4096), 512, 1024.  The backward reads y, g, r again instead of r' and
+// taken on the way: NT = 16 (D <= 128), 64 (<= 512), 128, 256, 512, 1024.  The backward reads y, g, r again instead of r' and
 // the forward's statistics: r' was rounded on its way out, and it is as many bytes.  Its column sums stay in registers over all rows
 // of a block and are folded in a fixed order.
 #include "urnn_seq.h"
@@ -29,12 +29,13 @@ __device__ __forceinline__ void row_sum2(float &a, float &b, float (*red)[2])
         }
     } else {
         wave_sum_n<2>(v);
-        if (NT > 64) {                               // red: this reduction's own NT / 64 pairs; the caller's next ones use others
+        if (NT > 64) {                               // red: this reduction's own pair of every wave; the caller's next ones use others
             if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6][0] = v[0]; red[threadIdx.x >> 6][1] = v[1]; }
             __syncthreads();
+            const int first = threadIdx.x / NT * (NT / 64);
             v[0] = v[1] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < NT / 64; ++w) { v[0] += red[w][0]; v[1] += red[w][1]; }
+            for (int w = 0; w < NT / 64; ++w) { v[0] += red[first + w][0]; v[1] += red[first + w][1]; }
         }
     }
     a = v[0];
@@ -114,7 +115,7 @@ __device__ __forceinline__ void par_store(float *w, int ln, int D, const float (
 template <typename T, int V, int NT, int EPT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const NormParams p)
 {
-    __shared__ float red[2][NT > 64 ? NT / 64 : 1][2];
+    __shared__ float red[2][NT < 256 ? 4 : NT / 64][2];
     constexpr int RB = NT < 256 ? 256 / NT : 1;
     const int ln = threadIdx.x % NT, D = p.dim;
     const long row0 = (long)blockIdx.x * RB + threadIdx.x / NT;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const NormPar
 template <typename T, int V, int NT, int EPT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(const NormParams p)
 {
-    __shared__ float red[3][NT > 64 ? NT / 64 : 1][2];
+    __shared__ float red[3][NT < 256 ? 4 : NT / 64][2];
     constexpr int RB = NT < 256 ? 256 / NT : 1;
     __shared__ float fold[RB > 1 ? 256 * EPT : 1];
     const int ln = threadIdx.x % NT, rg = threadIdx.x / NT, D = p.dim;
@@ -284,12 +285,13 @@ hipError_t urnn_launch_sum_parts(const float *src, int parts, const long (&n)[3]
     return hipGetLastError();
 }
 
-static int row_threads(int D) { return D <= 128 ? 16 : D <= 1024 ? 64 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024; }
+static int row_threads(int D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
 int urnn_norm_parts(long rows, int D)
 {
     const int nt = row_threads(D), rb = nt < 256 ? 256 / nt : 1;
-    const long blocks = (rows + rb - 1) / rb, most = nt <= 256 ? 1024 : 512;
-    return (int)(blocks < most ? blocks : most);
+    const long blocks = (rows + rb - 1) / rb, most = nt <= 256 ? 768 : 256;      // what is resident
+    const long turns = (blocks + most - 1) / most;                // the same number of turns for every block
+    return (int)((blocks + turns - 1) / turns);
 }
 
 template <typename T, int V, int NT, int EPT>
@@ -306,10 +308,10 @@ static hipError_t by_width(const NormParams &p, bool backward, hipStream_t st)
     const int D = p.dim;
     if (D <= 128) return launch_norm<T, V, 16, 8>(p, backward, st);
     if (D <= 512) return launch_norm<T, V, 64, 8>(p, backward, st);
-    if (D <= 1024) return launch_norm<T, V, 64, 16>(p, backward, st);
+    if (D <= 1024) return launch_norm<T, V, 128, 8>(p, backward, st);
     if (D <= 2048) return launch_norm<T, V, 256, 8>(p, backward, st);
-    if (D <= 4096) return launch_norm<T, V, 256, 16>(p, backward, st);
-    if (D <= 8192) return launch_norm<T, V, 512, 16>(p, backward, st);
+    if (D <= 4096) return launch_norm<T, V, 512, 8>(p, backward, st);
+    if (D <= 8192) return launch_norm<T, V, 1024, 8>(p, backward, st);
     return launch_norm<T, V, 1024, 16>(p, backward, st);
 }
 static hipError_t by_type(const NormParams &p, int dtype, bool wide, bool backward, hipStream_t st)

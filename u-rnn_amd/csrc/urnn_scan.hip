@@ -254,49 +254,82 @@ static hipError_t launch_scan(const ScanParams &p, hipStream_t st)
     return hipGetLastError();
 }
 
-// One token: state and inputs are read once, the new state and y written once.  A quad per channel again, no LDS.  state_out may be
+// One token: state and inputs are read once, the new state and y written once.  A quad per channel, no LDS; a thread takes the same
+// channel of R sequences, so that their loads are in flight together and A, bias and skip are read once for them.  state_out may be
 // state: every thread reads its own states before it writes them.
-template <typename T, int NP>
+template <typename T, int E>
+__device__ __forceinline__ void load_row(const T *row, int q, int N, bool vec, float (&v)[E])
+{
+    constexpr int W = E < 4 ? E : 4;
+    if (vec) {
+#pragma unroll
+        for (int e = 0; e < E; e += W) {
+            Pack<T, W> t = {};
+            if (q * E + e < N) t = *reinterpret_cast<const Pack<T, W> *>(row + q * E + e);
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[e + i] = to_f(t.v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = q * E + e < N ? to_f(row[q * E + e]) : 0.0f;
+    }
+}
+
+template <typename T, int NP, int R>
 __global__ __launch_bounds__(256) void scan_step_kernel(const ScanParams p)
 {
     constexpr int E = NP / 4, W = E < 4 ? E : 4;
-    const long item = (long)blockIdx.x * 64 + (threadIdx.x >> 2);
-    const int q = threadIdx.x & 3;
-    if (item >= (long)p.batch * p.dim) return;
-    const int b = (int)(item / p.dim), d = (int)(item % p.dim), g = d / (p.dim / p.G);
-    float h[E], A2[E], Bv[E], Cv[E];
-    load_states<E>(p.state + item * p.N, q, p.N, states_vec(p.state, p.N, W), h);
+    const unsigned item = blockIdx.x * 64u + (threadIdx.x >> 2), d = item % p.dim;
+    const int q = threadIdx.x & 3, b0 = (int)(item / p.dim) * R, g = d / (p.dim / p.G);
+    if (b0 >= p.batch) return;
+    const bool vs = states_vec(p.state, p.N, W), vo = states_vec(p.state_out, p.N, W);
+    const bool vB = ((reinterpret_cast<uintptr_t>(p.B) | (p.sB.b | p.N) * sizeof(T)) & (W * sizeof(T) - 1)) == 0;
+    const bool vC = ((reinterpret_cast<uintptr_t>(p.C) | (p.sC.b | p.N) * sizeof(T)) & (W * sizeof(T) - 1)) == 0;
+    float h[R][E], Bv[R][E], Cv[R][E], A2[E], u[R], dl[R], zf[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const long b = b0 + r < p.batch ? b0 + r : b0;
+        load_states<E>(p.state + (b * p.dim + d) * p.N, q, p.N, vs, h[r]);
+        load_row<T, E>(reinterpret_cast<const T *>(p.B) + b * p.sB.b + (long)g * p.N, q, p.N, vB, Bv[r]);
+        load_row<T, E>(reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N, q, p.N, vC, Cv[r]);
+        u[r] = to_f(reinterpret_cast<const T *>(p.u)[b * p.su.b + d]);
+        dl[r] = to_f(reinterpret_cast<const T *>(p.delta)[b * p.sd.b + d]);
+        zf[r] = p.z ? to_f(reinterpret_cast<const T *>(p.z)[b * p.sz.b + d]) : 0.0f;
+    }
     load_states<E>(p.A + (long)d * p.N, q, p.N, states_vec(p.A, p.N, W), A2);
-    const T *Bp = reinterpret_cast<const T *>(p.B) + b * p.sB.b + (long)g * p.N, *Cp = reinterpret_cast<const T *>(p.C) + b * p.sC.b + (long)g * p.N;
+    const float bias = p.bias ? p.bias[d] : 0.0f, skip = p.D ? p.D[d] : 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int n = q * E + e;
-        Bv[e] = n < p.N ? to_f(Bp[n]) : 0.0f;
-        Cv[e] = n < p.N ? to_f(Cp[n]) : 0.0f;
-    }
-    const float u = to_f(reinterpret_cast<const T *>(p.u)[b * p.su.b + d]);
-    const float raw = to_f(reinterpret_cast<const T *>(p.delta)[b * p.sd.b + d]) + (p.bias ? p.bias[d] : 0.0f);
-    const float zf = p.z ? to_f(reinterpret_cast<const T *>(p.z)[b * p.sz.b + d]) : 0.0f;
-    const float skip = p.D ? p.D[d] : 0.0f;
-    const float step = p.softplus ? softplus_f(raw) : raw, su = step * u;
-    float y = 0.0f;
+    for (int r = 0; r < R; ++r) {
+        if (b0 + r >= p.batch) break;
+        const long b = b0 + r;
+        const float raw = dl[r] + bias, step = p.softplus ? softplus_f(raw) : raw, su = step * u[r];
+        float y = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        h[e] = fmaf(exp_fast(step * A2[e]), h[e], su * Bv[e]);
-        y = fmaf(Cv[e], h[e], y);
+        for (int e = 0; e < E; ++e) {
+            h[r][e] = fmaf(exp_fast(step * A2[e]), h[r][e], su * Bv[r][e]);
+            y = fmaf(Cv[r][e], h[r][e], y);
+        }
+        y = fmaf(skip, u[r], quad_sum(y));
+        if (p.z) y *= silu_f(zf[r]);
+        store_states<E>(p.state_out + (b * p.dim + d) * p.N, q, p.N, vo, h[r]);
+        if (q == 0) reinterpret_cast<T *>(p.y)[b * p.dim + d] = from_f<T>(y);
     }
-    y = fmaf(skip, u, quad_sum(y));
-    if (p.z) y *= silu_f(zf);
-    store_states<E>(p.state_out + item * p.N, q, p.N, states_vec(p.state_out, p.N, W), h);
-    if (q == 0) reinterpret_cast<T *>(p.y)[item] = from_f<T>(y);
 }
 
+template <typename T, int NP, int R>
+static hipError_t launch_step_rows(const ScanParams &p, hipStream_t st)
+{
+    const long items = (long)((p.batch + R - 1) / R) * p.dim;
+    scan_step_kernel<T, NP, R><<<dim3((unsigned)((items + 63) / 64)), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+// Four sequences to a thread once the threads still fill the chip (2048 blocks of 256)
 template <typename T, int NP>
 static hipError_t launch_step(const ScanParams &p, hipStream_t st)
 {
-    const long items = (long)p.batch * p.dim;
-    scan_step_kernel<T, NP><<<dim3((unsigned)((items + 63) / 64)), 256, 0, st>>>(p);
-    return hipGetLastError();
+    if constexpr (NP <= 16)
+        if ((long)p.batch * p.dim >= 4l * 64 * 2048) return launch_step_rows<T, NP, 4>(p, st);
+    return launch_step_rows<T, NP, 1>(p, st);
 }
 
 template <typename T>

@@ -188,7 +188,7 @@ struct ConvSeqParams {
     // backward
     const void *dstate_out;                          // (B,K-1,D) or NULL
     void *dx, *dstate;                               // (B,L,D), (B,K-1,D) or NULL
-    float *partial;                                  // [parts][K + 1][dim]: sums of a block's tokens for weight and bias
+    float *partial;                                  // [parts][dim K | dim]: sums of a block's tokens for weight and bias
     int parts;
 };
 
