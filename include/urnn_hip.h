@@ -489,21 +489,23 @@ int urnn_selective_scan_step(const void *u, const void *delta, const void *Bmat,
 /* The norms around a block: per row of D channels (D <= 16384)
  *   residual_out = residual + scale * act(gate) * post_w * y / rms(y),   normed = pre_w * residual_out / rms(residual_out),
  * rms(x) = sqrt(mean(x^2) + eps).  post_w NULL: y enters as it is; gate / residual / scale NULL: left out; act: URNN_GATE_*.
- * strides: row strides of y, gate, residual.  normed, residual_out (rows,D) contiguous, residual_out may be NULL; either may be y, gate or
+ * Row r of an input lies at (r / inner) * strides[2 k] + (r % inner) * strides[2 k + 1] elements, k = 0 y, 1 gate, 2 residual (inner divides
+ * rows; inner == rows: evenly spaced rows).  normed, residual_out (rows,D) contiguous, residual_out may be NULL; either may be y, gate or
  * residual themselves where those are contiguous. */
 #define URNN_GATE_NONE 0
 #define URNN_GATE_SIGMOID 1
 #define URNN_GATE_SILU 2
 int urnn_norm_residual(const void *y, const void *gate, const void *residual, const long *strides, const float *pre_w,
-                       const float *post_w, const float *scale, void *normed, void *residual_out, int dtype, long rows, int D, int act,
-                       float eps, void *stream);
-/* Gradients, given dnormed and dresidual_out (either may be NULL: zeros).  strides: y, gate, residual, dnormed, dresidual_out.  dgate /
+                       const float *post_w, const float *scale, void *normed, void *residual_out, int dtype, long rows, long inner, int D,
+                       int act, float eps, void *stream);
+/* Gradients, given dnormed and dresidual_out (either may be NULL: zeros).  strides: of y, gate, residual, dnormed,
+ * dresidual_out, as above.  dgate /
  * dresidual may be NULL; dpre_w, dpost_w, dscale (D) float32, each may be NULL, overwritten or added to (accumulate != 0). */
 size_t urnn_norm_residual_backward_workspace_bytes(long rows, int D);
 int urnn_norm_residual_backward(const void *y, const void *gate, const void *residual, const void *dnormed, const void *dresidual_out,
                                 const long *strides, const float *pre_w, const float *post_w, const float *scale, void *dy, void *dgate,
                                 void *dresidual, float *dpre_w, float *dpost_w, float *dscale, void *workspace, size_t workspace_bytes,
-                                int dtype, long rows, int D, int act, float eps, int accumulate, void *stream);
+                                int dtype, long rows, long inner, int D, int act, float eps, int accumulate, void *stream);
 
 #ifdef __cplusplus
 }

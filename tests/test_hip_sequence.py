@@ -489,7 +489,7 @@ def test_refusals_norm_residual():
     refused("gate has shape", ops.norm_residual, **{**c, "gate": torch.zeros(1, 8)})
     refused("residual is torch.bfloat16", ops.norm_residual, **{**c, "residual": c["residual"].bfloat16()})
     refused("16384", ops.norm_residual, torch.zeros(1, 16385), torch.zeros(16385))
-    refused("not evenly spaced", ops.norm_residual, torch.zeros(3, 4, 16, 8)[:, :, ::3], c["pre_w"])
+    refused("not evenly spaced", ops.norm_residual, torch.zeros(3, 4, 16, 8)[:, :, ::3], c["pre_w"])      # (B, L, D) may be spaced in any way
     buf = torch.zeros(5, 8)
     refused("out overlaps an input", ops.norm_residual, **{**c, "y": buf[:4]}, out=buf[1:])
     refused("out overlaps an input", ops.norm_residual, **c, out=buf[1:], residual_out=buf[:4])
@@ -515,5 +515,223 @@ def test_c_entries_refuse_without_a_gpu():
     assert L.urnn_selective_scan(*args, 16, 16, 0, 0, 1, 300, 8, 1, 4, 1, 0) == -3
     assert L.urnn_selective_scan(*args, 8, 1 << 30, 0, 0, 1, 300, 8, 1, 4, 1, 0) == -4
     assert L.urnn_selective_scan_workspace_bytes(1, 300, 8, 4, 1) > L.urnn_selective_scan_workspace_bytes(1, 300, 8, 4, 0) > 0
-    assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 32, 32, 0, 1, 8, 0, 1e-5, 0) == -1 and b"same buffer" in L.urnn_last_error()
-    assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 32, 0, 0, 1, 16385, 0, 1e-5, 0) == -1
+    assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 32, 32, 0, 1, 1, 8, 0, 1e-5, 0) == -1 and b"same buffer" in L.urnn_last_error()
+    assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 32, 0, 0, 1, 1, 16385, 0, 1e-5, 0) == -1
+    assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 32, 0, 0, 6, 4, 8, 0, 1e-5, 0) == -1 and b"rows" in L.urnn_last_error()
+
+
+# ---- a run of them together -------------------------------------------------------------------------------------------------------
+class Block:
+    """norm -> projection -> convolution -> projection -> scan -> projection -> norm, as a model's layer: the projections are plain
+    products, everything between them is this library's."""
+
+    def __init__(self, width, dim, N, K, rank, dtype, seed):
+        g = rng(seed)
+        self.dim, self.N, self.rank, self.dtype = dim, N, rank, dtype
+        self.w_in = make(g, width, 2 * dim, scale=width ** -0.5, dtype=dtype)
+        self.w_x = make(g, dim, rank + 2 * N, scale=dim ** -0.5, dtype=dtype)
+        self.w_dt = make(g, rank, dim, scale=rank ** -0.5, dtype=dtype)
+        self.w_out = make(g, dim, width, scale=dim ** -0.5, dtype=dtype)
+        self.conv_w, self.conv_b = make(g, dim, K, scale=0.5), make(g, dim, scale=0.1)
+        self.A = -torch.arange(1, N + 1).float().repeat(dim, 1).cuda()
+        self.D, self.dt_b = make(g, dim), make(g, dim, scale=0.3) - 2.0
+        self.pre_w, self.post_w, self.scale = 1 + make(g, width, scale=0.1), 1 + make(g, width, scale=0.1), make(g, width, scale=0.3)
+
+    def first(self, x):
+        return ops.norm_residual(x, self.pre_w)[0]
+
+    def split(self, u):
+        p = u @ self.w_x
+        return (p[..., :self.rank] @ self.w_dt), p[..., self.rank:self.rank + self.N], p[..., self.rank + self.N:]
+
+    def inner(self, x, n, conv_state=None, state=None, lengths=None):
+        """-> (residual, normed, conv state, state) of a (B, L, width) run."""
+        xz = n @ self.w_in
+        u, cs = ops.causal_conv(xz[..., :self.dim], self.conv_w, bias=self.conv_b, state=conv_state, lengths=lengths, want_state=True)
+        dt, B, C = self.split(u)
+        y, st = ops.selective_scan(u, dt, self.A, B, C, D=self.D, z=xz[..., self.dim:], delta_bias=self.dt_b, state=state, lengths=lengths,
+                                   want_state=True)
+        normed, res = ops.norm_residual(y @ self.w_out, self.pre_w, residual=x, post_w=self.post_w, scale=self.scale)
+        return res, normed, cs, st
+
+    def token(self, x, n, conv_state, state):
+        """One token, states in place."""
+        xz = n @ self.w_in
+        u, _ = ops.causal_conv_step(xz[:, :self.dim], conv_state, self.conv_w, bias=self.conv_b, state_out=conv_state)
+        dt, B, C = self.split(u)
+        y, _ = ops.selective_scan_step(u, dt, self.A, B, C, state, D=self.D, z=xz[:, self.dim:], delta_bias=self.dt_b, state_out=state)
+        return ops.norm_residual(y @ self.w_out, self.pre_w, residual=x, post_w=self.post_w, scale=self.scale)
+
+
+@gpu
+def test_block_prompt_then_tokens():
+    """A prompt in two pieces and then token by token gives what the whole sequence gives at once, and a padded batch what its rows give
+    alone.  float32; the two ways add the same terms in different orders: 2^-24 x 400 roundings along 40 tokens and three products."""
+    blk = Block(24, 48, 8, 4, 6, torch.float32, 5)
+    x = make(rng(6), 3, 40, 24)
+    res, normed, cs, st = blk.inner(x, blk.first(x))
+    tol = dict(rtol=400 * seq_ref.U32, atol=400 * seq_ref.U32 * 8)
+    r1, n1, c1, s1 = blk.inner(x[:, :17], blk.first(x[:, :17]))
+    r2, n2, c2, s2 = blk.inner(x[:, 17:33], blk.first(x[:, 17:33]), c1, s1)
+    assert torch.allclose(torch.cat([r1, r2], 1), res[:, :33], **tol) and torch.allclose(torch.cat([n1, n2], 1), normed[:, :33], **tol)
+    for t in range(33, 40):
+        n, r = blk.token(x[:, t], blk.first(x[:, t]), c2, s2)
+        assert torch.allclose(r, res[:, t], **tol) and torch.allclose(n, normed[:, t], **tol)
+    assert torch.allclose(c2, cs, **tol) and torch.allclose(s2, st, **tol)
+    lens = [40, 9, 0]
+    _, _, cp, sp = blk.inner(x, blk.first(x), lengths=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    rp, _, _, _ = blk.inner(x, blk.first(x), lengths=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    for b, n in enumerate(lens):
+        if n:
+            ra, _, ca, sa = blk.inner(x[b:b + 1, :n], blk.first(x[b:b + 1, :n]))
+            assert torch.allclose(rp[b, :n], ra[0], **tol) and torch.allclose(cp[b], ca[0], **tol) and torch.allclose(sp[b], sa[0], **tol)
+    assert torch.equal(sp[2], torch.zeros_like(sp[2])) and torch.equal(rp[1, 9:], x[1, 9:])      # a block of zeros adds nothing
+
+
+@gpu
+def test_block_training_window_against_autograd():
+    """The chain's gradients -- norm, convolution, scan, norm, with plain products between -- against autograd through the float64 formulas.
+    400 roundings of float32 on every path, relative to the largest gradient of a tensor (sums of both signs)."""
+    B, L, W, dim, N, K, R = 2, 23, 12, 20, 4, 3, 5
+    blk = Block(W, dim, N, K, R, torch.float32, 9)
+    x = make(rng(10), B, L, W)
+    dn, dr = make(rng(11), B, L, W), make(rng(12), B, L, W)
+    cs0, st0 = make(rng(13), B, K - 1, dim), make(rng(14), B, dim, N)
+
+    # the library's kernels, the products' gradients written out
+    n0, _ = ops.norm_residual(x, blk.pre_w)
+    xz = n0 @ blk.w_in
+    xc, z = xz[..., :dim], xz[..., dim:]
+    u = ops.causal_conv(xc, blk.conv_w, bias=blk.conv_b, state=cs0)
+    dt, Bm, Cm = blk.split(u)
+    ws = ops.selective_scan_workspace(u, blk.A)
+    scan = dict(A=blk.A, B=Bm, C=Cm, D=blk.D, z=z, delta_bias=blk.dt_b)
+    y = ops.selective_scan(u, dt, state=st0, ws=ws, **scan)
+    o = y @ blk.w_out
+    gn = train_ops.norm_residual_backward(o, blk.pre_w, dn, dresidual_out=dr, residual=x, post_w=blk.post_w, scale=blk.scale)
+    gs = train_ops.selective_scan_backward(u, dt, dout=gn["dy"] @ blk.w_out.t(), fwd_ws=ws, want_dstate=True, **scan)
+    dp = torch.cat([gs["ddelta"] @ blk.w_dt.t(), gs["dB"], gs["dC"]], -1)
+    gc = train_ops.causal_conv_backward(xc, blk.conv_w, gs["du"] + dp @ blk.w_x.t(), bias=blk.conv_b, state=cs0)
+    gp = train_ops.norm_residual_backward(x, blk.pre_w, torch.cat([gc["dx"], gs["dz"]], -1) @ blk.w_in.t(), grads={"dpre_w": gn["dpre_w"]},
+                                          accumulate=True)
+    got = {"x": gn["dresidual"] + gp["dy"], "pre_w": gp["dpre_w"], "post_w": gn["dpost_w"], "scale": gn["dscale"], "conv_w": gc["dweight"],
+           "conv_b": gc["dbias"], "A": gs["dA"], "D": gs["dD"], "dt_b": gs["ddelta_bias"], "cs0": gc["dstate"], "st0": gs["dstate"]}
+
+    f = lambda t: t.double().cpu().requires_grad_(True)      # noqa: E731
+    P = {k: f(v) for k, v in {"x": x, "pre_w": blk.pre_w, "post_w": blk.post_w, "scale": blk.scale, "conv_w": blk.conv_w, "conv_b": blk.conv_b,
+                              "A": blk.A, "D": blk.D, "dt_b": blk.dt_b, "cs0": cs0, "st0": st0}.items()}
+    wi, wx, wd, wo = (t.double().cpu() for t in (blk.w_in, blk.w_x, blk.w_dt, blk.w_out))
+    rms = lambda t: t * torch.rsqrt((t * t).mean(-1, keepdim=True) + 1e-5)      # noqa: E731
+    pz = rms(P["x"]) * P["pre_w"] @ wi
+    line = torch.cat([P["cs0"], pz[..., :dim]], 1)
+    uu = torch.nn.functional.silu(sum(line[:, k:k + L] * P["conv_w"][:, k] for k in range(K)) + P["conv_b"])
+    pr = uu @ wx
+    step = seq_ref.softplus64(pr[..., :R] @ wd + P["dt_b"])
+    h, rows = P["st0"], []
+    for t in range(L):
+        h = torch.exp(step[:, t, :, None] * P["A"]) * h + (step[:, t] * uu[:, t])[..., None] * pr[:, t, None, R:R + N]
+        rows.append((h * pr[:, t, None, R + N:]).sum(-1) + P["D"] * uu[:, t])
+    yy = torch.stack(rows, 1) * torch.nn.functional.silu(pz[..., dim:])
+    res = P["x"] + P["scale"] * rms(yy @ wo) * P["post_w"]
+    want = torch.autograd.grad([rms(res) * P["pre_w"], res], list(P.values()), [dn.double().cpu(), dr.double().cpu()])
+    for (k, w) in zip(P, want):
+        off = (got[k].double().cpu() - w).abs().max().item()
+        assert off <= 400 * seq_ref.U32 * w.abs().max().item() + 1e-7, (k, off, w.abs().max().item())
+
+
+@gpu
+def test_calls_are_bit_reproducible_on_any_stream_and_in_graphs():
+    """Two calls at once on two streams, and graphs replayed several times with eager work between, give the eager bits; two captured graphs
+    with one Arena's buffers between them replay in turn."""
+    c, n = scan_case(2, 210, 48, 16, 2, torch.bfloat16, 31, lengths=[210, 77])
+    cc, _ = conv_case(2, 210, 48, 4, torch.bfloat16, 32)
+    nc = norm_case(300, 96, torch.bfloat16, 33)
+    dout, dn = make(rng(34), 2, 210, 48, dtype=torch.bfloat16), make(rng(35), 300, 96, dtype=torch.bfloat16)
+    arena = ops.Arena("cuda")
+    back = {k: v for k, v in c.items() if k != "state"}
+
+    def work(ar=None):
+        y = ops.causal_conv(cc["x"], cc["weight"], bias=cc["bias"], state=cc["state"])
+        gc = train_ops.causal_conv_backward(cc["x"], cc["weight"], dout, bias=cc["bias"], state=cc["state"], scratch=ar)
+        ws = ar if ar is not None else ops.selective_scan_workspace(c["u"], c["A"])
+        s = ops.selective_scan(**c, lengths=n, ws=ws)
+        gs = train_ops.selective_scan_backward(**back, dout=dout, fwd_ws=ws, lengths=n, scratch=ar)
+        m, r = ops.norm_residual(**nc)
+        gn = train_ops.norm_residual_backward(dnormed=dn, scratch=ar, **nc)
+        h = ops.selective_scan_step(**{**c, **{k: c[k][:, 0] for k in ("u", "delta", "B", "C", "z")}})
+        return [y, s, m, r, *h] + [v for g in (gc, gs, gn) for k, v in sorted(g.items()) if v is not None]
+
+    eager = [t.clone() for t in work()]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    s1.wait_stream(torch.cuda.current_stream())
+    s2.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s1):
+        a = work()
+    with torch.cuda.stream(s2):
+        b = work()
+    torch.cuda.synchronize()
+    for x, y, z in zip(eager, a, b):
+        assert torch.equal(x, y) and torch.equal(x, z)
+    work(arena)                                                # sizes the arena
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(work(arena))
+        graphs.append(g)
+    for turn in range(4):
+        for g, out in zip(graphs, outs):
+            for t in out:
+                t.fill_(7)
+            g.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(eager, out):
+                assert torch.equal(x, y), turn
+            assert torch.equal(work()[1], eager[1])
+
+
+@gpu
+def test_tensors_of_another_device_are_refused():
+    class Elsewhere:                                           # a box has one GPU: a tensor that says it is on another one
+        shape, dtype, device = (1, 2), torch.float32, torch.device("cuda:1")
+        is_cuda = True
+
+        def get_device(self):
+            return 1
+    with pytest.raises(RuntimeError, match="current device"):
+        ops._seq_device("op", Elsewhere())
+    with pytest.raises(RuntimeError, match="tensors on"):
+        ops._seq_device("op", torch.zeros(1, device="cuda"), Elsewhere())
+
+
+@gpu
+def test_large_offsets():
+    """A sequence whose tokens lie beyond 2^31 elements of the first: strides of 64 bits."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB")
+    L, D, N = 66, 64, 4
+    stride = (1 << 32) // 128 + 64                             # elements between tokens: 64 tokens are 2^31
+    big = torch.empty(stride * L + 2 * D, dtype=torch.bfloat16, device="cuda")
+    x, z = big.as_strided((1, L, D), (stride * L, stride, 1)), big.as_strided((1, L, D), (stride * L, stride, 1), D)
+    small, zs = make(rng(1), 1, L, D, dtype=torch.bfloat16), make(rng(2), 1, L, D, dtype=torch.bfloat16)
+    x.copy_(small)
+    z.copy_(zs)
+    c, _ = scan_case(1, L, D, N, 1, torch.bfloat16, 3)
+    assert torch.equal(ops.selective_scan(**{**c, "u": x, "z": z}), ops.selective_scan(**{**c, "u": small, "z": zs}))
+    w = make(rng(4), D, 4)
+    assert torch.equal(ops.causal_conv(x, w), ops.causal_conv(small, w))
+    a, b = train_ops.causal_conv_backward(x, w, z), train_ops.causal_conv_backward(small, w, zs)
+    assert torch.equal(a["dx"], b["dx"]) and torch.equal(a["dweight"], b["dweight"])
+    g = {}
+    for u_, z_, d_ in ((x, z, x), (small, zs, small)):
+        ws = ops.selective_scan_workspace(u_, c["A"])
+        ops.selective_scan(**{**c, "u": u_, "z": z_}, ws=ws)
+        g[u_.stride(1)] = train_ops.selective_scan_backward(**{**{k: v for k, v in c.items() if k != "state"}, "u": u_, "z": z_}, dout=d_, fwd_ws=ws)
+    a, b = g.values()
+    for k in ("du", "ddelta", "dz", "dA", "dB", "dC", "dD"):
+        assert torch.equal(a[k], b[k]), k
+    n1 = ops.norm_residual(x[0], w[:, 0].contiguous())
+    n2 = ops.norm_residual(small[0], w[:, 0].contiguous())
+    assert torch.equal(n1[0], n2[0])

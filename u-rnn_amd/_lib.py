@@ -84,9 +84,9 @@ SIGNATURES = {
     "urnn_selective_scan_backward_workspace_bytes": (_sz, [_i] * 5),
     "urnn_selective_scan_backward": (_i, [_p] * 13 + [_sz] + [_p] * 10 + [_sz] + [_i] * 8 + [_p]),
     "urnn_selective_scan_step": (_i, [_p] * 12 + [_i] * 6 + [_p]),
-    "urnn_norm_residual": (_i, [_p] * 9 + [_i, _l, _i, _i, _f, _p]),
+    "urnn_norm_residual": (_i, [_p] * 9 + [_i, _l, _l, _i, _i, _f, _p]),
     "urnn_norm_residual_backward_workspace_bytes": (_sz, [_l, _i]),
-    "urnn_norm_residual_backward": (_i, [_p] * 16 + [_sz, _i, _l, _i, _i, _f, _i, _p]),
+    "urnn_norm_residual_backward": (_i, [_p] * 16 + [_sz, _i, _l, _l, _i, _i, _f, _i, _p]),
 }
 
 

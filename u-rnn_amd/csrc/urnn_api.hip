@@ -1748,29 +1748,30 @@ extern "C" int urnn_selective_scan_step(const void *u, const void *delta, const 
     return URNN_OK;
 }
 
-static int norm_args(const char *what, const void *y, const long *strides, const float *pre_w, int dtype, long rows, int D, int act)
+static int norm_args(const char *what, const void *y, const long *strides, const float *pre_w, int dtype, long rows, long inner, int D, int act)
 {
     if (!y || !strides || !pre_w) return fail(URNN_ENULL, "%s: NULL argument", what);
     if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
     if (rows < 1 || rows > 8388608 || D < 1 || D > URNN_SEQ_MAX_NORM) return fail(URNN_EINVAL, "%s: rows=%ld (1..8388608) D=%d (1..%d)", what, rows, D, URNN_SEQ_MAX_NORM);
+    if (inner < 1 || inner > rows || rows % inner) return fail(URNN_EINVAL, "%s: %ld rows of %ld each", what, rows, inner);
     if (act < URNN_GATE_NONE || act > URNN_GATE_SILU) return fail(URNN_EINVAL, "%s: act=%d", what, act);
     return URNN_OK;
 }
 
 extern "C" int urnn_norm_residual(const void *y, const void *gate, const void *residual, const long *strides, const float *pre_w,
-                                  const float *post_w, const float *scale, void *normed, void *residual_out, int dtype, long rows, int D, int act,
-                                  float eps, void *stream)
+                                  const float *post_w, const float *scale, void *normed, void *residual_out, int dtype, long rows, long inner, int D,
+                                  int act, float eps, void *stream)
 {
-    const int rc = norm_args("urnn_norm_residual", y, strides, pre_w, dtype, rows, D, act);
+    const int rc = norm_args("urnn_norm_residual", y, strides, pre_w, dtype, rows, inner, D, act);
     if (rc) return rc;
     if (!normed) return fail(URNN_ENULL, "urnn_norm_residual: NULL argument");
     if (normed == residual_out) return fail(URNN_EINVAL, "urnn_norm_residual: normed and residual_out are the same buffer");
     NormParams p = {};
-    p.y = y; p.gate = gate; p.residual = residual; p.sy = strides[0]; p.sg = strides[1]; p.sr = strides[2];
+    p.y = y; p.gate = gate; p.residual = residual; p.sy = {strides[0], strides[1]}; p.sg = {strides[2], strides[3]}; p.sr = {strides[4], strides[5]}; p.inner = (unsigned)inner;
     p.pre_w = pre_w; p.post_w = post_w; p.scale = scale; p.normed = normed; p.res_out = residual_out;
     p.rows = rows; p.dim = D; p.act = act; p.eps = eps;
     const int e = seq_elem(dtype);
-    const bool wide = wide_rows(y, strides[0], 0, e) && wide_rows(gate, strides[1], 0, e) && wide_rows(residual, strides[2], 0, e) && (long)D * e % 16 == 0 &&
+    const bool wide = wide_rows(y, strides[0], strides[1], e) && wide_rows(gate, strides[2], strides[3], e) && wide_rows(residual, strides[4], strides[5], e) && (long)D * e % 16 == 0 &&
                       aligned16(pre_w) && (!post_w || aligned16(post_w)) && (!scale || aligned16(scale)) && aligned16(normed) && (!residual_out || aligned16(residual_out));
     CHECK_HIP(urnn_launch_norm(p, dtype, wide, (hipStream_t)stream), "norm_residual");
     return URNN_OK;
@@ -1785,9 +1786,9 @@ extern "C" size_t urnn_norm_residual_backward_workspace_bytes(long rows, int D)
 extern "C" int urnn_norm_residual_backward(const void *y, const void *gate, const void *residual, const void *dnormed, const void *dresidual_out,
                                            const long *strides, const float *pre_w, const float *post_w, const float *scale, void *dy, void *dgate,
                                            void *dresidual, float *dpre_w, float *dpost_w, float *dscale, void *workspace, size_t workspace_bytes,
-                                           int dtype, long rows, int D, int act, float eps, int accumulate, void *stream)
+                                           int dtype, long rows, long inner, int D, int act, float eps, int accumulate, void *stream)
 {
-    const int rc = norm_args("urnn_norm_residual_backward", y, strides, pre_w, dtype, rows, D, act);
+    const int rc = norm_args("urnn_norm_residual_backward", y, strides, pre_w, dtype, rows, inner, D, act);
     if (rc) return rc;
     if (!dy || !workspace) return fail(URNN_ENULL, "urnn_norm_residual_backward: NULL argument");
     if (dgate && !gate) return fail(URNN_ENULL, "urnn_norm_residual_backward: dgate without gate");
@@ -1795,13 +1796,13 @@ extern "C" int urnn_norm_residual_backward(const void *y, const void *gate, cons
     if (workspace_bytes < urnn_norm_residual_backward_workspace_bytes(rows, D)) return fail(URNN_EWORKSPACE, "urnn_norm_residual_backward: workspace too small");
     NormParams p = {};
     p.y = y; p.gate = gate; p.residual = residual; p.dnormed = dnormed; p.dres = dresidual_out;
-    p.sy = strides[0]; p.sg = strides[1]; p.sr = strides[2]; p.sdn = strides[3]; p.sdr = strides[4];
+    p.sy = {strides[0], strides[1]}; p.sg = {strides[2], strides[3]}; p.sr = {strides[4], strides[5]}; p.inner = (unsigned)inner; p.sdn = {strides[6], strides[7]}; p.sdr = {strides[8], strides[9]};
     p.pre_w = pre_w; p.post_w = post_w; p.scale = scale; p.dy = dy; p.dgate = dgate; p.dresidual = dresidual;
     p.partial = reinterpret_cast<float *>(workspace);
     p.rows = rows; p.dim = D; p.act = act; p.eps = eps; p.parts = urnn_norm_parts(rows, D);
     const int e = seq_elem(dtype);
-    const bool wide = wide_rows(y, strides[0], 0, e) && wide_rows(gate, strides[1], 0, e) && wide_rows(residual, strides[2], 0, e) &&
-                      wide_rows(dnormed, strides[3], 0, e) && wide_rows(dresidual_out, strides[4], 0, e) && (long)D * e % 16 == 0 && aligned16(pre_w) &&
+    const bool wide = wide_rows(y, strides[0], strides[1], e) && wide_rows(gate, strides[2], strides[3], e) && wide_rows(residual, strides[4], strides[5], e) &&
+                      wide_rows(dnormed, strides[6], strides[7], e) && wide_rows(dresidual_out, strides[8], strides[9], e) && (long)D * e % 16 == 0 && aligned16(pre_w) &&
                       (!post_w || aligned16(post_w)) && (!scale || aligned16(scale)) && aligned16(dy) && (!dgate || aligned16(dgate)) &&
                       (!dresidual || aligned16(dresidual));
     CHECK_HIP(urnn_launch_norm_backward(p, dtype, wide, dpre_w, dpost_w, dscale, accumulate, (hipStream_t)stream), "norm_residual_backward");

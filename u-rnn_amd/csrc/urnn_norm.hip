@@ -53,6 +53,12 @@ __device__ __forceinline__ void gate_of(int act, float g, float &a, float &da)
 }
 
 // Values of a thread: EPT / V groups of V adjacent channels, NT V apart.
+template <typename T>
+__device__ __forceinline__ const T *row_at(const void *base, const SeqStride &s, long row, unsigned inner)
+{
+    const unsigned r = (unsigned)row;                // at most 2^23 rows
+    return reinterpret_cast<const T *>(base) + (long)(r / inner) * s.b + (long)(r % inner) * s.t;
+}
 template <typename T, int V, int NT, int EPT>
 __device__ __forceinline__ void row_load(const T *row, int ln, int D, float (&v)[EPT])
 {
@@ -123,12 +129,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const NormPar
     const long row = ok ? row0 : 0;
     const float inv = 1.0f / (float)D;
     float y[EPT], r[EPT], w[EPT], s[EPT], v[EPT];
-    row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.y) + row * p.sy, ln, D, y);
+    row_load<T, V, NT, EPT>(row_at<T>(p.y, p.sy, row, p.inner), ln, D, y);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) r[i] = 0.0f;
-    if (p.residual) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.residual) + row * p.sr, ln, D, r);
+    if (p.residual) row_load<T, V, NT, EPT>(row_at<T>(p.residual, p.sr, row, p.inner), ln, D, r);
     float g[EPT];
-    if (p.gate) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.gate) + row * p.sg, ln, D, g);
+    if (p.gate) row_load<T, V, NT, EPT>(row_at<T>(p.gate, p.sg, row, p.inner), ln, D, g);
     par_load<V, NT, EPT>(p.post_w, ln, D, 1.0f, w);
     par_load<V, NT, EPT>(p.scale, ln, D, 1.0f, s);
     par_load<V, NT, EPT>(p.pre_w, ln, D, 0.0f, v);
@@ -175,13 +181,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(cons
         const bool ok = row0 < p.rows;
         const long row = ok ? row0 : base;
         float y[EPT], r[EPT], g[EPT], dn[EPT], dr[EPT], a[EPT], da[EPT];
-        row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.y) + row * p.sy, ln, D, y);
+        row_load<T, V, NT, EPT>(row_at<T>(p.y, p.sy, row, p.inner), ln, D, y);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) { r[i] = dn[i] = dr[i] = 0.0f; a[i] = 1.0f; da[i] = 0.0f; }
-        if (p.residual) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.residual) + row * p.sr, ln, D, r);
-        if (p.gate) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.gate) + row * p.sg, ln, D, g);
-        if (p.dnormed) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.dnormed) + row * p.sdn, ln, D, dn);
-        if (p.dres) row_load<T, V, NT, EPT>(reinterpret_cast<const T *>(p.dres) + row * p.sdr, ln, D, dr);
+        if (p.residual) row_load<T, V, NT, EPT>(row_at<T>(p.residual, p.sr, row, p.inner), ln, D, r);
+        if (p.gate) row_load<T, V, NT, EPT>(row_at<T>(p.gate, p.sg, row, p.inner), ln, D, g);
+        if (p.dnormed) row_load<T, V, NT, EPT>(row_at<T>(p.dnormed, p.sdn, row, p.inner), ln, D, dn);
+        if (p.dres) row_load<T, V, NT, EPT>(row_at<T>(p.dres, p.sdr, row, p.inner), ln, D, dr);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) s1 = fmaf(y[i], y[i], s1);

@@ -200,7 +200,8 @@ int urnn_conv_seq_parts(int B, int L, int D);
 // ---- norms around a block ----------------------------------------------------------------------------------------------
 struct NormParams {
     const void *y, *gate, *residual, *dnormed, *dres; // (M,D) rows; gate, residual, dnormed, dres may be NULL
-    long sy, sg, sr, sdn, sdr;                       // row strides in elements
+    SeqStride sy, sg, sr, sdn, sdr;                  // row r is at (r / inner) b + (r % inner) t
+    unsigned inner;
     const float *pre_w, *post_w, *scale;             // (D); post_w / scale may be NULL
     void *normed, *res_out;                          // (M,D) contiguous
     void *dy, *dgate, *dresidual;                    // (M,D) contiguous; dgate / dresidual may be NULL

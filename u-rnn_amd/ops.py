@@ -710,10 +710,12 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
 
 
 def _rows(what, name, t, shape, dtype):
-    """(..., D) as rows of D adjacent channels a fixed stride apart: the row stride."""
+    """(..., D): strides of the rows, as (outer, inner) of a (B, L, D) tensor or (anything, row) of evenly spaced rows."""
     _seq_check(what, name, t, shape, dtype)
+    if len(shape) == 3:
+        return t.stride()[:2]
     stride, n = None, 1
-    for size, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for size, s in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
         if size == 1:
             continue
         if stride is None:
@@ -721,7 +723,7 @@ def _rows(what, name, t, shape, dtype):
         elif s != stride * n:
             raise RuntimeError(f"{what}: the rows of {name} are not evenly spaced (strides {t.stride()})")
         n *= size
-    return t.shape[-1] if stride is None else stride
+    return 0, shape[-1] if stride is None else stride
 
 
 def _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act):
@@ -734,8 +736,19 @@ def _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act):
     for name, t in (("pre_w", pre_w), ("post_w", post_w), ("scale", scale)):
         if t is not None:
             _seq_check(what, name, t, (D,), torch.float32, contiguous=True)
-    shape = tuple(y.shape)
-    return [_rows(what, name, t, shape, y.dtype) if t is not None else 0 for name, t in (("y", y), ("gate", gate), ("residual", residual))]
+    return _row_strides(what, y, (("y", y), ("gate", gate), ("residual", residual)))
+
+
+def _row_strides(what, y, named):
+    """[outer, inner] of every tensor, one after the other (zeros for None)."""
+    shape, out = tuple(y.shape), []
+    for name, t in named:
+        out += _rows(what, name, t, shape, y.dtype) if t is not None else (0, 0)
+    return out
+
+
+def _inner_rows(shape, rows):
+    return shape[1] if len(shape) == 3 else rows
 
 
 def norm_residual(y, pre_w, residual=None, post_w=None, gate=None, scale=None, gate_act="silu", eps=NORM_EPS, out=None, residual_out=None):
@@ -748,7 +761,7 @@ def norm_residual(y, pre_w, residual=None, post_w=None, gate=None, scale=None, g
     Parameters (D) float32.  Returns (normed, r'), both contiguous.  ``residual_out`` may be ``residual`` (in place)."""
     what = "norm_residual"
     dt = _seq_dtype(what, y)
-    sy, sg, sr = _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act)
+    strides = _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act)
     shape, inputs = tuple(y.shape), (y, residual, gate)
     if out is not None:
         _seq_out(what, "out", out, shape, y.dtype, inputs + (residual_out,), same=inputs)
@@ -760,6 +773,8 @@ def norm_residual(y, pre_w, residual=None, post_w=None, gate=None, scale=None, g
     if residual_out is None:
         residual_out = torch.empty(shape, dtype=y.dtype, device=y.device)
     D = shape[-1]
-    check(lib().urnn_norm_residual(_ptr(y), _ptr(gate), _ptr(residual), (ctypes.c_long * 3)(sy, sg, sr), _ptr(pre_w), _ptr(post_w), _ptr(scale),
-                                   _ptr(out), _ptr(residual_out), dt, y.numel() // D, D, GATE_ACTS[gate_act], float(eps), stream), "urnn_norm_residual")
+    rows = y.numel() // D
+    check(lib().urnn_norm_residual(_ptr(y), _ptr(gate), _ptr(residual), (ctypes.c_long * 6)(*strides), _ptr(pre_w), _ptr(post_w), _ptr(scale),
+                                   _ptr(out), _ptr(residual_out), dt, rows, _inner_rows(shape, rows), D, GATE_ACTS[gate_act], float(eps), stream),
+          "urnn_norm_residual")
     return out, residual_out

@@ -254,7 +254,7 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
     dt = ops._seq_dtype(what, y)
     strides = ops._norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act)
     shape, D = tuple(y.shape), y.shape[-1]
-    strides += [ops._rows(what, name, t, shape, y.dtype) if t is not None else 0 for name, t in (("dnormed", dnormed), ("dresidual_out", dresidual_out))]
+    strides += ops._row_strides(what, y, (("dnormed", dnormed), ("dresidual_out", dresidual_out)))
     params = {"dpre_w": pre_w, "dpost_w": post_w, "dscale": scale}
     shapes = {k: (D,) for k, w in params.items() if w is not None}
     g, given = _param_grads_check(what, grads, accumulate, shapes)
@@ -269,8 +269,8 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
     out = [p(g[k]) if w is not None else 0 for k, w in params.items()]
     for k in params:
         g.setdefault(k, None)
-    check(L_.urnn_norm_residual_backward(p(y), p(gate), p(residual), p(dnormed), p(dresidual_out), (ctypes.c_long * 5)(*strides), p(pre_w), p(post_w),
-                                         p(scale), p(g["dy"]), p(g["dgate"]), p(g["dresidual"]), *out, p(ws), ws.numel(), dt, rows, D,
+    check(L_.urnn_norm_residual_backward(p(y), p(gate), p(residual), p(dnormed), p(dresidual_out), (ctypes.c_long * 10)(*strides), p(pre_w), p(post_w),
+                                         p(scale), p(g["dy"]), p(g["dgate"]), p(g["dresidual"]), *out, p(ws), ws.numel(), dt, rows, ops._inner_rows(shape, rows), D,
                                          ops.GATE_ACTS[gate_act], float(eps), int(bool(accumulate)), stream), "urnn_norm_residual_backward")
     return g
 
