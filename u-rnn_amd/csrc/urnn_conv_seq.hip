@@ -21,7 +21,7 @@ __device__ __forceinline__ void store_v(T *dst, const float (&v)[V])
     Pack<T, V> t;
 #pragma unroll
     for (int i = 0; i < V; ++i) t.v[i] = from_f<T>(v[i]);
-    *reinterpret_cast<Pack<T, V> *>(dst) = t;
+    stream_store(dst, t);
 }
 
 // The taps of V channels: w[k] belongs to line[t + k].  The weights of V adjacent channels are V K adjacent floats.

@@ -80,7 +80,7 @@ __device__ __forceinline__ void row_store(T *row, int ln, int D, const float (&v
         Pack<T, V> t;
 #pragma unroll
         for (int i = 0; i < V; ++i) t.v[i] = from_f<T>(v[c * V + i]);
-        if (d < D) *reinterpret_cast<Pack<T, V> *>(row + d) = t;
+        if (d < D) stream_store(row + d, t);
     }
 }
 // A parameter (fp32): in groups of at most four

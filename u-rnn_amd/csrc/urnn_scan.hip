@@ -21,26 +21,34 @@
 #include "urnn_seq.h"
 
 #include <type_traits>
+#include <utility>
 
 // h[k] = (decayed h[k]) + outer product of x (one per lane) with the row's values 4 k .. 4 k + 3: v_mfma_f32_4x4x1, sixteen blocks of four
-// states by four lanes.  The rows of four tokens lie across the lanes of v, NP values after one another; the instruction broadcasts
+// states by four lanes.  The rows of the tokens lie across the lanes of v, NP values after one another; the instruction broadcasts
 // four of them, of token J, to all blocks.
-template <int J, int K, int NP>
-__device__ __forceinline__ void add_outer(const float (&v)[NP < 16 ? 1 : NP / 16], float x, f32x4 (&h)[NP / 4])
+template <int J, int K, int NP, int RV>
+__device__ __forceinline__ void add_outer(const float (&v)[RV], float x, f32x4 (&h)[NP / 4])
 {
     if constexpr (K < NP / 4) {
         constexpr int at = J * NP + 4 * K;
         h[K] = __builtin_amdgcn_mfma_f32_4x4x1f32(v[at / 64], x, h[K], 4, at % 64 / 4, 0);
-        add_outer<J, K + 1, NP>(v, x, h);
+        add_outer<J, K + 1, NP, RV>(v, x, h);
     }
+}
+
+// f(0), f(1), ... f(G - 1), the first `left` of them (left >= G: without a test)
+template <bool ALL, typename F, int... I>
+__device__ __forceinline__ void tokens(F &f, int left, std::integer_sequence<int, I...>)
+{
+    ((ALL || I < left ? f(std::integral_constant<int, I>()) : void()), ...);
 }
 
 template <typename T, int NP, int MODE>
 __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
 {
-    constexpr int CK = urnn_scan_ck(NP), CB = URNN_SCAN_CB, G4 = 4, RV = NP < 16 ? 1 : NP / 16, TPV = NP < 16 ? 4 : 64 / NP;
+    constexpr int CK = urnn_scan_ck(NP), CB = URNN_SCAN_CB, GT = NP <= 16 ? 8 : 4, RV = GT * NP < 64 ? 1 : GT * NP / 64, TPV = 64 / NP;
     constexpr bool FULL = MODE == SCAN_FULL, BACK = MODE == SCAN_BACK;
-    __shared__ alignas(16) float s_C[FULL ? G4 * NP : 4];
+    __shared__ alignas(16) float s_C[FULL ? GT * NP : 4];
     const int lane = threadIdx.x;
     const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
@@ -53,11 +61,11 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
     // Lanes beyond the group repeat its block's first channel, bit for bit: what they store is what that lane stores.
     const int ch = c0 + lane < cend ? c0 + lane : c0;
     // Every stream is a uniform running pointer, to the next token to fetch, and the lane's byte offset in a row.  The rows of B and C of
-    // four tokens come as RV values to a lane: value lane + 64 r is state (lane + 64 r) % NP of token (lane + 64 r) / NP.
+    // GT tokens come as RV values to a lane: value lane + 64 r is state (lane + 64 r) % NP of token (lane + 64 r) / NP.
     const bool gated = MODE != SCAN_STATES && p.z != nullptr;
     const unsigned chb = ch * (unsigned)sizeof(T);
     const int rn = lane % NP, rt = lane / NP;
-    const bool okr = rn < p.N && rt < G4;
+    const bool okr = rn < p.N && rt < GT;
     const long ut = (BACK ? -p.so.t : p.su.t) * (long)sizeof(T), dt = dir * p.sd.t * (long)sizeof(T), zt = gated ? dir * p.sz.t * (long)sizeof(T) : dt;
     const long Bt = p.sB.t * (long)sizeof(T), Ct = dir * p.sC.t * (long)sizeof(T), yt = (long)p.dim * sizeof(T);
     const char *pu = reinterpret_cast<const char *>(BACK ? p.dout : p.u) + (BACK ? b * p.so.b + first * p.so.t : b * p.su.b + first * p.su.t) * (long)sizeof(T);
@@ -81,18 +89,18 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
     float total = 0.0f;                                          // summaries: the chunk's sum of steps
 
     const long offr = (okr ? rn : 0) * (long)sizeof(T), offB = (okr ? rt : 0) * Bt + offr, offC = (okr ? rt : 0) * Ct + offr;
-    T fu[G4], fd[G4], fz[G4], fB[RV], fC[RV];
-    auto fetch_tokens = [&](int left) {                          // the next min(G4, left) tokens; the last again where there are fewer
-        if (left >= G4) {
+    T fu[GT], fd[GT], fz[GT], fB[RV], fC[RV];
+    auto fetch_tokens = [&](int left) {                          // the next min(GT, left) tokens; the last again where there are fewer
+        if (left >= GT) {
 #pragma unroll
             for (int r = 0; r < RV; ++r) {
                 if (!BACK) fB[r] = *reinterpret_cast<const T *>(pB + r * TPV * Bt + offB);
                 if (MODE != SCAN_STATES) fC[r] = *reinterpret_cast<const T *>(pC + r * TPV * Ct + offC);
             }
-            pB += G4 * Bt;
-            pC += G4 * Ct;
+            pB += GT * Bt;
+            pC += GT * Ct;
 #pragma unroll
-            for (int j = 0; j < G4; ++j) {
+            for (int j = 0; j < GT; ++j) {
                 fu[j] = *reinterpret_cast<const T *>(pu + chb);
                 fd[j] = *reinterpret_cast<const T *>(pd + chb);
                 if (MODE != SCAN_STATES) fz[j] = *reinterpret_cast<const T *>(pz + chb);
@@ -108,7 +116,7 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
                 if (MODE != SCAN_STATES) fC[r] = *reinterpret_cast<const T *>(pC + k * Ct + offr);
             }
 #pragma unroll
-            for (int j = 0; j < G4; ++j) {
+            for (int j = 0; j < GT; ++j) {
                 const long k = j < left ? j : left - 1;
                 fu[j] = *reinterpret_cast<const T *>(pu + k * ut + chb);
                 fd[j] = *reinterpret_cast<const T *>(pd + k * dt + chb);
@@ -117,16 +125,16 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
         }
     };
     if (n > 0) fetch_tokens(n);
-    for (int i = 0; i < n; i += G4) {
-        float st[G4], in[G4], gate[G4], uf[G4], row[RV];         // row: B's; BACK: C's
+    for (int i = 0; i < n; i += GT) {
+        float st[GT], in[GT], gate[GT], uf[GT], row[RV];         // row: B's; BACK: C's
 #pragma unroll
         for (int r = 0; r < RV; ++r) {
             row[r] = okr ? to_f(BACK ? fC[r] : fB[r]) : 0.0f;
-            if (FULL && rt < G4) s_C[lane + 64 * r] = okr ? to_f(fC[r]) : 0.0f;
+            if (FULL && rt < GT) s_C[lane + 64 * r] = okr ? to_f(fC[r]) : 0.0f;
         }
         if (FULL) __syncthreads();                               // one wave: orders the rows' writes before their reads
 #pragma unroll
-        for (int j = 0; j < G4; ++j) {
+        for (int j = 0; j < GT; ++j) {
             const float raw = to_f(fd[j]) + bias, s = softplus_f(raw);
             st[j] = sp ? s : raw;
             uf[j] = to_f(fu[j]);
@@ -134,20 +142,21 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
             gate[j] = gated ? sl : 1.0f;
             in[j] = uf[j] * (BACK ? gate[j] : st[j]);            // step u, or d
         }
-        if (i + G4 < n) fetch_tokens(n - (i + G4));
-        if (FULL && p.keep && i % CK == 0) {                     // the state before token tb + i
+        if (i + GT < n) fetch_tokens(n - (i + GT));
+        auto checkpoint = [&](int j) {                           // the state before token tb + i + j
             const int blk = 16 * urnn_scan_ed(NP), cl = ch - g * Dg, cbeg = cl / blk * blk, w = Dg - cbeg < blk ? Dg - cbeg : blk;
-            const long seg = (tb + i) / CK, segs = (p.L + CK - 1) / CK;
+            const long seg = (tb + i + j) / CK, segs = (p.L + CK - 1) / CK;
             f32x4 *k = reinterpret_cast<f32x4 *>(p.keep + (((long)b * segs + seg) * p.dim + g * Dg + cbeg + keep_rank(cl - cbeg, w, urnn_scan_v(NP))) * NP);
 #pragma unroll
             for (int e = 0; e < NP / 4; ++e) k[e] = h[e];
-        }
+        };
         auto token = [&](auto jc) {
             constexpr int j = decltype(jc)::value;
-            if (BACK) add_outer<j, 0, NP>(row, in[j], h);        // h <- a (h + C d), otherwise h <- a h + B (step u)
+            if (FULL && j % (CK < GT ? CK : GT) == 0 && (i + j) % CK == 0 && p.keep) checkpoint(j);
+            if (BACK) add_outer<j, 0, NP, RV>(row, in[j], h);        // h <- a (h + C d), otherwise h <- a h + B (step u)
 #pragma unroll
             for (int k = 0; k < NP; ++k) h[k / 4][k % 4] *= __builtin_amdgcn_exp2f(st[j] * A2[k]);
-            if (!BACK) add_outer<j, 0, NP>(row, in[j], h);
+            if (!BACK) add_outer<j, 0, NP, RV>(row, in[j], h);
             if (FULL) {
                 float y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
@@ -165,16 +174,8 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
                 total += st[j];
             }
         };
-        if (i + G4 <= n) {
-            token(std::integral_constant<int, 0>());
-            token(std::integral_constant<int, 1>());
-            token(std::integral_constant<int, 2>());
-            token(std::integral_constant<int, 3>());
-        } else {
-            token(std::integral_constant<int, 0>());
-            if (i + 1 < n) token(std::integral_constant<int, 1>());
-            if (i + 2 < n) token(std::integral_constant<int, 2>());
-        }
+        if (i + GT <= n) tokens<true>(token, GT, std::make_integer_sequence<int, GT>());
+        else tokens<false>(token, n - i, std::make_integer_sequence<int, GT>());
     }
 #pragma unroll
     for (int k = 0; k < NP; ++k) h0[k] = h[k / 4][k % 4];
@@ -221,11 +222,15 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
     }
 }
 
+// Chunks of the time axis: one from 640 waves on, where the pass over the chunks' ends would cost more than the waves it wins;
+// below that as many as give 6144 waves (three turns of two waves on each of the 1024 SIMDs), but none shorter than 32 tokens.
+// Measured with 3000 waves of 64 tokens at least and with 6144 of 32: 32 768 tokens of 2048 channels 483 and 468 us, seven
+// sequences of up to 1021 tokens of 1000 channels 72 and 67 us, forward and backward of 4 x 2048 x 2048 491 and 492 us.
 int urnn_scan_chunks(int B, int L, int D, int *CL)
 {
     const long waves = (long)B * ((D + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
-    long want = waves >= 640 ? 1 : (3000 + waves - 1) / waves;
-    const long most = (L + 63) / 64;
+    long want = waves >= 640 ? 1 : (6144 + waves - 1) / waves;
+    const long most = (L + 31) / 32;
     if (want > most) want = most;
     if (want < 1) want = 1;
     long cl = (L + want - 1) / want;
@@ -311,7 +316,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const ScanParams p)
         }
         y = fmaf(skip, u[r], quad_sum(y));
         if (p.z) y *= silu_f(zf[r]);
-        store_states<E>(p.state_out + (b * p.dim + d) * p.N, q, p.N, vo, h[r]);
+        store_states<E, true>(p.state_out + (b * p.dim + d) * p.N, q, p.N, vo, h[r]);
         if (q == 0) reinterpret_cast<T *>(p.y)[b * p.dim + d] = from_f<T>(y);
     }
 }
