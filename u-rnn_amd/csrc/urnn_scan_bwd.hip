@@ -472,6 +472,7 @@ __global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(con
                 if (w >= NP) sum = fmaf(rowB[t * NP + n], ds, sum);
                 if (n < p.N) put_bc(w / NP, t0 + t, n, sum);
             }
+            wave_fence();                                        // the wave's rows are read: the next segment's may be written
         }
         const float none[V] = {};
         for (long t = te; t < tfull; t += CK) {                  // rows behind the sequence are zeros
