@@ -498,6 +498,43 @@ def test_refusals_norm_residual():
     refused("accumulate needs", train_ops.norm_residual_backward, dnormed=c["y"], accumulate=True, **c)
 
 
+def test_refusals_of_buffers():
+    """Workspaces, records and gradient buffers: plain bytes of their own, no buffer for two things at once."""
+    c, _ = scan_case(2, 5, 8, 4, 2, torch.float32, 0, dev="cpu")
+    back = {k: v for k, v in c.items() if k != "state"}
+    ws = torch.zeros(1 << 16, dtype=torch.uint8)
+    refused("contiguous uint8", ops.selective_scan, **c, ws=ops.Arena("cpu"))            # the next call would get the same record
+    refused("contiguous uint8", ops.selective_scan, **c, ws=ws[::2])
+    refused("contiguous uint8", ops.selective_scan, **c, ws=torch.zeros(1, dtype=torch.uint8).expand(1 << 16))
+    refused("contiguous uint8", ops.selective_scan, **c, ws=torch.zeros(1 << 16))
+    refused("of 64 bytes given", ops.selective_scan, **c, ws=ws[:64])
+    both = torch.zeros(1 << 16, dtype=torch.uint8)
+    refused("ws overlaps", ops.selective_scan, **c, ws=both, out=both[:2 * 5 * 8 * 4].view(torch.float32).view(2, 5, 8))
+    refused("contiguous uint8", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ops.Arena("cpu"))
+    refused("fwd_ws of 64 bytes", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws[:64])
+    refused("expected .batch, L, dim. and .dim, N.", ops.selective_scan_workspace, c["u"][0], c["A"])
+    d = torch.zeros(8)
+    refused("overlaps", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, grads={"dD": d, "ddelta_bias": d.view(8)})
+    refused("one buffer", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, grads={"dD": d, "ddelta_bias": d})
+    refused("dA overlaps", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, grads={"dA": c["A"]})
+    x, w, b = torch.zeros(2, 5, 8), torch.zeros(8, 4), torch.zeros(8)
+    refused("dbias overlaps", train_ops.causal_conv_backward, x, w, x, bias=b, grads={"dbias": b})
+    y, v = torch.zeros(3, 8), torch.zeros(8)
+    refused("one buffer", train_ops.norm_residual_backward, y, v, y, post_w=v, grads={"dpre_w": d, "dpost_w": d})
+
+
+def test_c_entries_refuse_what_no_launch_holds():
+    from urnn_amd._lib import lib
+    L = lib()
+    strides = (__import__("ctypes").c_long * 12)()
+    assert L.urnn_causal_conv_backward(16, 0, 0, 16, 0, 0, 0, 32, 0, 0, 0, 64, 0, 16, 0, 16, 1 << 40, 0, 1, 1, 1 << 24, 4, 1, 0, 0) == -1
+    assert b"one launch" in L.urnn_last_error()
+    big = (16, 16, 16, 16, 0, 16, strides, 16, 0, 0, 0, 0, 16, 1 << 60, 16, 16, 16, 16, 0, 16, 0, 0, 0, 16, 1 << 60, 0)
+    assert L.urnn_selective_scan_backward(*big, 1, 1, 1 << 21, 1, 64, 1, 0, 0) == -1 and b"one launch" in L.urnn_last_error()
+    assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 32, 0, 0, 4194304, 4194304, 4097, 0, 1e-5, 0) == -1 and b"one launch" in L.urnn_last_error()
+    assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 32, 0, 0, 8388608, 8388608, 2049, 0, 1e-5, 0) == -1 and b"one launch" in L.urnn_last_error()
+
+
 def test_c_entries_refuse_without_a_gpu():
     """Argument errors come before any HIP call, as codes with a message."""
     from urnn_amd._lib import lib
@@ -653,7 +690,7 @@ def test_calls_are_bit_reproducible_on_any_stream_and_in_graphs():
     def work(ar=None):
         y = ops.causal_conv(cc["x"], cc["weight"], bias=cc["bias"], state=cc["state"])
         gc = train_ops.causal_conv_backward(cc["x"], cc["weight"], dout, bias=cc["bias"], state=cc["state"], scratch=ar)
-        ws = ar if ar is not None else ops.selective_scan_workspace(c["u"], c["A"])
+        ws = ops.selective_scan_workspace(c["u"], c["A"])
         s = ops.selective_scan(**c, lengths=n, ws=ws)
         gs = train_ops.selective_scan_backward(**back, dout=dout, fwd_ws=ws, lengths=n, scratch=ar)
         m, r = ops.norm_residual(**nc)

@@ -1536,6 +1536,9 @@ static inline bool wide_rows(const void *base, long s1, long s2, int elem)
     return !base || (aligned16(base) && s1 * elem % 16 == 0 && s2 * elem % 16 == 0);
 }
 
+// A launch has fewer than 2^32 threads: the sum over the parts takes 64 for a value.
+static const double SUM_VALUES = 67108848.0;
+
 static int conv_seq_args(const char *what, const void *x, const void *weight, int dtype, long B, long L, long D, int K)
 {
     if (!x || !weight) return fail(URNN_ENULL, "%s: NULL argument", what);
@@ -1597,6 +1600,7 @@ extern "C" int urnn_causal_conv_backward(const void *x, long x_batch, long x_tok
     if (!dout || !dx || !dweight || !workspace) return fail(URNN_ENULL, "urnn_causal_conv_backward: NULL argument");
     if (dx == dout || dx == x) return fail(URNN_EINVAL, "urnn_causal_conv_backward: dx must be a buffer of its own");
     if (!aligned16(workspace)) return fail(URNN_EALIGN, "urnn_causal_conv_backward: workspace not 16-byte aligned");
+    if ((double)D * (K + 1) > SUM_VALUES) return fail(URNN_EINVAL, "urnn_causal_conv_backward: D=%d is beyond one launch", D);
     if (workspace_bytes < urnn_causal_conv_backward_workspace_bytes(B, L, D, K)) return fail(URNN_EWORKSPACE, "urnn_causal_conv_backward: workspace too small");
     ConvSeqParams p = {};
     p.x = x; p.sx = {x_batch, x_token};
@@ -1710,6 +1714,8 @@ extern "C" int urnn_selective_scan_backward(const void *u, const void *delta, co
     for (int k = 1; L > 1 && k < 12; k += 2)                     // the kernel's offsets within a segment of eight tokens are of 32 bits
         if (strides[k] < 0 || (k != 9 || z ? ((double)strides[k] * 7 + D + 64) * seq_elem(dtype) : 0.0) >= 4294967296.0)
             return fail(URNN_EINVAL, "urnn_selective_scan_backward: a token stride of %ld elements is beyond 4 GB in eight tokens", strides[k]);
+    if ((double)D * (N + 2) > SUM_VALUES || (double)B * L * G * N > 4294967040.0)
+        return fail(URNN_EINVAL, "urnn_selective_scan_backward: B=%d L=%d D=%d G=%d N=%d is beyond one launch", B, L, D, G, N);
     const ScanBackWork w = scan_back_work(B, L, D, G, N);
     if (workspace_bytes < w.total) return fail(URNN_EWORKSPACE, "urnn_selective_scan_backward: workspace too small");
     char *base = reinterpret_cast<char *>(workspace);
@@ -1753,6 +1759,7 @@ static int norm_args(const char *what, const void *y, const long *strides, const
     if (!y || !strides || !pre_w) return fail(URNN_ENULL, "%s: NULL argument", what);
     if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
     if (rows < 1 || rows > 8388608 || D < 1 || D > URNN_SEQ_MAX_NORM) return fail(URNN_EINVAL, "%s: rows=%ld (1..8388608) D=%d (1..%d)", what, rows, D, URNN_SEQ_MAX_NORM);
+    if ((D > 4096 && rows > 4194303) || (D > 2048 && rows > 8388607)) return fail(URNN_EINVAL, "%s: rows=%ld of D=%d are beyond one launch", what, rows, D);
     if (inner < 1 || inner > rows || rows % inner) return fail(URNN_EINVAL, "%s: %ld rows of %ld each", what, rows, inner);
     if (act < URNN_GATE_NONE || act > URNN_GATE_SILU) return fail(URNN_EINVAL, "%s: act=%d", what, act);
     return URNN_OK;

@@ -516,6 +516,8 @@ def _empty_as(t):
 
 
 def _span(t):
+    if t.is_contiguous():
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
     return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
 
@@ -529,6 +531,25 @@ def _seq_out(what, name, t, shape, dtype, inputs, same=()):
         a, b = _span(x)
         if a < hi and lo < b and not any(x is s and a == lo and x.is_contiguous() for s in same):
             raise RuntimeError(f"{what}: {name} overlaps an input")
+
+
+def _seq_buffer(what, name, buf, nbytes, others):
+    """A workspace or record that the caller gives: nbytes of plain bytes, apart from every tensor of the call."""
+    if not isinstance(buf, torch.Tensor) or buf.dtype != torch.uint8 or not buf.is_contiguous():
+        raise RuntimeError(f"{what}: {name} is a contiguous uint8 tensor")
+    if buf.numel() < nbytes:
+        raise RuntimeError(f"{what}: {name} of {buf.numel()} bytes given, {nbytes} needed")
+    _apart(what, name, buf, others)
+    return buf
+
+
+def _apart(what, name, t, others):
+    lo, hi = _span(t)
+    for x in others:
+        if x is not None and x.numel():
+            a, b = _span(x)
+            if a < hi and lo < b:
+                raise RuntimeError(f"{what}: {name} overlaps another tensor of the call")
 
 
 def _lengths_check(what, lengths, B):
@@ -640,6 +661,8 @@ def _scan_check(what, u, delta, A, B, C, D, z, delta_bias, lead):
 
 def selective_scan_workspace(u, A):
     """The record that a training forward leaves for ``train_ops.selective_scan_backward``: a buffer for ``selective_scan(..., ws=)``."""
+    if u.dim() != 3 or A.dim() != 2:
+        raise RuntimeError(f"selective_scan_workspace: u {tuple(u.shape)} and A {tuple(A.shape)}, expected (batch, L, dim) and (dim, N)")
     B, L, dim = u.shape
     n = lib().urnn_selective_scan_workspace_bytes(B, L, dim, A.shape[1], 1)
     return torch.empty(int(n), dtype=torch.uint8, device=u.device)
@@ -653,7 +676,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     u, delta, z (batch,L,dim); A (dim,N), N = 1..64; B, C (batch,L,N) or (batch,L,G,N) with dim / G channels to a group; D, delta_bias
     (dim).  ``softplus`` False: step = delta + delta_bias.  ``state`` (batch,dim,N) float32: the state before the first token (None: zeros);
     ``lengths`` (batch) int32: tokens of each sequence of a padded batch -- later ones are not read and give zeros.  ``ws``: a buffer of
-    ``selective_scan_workspace(u, A)`` (or an Arena) that the backward will read: a training forward; None: scratch for this call.
+    ``selective_scan_workspace(u, A)`` that the backward will read: a training forward, with a buffer for every call whose backward is still
+    to come (an Arena, which hands out the same one again, is refused); None: scratch for this call.
     Returns y, or (y, state after each sequence's last token) with ``want_state``."""
     what = "selective_scan"
     dt = _seq_dtype(what, u)
@@ -669,14 +693,13 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
         _seq_out(what, "out", out, (nb, L, dim), u.dtype, inputs + (state_out,))
     if state_out is not None:
         _seq_out(what, "state_out", state_out, (nb, dim, N), torch.float32, inputs)
-    stream = _seq_device(what, *inputs, lengths, out, state_out)
     Lb = lib()
     keep = ws is not None
     nbytes = Lb.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1 if keep else 0)
     if keep:
-        ws = _scratch(ws, nbytes, u.device, key="scan")
-        _seq_device(what, u, ws)
-    elif nbytes:
+        _seq_buffer(what, "ws", ws, nbytes, inputs + (lengths, out, state_out))
+    stream = _seq_device(what, *inputs, lengths, out, state_out, ws)
+    if nbytes and not keep:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=u.device)
     if out is None:
         out = torch.empty((nb, L, dim), dtype=u.dtype, device=u.device)

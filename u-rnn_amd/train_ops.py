@@ -190,8 +190,8 @@ def adam_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.9
 
 
 # ---- sequence operators (ops.causal_conv, ops.selective_scan, ops.norm_residual) --------------------------------------------
-def _param_grads_check(what, grads, accumulate, shapes):
-    """-> (the dict that receives the gradients, the buffers in it that the caller gave)."""
+def _param_grads_check(what, grads, accumulate, shapes, inputs):
+    """-> (the dict that receives the gradients, the buffers in it that the caller gave: apart from the inputs and from one another)."""
     g = {} if grads is None else grads
     if accumulate and any(g.get(k) is None for k in shapes):
         raise RuntimeError(f"{what}: accumulate needs the gradients {sorted(shapes)} in grads")
@@ -199,6 +199,9 @@ def _param_grads_check(what, grads, accumulate, shapes):
     for k, shape in shapes.items():
         if g.get(k) is not None:
             ops._seq_check(what, k, g[k], shape, torch.float32, contiguous=True)
+            ops._apart(what, k, g[k], (*inputs, *(t for t in given if t is not g[k])))
+    if len({t.data_ptr() for t in given}) < len(given):
+        raise RuntimeError(f"{what}: one buffer for several of the gradients {sorted(shapes)}")
     return g, given
 
 
@@ -226,14 +229,15 @@ def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, s
     if dstate_out is not None:
         ops._seq_check(what, "dstate_out", dstate_out, (B, K - 1, D), x.dtype, contiguous=True)
     shapes = {"dweight": (D, K), **({"dbias": (D,)} if bias is not None else {})}
-    g, given = _param_grads_check(what, grads, accumulate, shapes)
-    stream = ops._seq_device(what, x, weight, dout, bias, state, lengths, dstate_out, *given)
+    inputs = (x, weight, dout, bias, state, lengths, dstate_out)
+    g, given = _param_grads_check(what, grads, accumulate, shapes, inputs)
+    stream = ops._seq_device(what, *inputs, *given)
     L_ = lib()
     _param_grads(g, shapes, x.device)
     g.setdefault("dbias", None)
     g["dx"] = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
     g["dstate"] = torch.empty_like(state) if state is not None else None
-    ws = _seq_scratch(scratch, L_.urnn_causal_conv_backward_workspace_bytes(B, L, D, K), x.device)
+    ws = _seq_scratch(what, scratch, L_.urnn_causal_conv_backward_workspace_bytes(B, L, D, K), x.device, (*inputs, *given))
     p = ops._ptr
     check(L_.urnn_causal_conv_backward(p(x), *x.stride()[:2], p(weight), p(bias), p(state), p(lengths), p(dout), *dout.stride()[:2], p(dstate_out),
                                        p(g["dx"]), p(g["dstate"]), p(g["dweight"]), p(g["dbias"]), p(ws), ws.numel(), dt, B, L, D, K,
@@ -241,9 +245,15 @@ def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, s
     return g
 
 
-def _seq_scratch(scratch, nbytes, dev):
+def _seq_scratch(what, scratch, nbytes, dev, others):
     """Scratch of a sequence operator's backward (no status words: nothing in it needs to start at zero)."""
-    return torch.empty(int(nbytes), dtype=torch.uint8, device=dev) if scratch is None else _bwd_scratch(scratch, nbytes, dev)
+    if scratch is None:
+        return torch.empty(int(nbytes), dtype=torch.uint8, device=dev)
+    if isinstance(scratch, ops.Arena):
+        return _bwd_scratch(scratch, nbytes, dev)
+    ops._seq_buffer(what, "scratch", scratch, nbytes, others)
+    ops._seq_device(what, others[0], scratch)
+    return scratch
 
 
 def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None, post_w=None, gate=None, scale=None, gate_act="silu",
@@ -257,14 +267,15 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
     strides += ops._row_strides(what, y, (("dnormed", dnormed), ("dresidual_out", dresidual_out)))
     params = {"dpre_w": pre_w, "dpost_w": post_w, "dscale": scale}
     shapes = {k: (D,) for k, w in params.items() if w is not None}
-    g, given = _param_grads_check(what, grads, accumulate, shapes)
-    stream = ops._seq_device(what, y, pre_w, dnormed, dresidual_out, residual, post_w, gate, scale, *given)
+    inputs = (y, pre_w, dnormed, dresidual_out, residual, post_w, gate, scale)
+    g, given = _param_grads_check(what, grads, accumulate, shapes, inputs)
+    stream = ops._seq_device(what, *inputs, *given)
     L_ = lib()
     _param_grads(g, shapes, y.device)
     new = lambda: torch.empty(shape, dtype=y.dtype, device=y.device)      # noqa: E731
     g["dy"], g["dgate"], g["dresidual"] = new(), new() if gate is not None else None, new() if residual is not None else None
     rows = y.numel() // D
-    ws = _seq_scratch(scratch, L_.urnn_norm_residual_backward_workspace_bytes(rows, D), y.device)
+    ws = _seq_scratch(what, scratch, L_.urnn_norm_residual_backward_workspace_bytes(rows, D), y.device, (*inputs, *given))
     p = ops._ptr
     out = [p(g[k]) if w is not None else 0 for k, w in params.items()]
     for k in params:
@@ -278,8 +289,8 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
 def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, delta_bias=None, softplus=True, lengths=None, dstate_out=None,
                             want_dstate=False, grads=None, accumulate=False, scratch=None):
     """Backward of ``ops.selective_scan`` given dout (batch,L,dim) and, where the returned state was used further, ``dstate_out``
-    (batch,dim,N).  ``fwd_ws``: the buffer that the forward of the SAME inputs ran with (``ws=``, untouched since; an Arena hands out the
-    forward's): it holds the states the gradients need, the initial one among them.  Returns a dict: du, ddelta, dB, dC, dz in the
+    (batch,dim,N).  ``fwd_ws``: the buffer that the forward of the SAME inputs ran with (``ws=``, untouched since): it holds the
+    states the gradients need, the initial one among them.  Returns a dict: du, ddelta, dB, dC, dz in the
     activations' type and B's shape, dA, dD, ddelta_bias float32 (into the buffers of ``grads`` if given, added to them with ``accumulate``),
     dstate float32 with ``want_dstate``; None where there is no such input."""
     what = "selective_scan_backward"
@@ -300,11 +311,11 @@ def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, del
         shapes["dD"] = (dim,)
     if delta_bias is not None:
         shapes["ddelta_bias"] = (dim,)
-    g, given = _param_grads_check(what, grads, accumulate, shapes)
-    stream = ops._seq_device(what, u, delta, A, B, C, D, z, delta_bias, dout, lengths, dstate_out, *given)
+    inputs = (u, delta, A, B, C, D, z, delta_bias, dout, lengths, dstate_out)
+    g, given = _param_grads_check(what, grads, accumulate, shapes, inputs)
     L_ = lib()
-    record = ops._scratch(fwd_ws, L_.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1), u.device, key="scan")
-    ops._seq_device(what, u, record)
+    record = ops._seq_buffer(what, "fwd_ws", fwd_ws, L_.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1), given)
+    stream = ops._seq_device(what, *inputs, *given, record)
     _param_grads(g, shapes, u.device)
     g.setdefault("dD", None)
     g.setdefault("ddelta_bias", None)
@@ -312,7 +323,7 @@ def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, del
     g["du"], g["ddelta"], g["dB"], g["dC"] = new(u.shape), new(u.shape), new(b_shape), new(c_shape)
     g["dz"] = new(u.shape) if z is not None else None
     g["dstate"] = torch.empty((nb, dim, N), dtype=torch.float32, device=u.device) if want_dstate else None
-    ws = _seq_scratch(scratch, L_.urnn_selective_scan_backward_workspace_bytes(nb, L, dim, G, N), u.device)
+    ws = _seq_scratch(what, scratch, L_.urnn_selective_scan_backward_workspace_bytes(nb, L, dim, G, N), u.device, (*inputs, *given, record))
     p = ops._ptr
     strides = (ctypes.c_long * 12)(*u.stride()[:2], *delta.stride()[:2], *B.stride()[:2], *C.stride()[:2], *(z.stride()[:2] if z is not None else (0, 0)),
                                    *dout.stride()[:2])
