@@ -546,10 +546,11 @@ def _seq_buffer(what, name, buf, nbytes, others):
 def _apart(what, name, t, others):
     lo, hi = _span(t)
     for x in others:
-        if x is not None and x.numel():
-            a, b = _span(x)
-            if a < hi and lo < b:
-                raise RuntimeError(f"{what}: {name} overlaps another tensor of the call")
+        if x is None:
+            continue
+        a = x.data_ptr()
+        if a < hi and (a >= lo or _span(x)[1] > lo) and x.numel():
+            raise RuntimeError(f"{what}: {name} overlaps another tensor of the call")
 
 
 def _lengths_check(what, lengths, B):
@@ -597,7 +598,7 @@ def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, out=N
         _seq_out(what, "state_out", state_out, (B, K - 1, D), x.dtype, (x, weight, bias, state))
     stream = _seq_device(what, x, weight, bias, state, lengths, out, state_out)
     if out is None:
-        out = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
+        out = _empty_as(x)
     if want_state and state_out is None:
         state_out = torch.empty((B, K - 1, D), dtype=x.dtype, device=x.device)
     sb, st, _ = x.stride()
@@ -702,7 +703,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     if nbytes and not keep:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=u.device)
     if out is None:
-        out = torch.empty((nb, L, dim), dtype=u.dtype, device=u.device)
+        out = _empty_as(u)
     if want_state and state_out is None:
         state_out = torch.empty((nb, dim, N), dtype=torch.float32, device=u.device)
     strides = (ctypes.c_long * 10)(*u.stride()[:2], *delta.stride()[:2], *B.stride()[:2], *C.stride()[:2], *(z.stride()[:2] if z is not None else (0, 0)))
@@ -744,6 +745,8 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
 def _rows(what, name, t, shape, dtype):
     """(..., D): strides of the rows, as (outer, inner) of a (B, L, D) tensor or (anything, row) of evenly spaced rows."""
     _seq_check(what, name, t, shape, dtype)
+    if len(shape) == 2:
+        return 0, t.stride(0) if shape[0] > 1 else shape[1]
     if len(shape) == 3:
         return t.stride()[:2]
     stride, n = None, 1

@@ -190,26 +190,28 @@ def adam_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.9
 
 
 # ---- sequence operators (ops.causal_conv, ops.selective_scan, ops.norm_residual) --------------------------------------------
-def _param_grads_check(what, grads, accumulate, shapes, inputs):
+def _param_grads_check(what, grads, accumulate, params, inputs):
     """-> (the dict that receives the gradients, the buffers in it that the caller gave: apart from the inputs and from one another)."""
     g = {} if grads is None else grads
-    if accumulate and any(g.get(k) is None for k in shapes):
-        raise RuntimeError(f"{what}: accumulate needs the gradients {sorted(shapes)} in grads")
-    given = [g[k] for k in shapes if g.get(k) is not None]
-    for k, shape in shapes.items():
+    if accumulate and any(g.get(k) is None for k in params):
+        raise RuntimeError(f"{what}: accumulate needs the gradients {sorted(params)} in grads")
+    given = [g[k] for k in params if g.get(k) is not None]
+    if not given:
+        return g, given
+    for k, w in params.items():
         if g.get(k) is not None:
-            ops._seq_check(what, k, g[k], shape, torch.float32, contiguous=True)
+            ops._seq_check(what, k, g[k], tuple(w.shape), torch.float32, contiguous=True)
             ops._apart(what, k, g[k], (*inputs, *(t for t in given if t is not g[k])))
     if len({t.data_ptr() for t in given}) < len(given):
-        raise RuntimeError(f"{what}: one buffer for several of the gradients {sorted(shapes)}")
+        raise RuntimeError(f"{what}: one buffer for several of the gradients {sorted(params)}")
     return g, given
 
 
-def _param_grads(grads, shapes, dev):
+def _param_grads(grads, params):
     """Buffers of the parameters' gradients: those of a former call's dict or the caller's own views, and new ones."""
-    for k, shape in shapes.items():
+    for k, w in params.items():
         if grads.get(k) is None:
-            grads[k] = torch.empty(shape, dtype=torch.float32, device=dev)
+            grads[k] = torch.empty_like(w)
     return grads
 
 
@@ -228,14 +230,14 @@ def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, s
     ops._lengths_check(what, lengths, B)
     if dstate_out is not None:
         ops._seq_check(what, "dstate_out", dstate_out, (B, K - 1, D), x.dtype, contiguous=True)
-    shapes = {"dweight": (D, K), **({"dbias": (D,)} if bias is not None else {})}
+    params = {"dweight": weight, **({"dbias": bias} if bias is not None else {})}
     inputs = (x, weight, dout, bias, state, lengths, dstate_out)
-    g, given = _param_grads_check(what, grads, accumulate, shapes, inputs)
+    g, given = _param_grads_check(what, grads, accumulate, params, inputs)
     stream = ops._seq_device(what, *inputs, *given)
     L_ = lib()
-    _param_grads(g, shapes, x.device)
+    _param_grads(g, params)
     g.setdefault("dbias", None)
-    g["dx"] = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
+    g["dx"] = ops._empty_as(x)
     g["dstate"] = torch.empty_like(state) if state is not None else None
     ws = _seq_scratch(what, scratch, L_.urnn_causal_conv_backward_workspace_bytes(B, L, D, K), x.device, (*inputs, *given))
     p = ops._ptr
@@ -265,20 +267,20 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
     strides = ops._norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act)
     shape, D = tuple(y.shape), y.shape[-1]
     strides += ops._row_strides(what, y, (("dnormed", dnormed), ("dresidual_out", dresidual_out)))
-    params = {"dpre_w": pre_w, "dpost_w": post_w, "dscale": scale}
-    shapes = {k: (D,) for k, w in params.items() if w is not None}
+    every = {"dpre_w": pre_w, "dpost_w": post_w, "dscale": scale}
+    params = {k: w for k, w in every.items() if w is not None}
     inputs = (y, pre_w, dnormed, dresidual_out, residual, post_w, gate, scale)
-    g, given = _param_grads_check(what, grads, accumulate, shapes, inputs)
+    g, given = _param_grads_check(what, grads, accumulate, params, inputs)
     stream = ops._seq_device(what, *inputs, *given)
     L_ = lib()
-    _param_grads(g, shapes, y.device)
-    new = lambda: torch.empty(shape, dtype=y.dtype, device=y.device)      # noqa: E731
-    g["dy"], g["dgate"], g["dresidual"] = new(), new() if gate is not None else None, new() if residual is not None else None
+    _param_grads(g, params)
+    new = lambda t: None if t is None else ops._empty_as(t)      # noqa: E731
+    g["dy"], g["dgate"], g["dresidual"] = new(y), new(gate), new(residual)
     rows = y.numel() // D
     ws = _seq_scratch(what, scratch, L_.urnn_norm_residual_backward_workspace_bytes(rows, D), y.device, (*inputs, *given))
     p = ops._ptr
-    out = [p(g[k]) if w is not None else 0 for k, w in params.items()]
-    for k in params:
+    out = [p(g[k]) if w is not None else 0 for k, w in every.items()]
+    for k in every:
         g.setdefault(k, None)
     check(L_.urnn_norm_residual_backward(p(y), p(gate), p(residual), p(dnormed), p(dresidual_out), (ctypes.c_long * 10)(*strides), p(pre_w), p(post_w),
                                          p(scale), p(g["dy"]), p(g["dgate"]), p(g["dresidual"]), *out, p(ws), ws.numel(), dt, rows, ops._inner_rows(shape, rows), D,
@@ -298,7 +300,7 @@ def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, del
     if u.dim() != 3:
         raise RuntimeError(f"{what}: u has shape {tuple(u.shape)}, expected (batch, L, dim)")
     nb, L = u.shape[0], u.shape[1]
-    b_shape, c_shape = tuple(B.shape), tuple(C.shape)
+    B_given, C_given = B, C
     dim, G, N, B, C = ops._scan_check(what, u, delta, A, B, C, D, z, delta_bias, (nb, L))
     ops._seq_check(what, "dout", dout, (nb, L, dim), u.dtype)
     ops._lengths_check(what, lengths, nb)
@@ -306,22 +308,22 @@ def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, del
         ops._seq_check(what, "dstate_out", dstate_out, (nb, dim, N), torch.float32, contiguous=True)
     if fwd_ws is None:
         raise RuntimeError(f"{what}: fwd_ws is None: run the forward with ws=ops.selective_scan_workspace(u, A)")
-    shapes = {"dA": (dim, N)}
+    params = {"dA": A}
     if D is not None:
-        shapes["dD"] = (dim,)
+        params["dD"] = D
     if delta_bias is not None:
-        shapes["ddelta_bias"] = (dim,)
+        params["ddelta_bias"] = delta_bias
     inputs = (u, delta, A, B, C, D, z, delta_bias, dout, lengths, dstate_out)
-    g, given = _param_grads_check(what, grads, accumulate, shapes, inputs)
+    g, given = _param_grads_check(what, grads, accumulate, params, inputs)
     L_ = lib()
     record = ops._seq_buffer(what, "fwd_ws", fwd_ws, L_.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1), given)
     stream = ops._seq_device(what, *inputs, *given, record)
-    _param_grads(g, shapes, u.device)
+    _param_grads(g, params)
     g.setdefault("dD", None)
     g.setdefault("ddelta_bias", None)
-    new = lambda shape: torch.empty(shape, dtype=u.dtype, device=u.device)      # noqa: E731
-    g["du"], g["ddelta"], g["dB"], g["dC"] = new(u.shape), new(u.shape), new(b_shape), new(c_shape)
-    g["dz"] = new(u.shape) if z is not None else None
+    new = ops._empty_as
+    g["du"], g["ddelta"], g["dB"], g["dC"] = new(u), new(delta), new(B_given), new(C_given)
+    g["dz"] = new(z) if z is not None else None
     g["dstate"] = torch.empty((nb, dim, N), dtype=torch.float32, device=u.device) if want_dstate else None
     ws = _seq_scratch(what, scratch, L_.urnn_selective_scan_backward_workspace_bytes(nb, L, dim, G, N), u.device, (*inputs, *given, record))
     p = ops._ptr
