@@ -438,7 +438,8 @@ int urnn_step_f32(const urnn_net_f32 *net, const float *x_t, float *const states
  *     projection can be handed over in place; outputs are contiguous.
  * lengths (B) int32 or NULL: sequence b counts its first lengths[b] tokens (clamped to [0, L]); later tokens are not read, their
  * outputs and gradients are zeros.  Nothing is read or written outside the tensors whatever lengths hold.
- * No atomics: the same inputs give the same bits.  In-place: only where stated. */
+ * No atomics: the same inputs give the same bits.  In-place: only where stated.  Sizes that one launch does not hold (2^32 threads) are
+ * refused with URNN_EINVAL: rows of a norm beyond 2^22 to 2^23, B * D of a scan beyond 2^26. */
 #define URNN_F32 0
 #define URNN_BF16 1
 #define URNN_F16 2
@@ -498,9 +499,9 @@ int urnn_selective_scan_step(const void *u, const void *delta, const void *Bmat,
 int urnn_norm_residual(const void *y, const void *gate, const void *residual, const long *strides, const float *pre_w,
                        const float *post_w, const float *scale, void *normed, void *residual_out, int dtype, long rows, long inner, int D,
                        int act, float eps, void *stream);
-/* Gradients, given dnormed and dresidual_out (either may be NULL: zeros).  strides: of y, gate, residual, dnormed,
- * dresidual_out, as above.  dgate /
- * dresidual may be NULL; dpre_w, dpost_w, dscale (D) float32, each may be NULL, overwritten or added to (accumulate != 0). */
+/* Gradients, given dnormed and dresidual_out (either may be NULL: zeros).  strides: of y, gate, residual, dnormed, dresidual_out, as
+ * above.  dgate / dresidual may be NULL; dpre_w, dpost_w, dscale (D) float32, each may be NULL, overwritten or added to
+ * (accumulate != 0). */
 size_t urnn_norm_residual_backward_workspace_bytes(long rows, int D);
 int urnn_norm_residual_backward(const void *y, const void *gate, const void *residual, const void *dnormed, const void *dresidual_out,
                                 const long *strides, const float *pre_w, const float *post_w, const float *scale, void *dy, void *dgate,

@@ -327,6 +327,26 @@ def test_selective_scan_extremes():
     seq_ref.check(st, ref["state"], scan_k(c), torch.float32, "state")
 
 
+@gpu
+def test_selective_scan_growing_states_across_chunks():
+    """A > 0: the product of a chunk's factors overflows (e^(3 * 32)); states and gradients that are zero stay zero."""
+    c, _ = scan_case(1, 200, 20, 4, 1, torch.float32, 6, carried=False, softplus=False, bias=False)
+    c["A"] = torch.full_like(c["A"], 3.0)
+    c["delta"] = torch.ones_like(c["delta"])
+    c["u"][:, :197] = 0
+    dout = torch.zeros_like(c["u"])
+    dout[:, :2] = 1.0
+    ref = seq_ref.selective_scan(**c, dout=dout)
+    ws = ops.selective_scan_workspace(c["u"], c["A"])
+    y, st = ops.selective_scan(**c, ws=ws, want_state=True)
+    k = scan_k(c)
+    seq_ref.check(y, ref["y"], k, torch.float32, "y")
+    seq_ref.check(st, ref["state"], k, torch.float32, "state")
+    got = train_ops.selective_scan_backward(**{n: v for n, v in c.items() if n != "state"}, dout=dout, fwd_ws=ws)
+    for name in ("du", "ddelta", "dz", "dB", "dC", "dA", "dD"):
+        seq_ref.check(got[name], ref[name], 2 * k + 200, torch.float32, name)
+
+
 # ---- the norms around a block ----------------------------------------------------------------------------------------------------
 # k: a thread's chain of 16 squares and a tree over at most 1024 threads (10 + 16), rsqrt and its argument (4), gate (8) and products;
 # the backward's means pass through the forward's once more; column sums: the rows a block walks (at most 4 here) and the fold

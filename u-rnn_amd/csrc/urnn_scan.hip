@@ -6,18 +6,23 @@
 //
 // Mapping.  A lane is a channel: all of its states stay in registers along the sequence, the sum over states needs no other lane, and
 // the elementwise work (softplus, gate, conversions) is done once.  A wave is 64 adjacent channels of one sequence -- whole 128-byte
-// lines of a 16-bit row per access -- and a block of its own, so that nothing waits for another wave and LDS is not used.  A row of B
-// lies across the lanes, a state to a lane; the outer product with the lanes' inputs, B_t[n] (step u), is added to the decayed states by
-// v_mfma_f32_4x4x1 (fp32 as the vector unit's; four states of 64 channels in 8 cycles of the otherwise idle matrix pipe), which
-// broadcasts four values of the row; the sum with C takes the row's values by DPP row_newbcast inside the fma.  Inputs of the next four
-// tokens are in flight meanwhile.  What bounds it is the vector unit: per state one exponential (measured: the time of 1.6 to 2 fp32
-// operations) and three fp32 operations, per token and channel about 45 more.
+// lines of a 16-bit row per access -- and a block of its own, so that nothing waits for another wave.  The rows of B of a group of
+// tokens (GT: eight, four from 32 states on) lie across the lanes, a state to a lane; the outer product with the lanes' inputs,
+// B_t[n] (step u), is added to the decayed states by v_mfma_f32_4x4x1 (fp32 as the vector unit's; four states of 64 channels in 8 cycles
+// of the otherwise idle matrix pipe), which broadcasts four values of the row; C's rows are read from LDS, the same address in all lanes.
+// The inputs of the next group are in flight meanwhile.  (With a quad to a channel, as in the backward, all four lanes repeat the
+// elementwise part or pass it on through LDS: the full pass over 32 768 x 2048 took 417 us then and 359 with a lane, at that step.)
+//
+// What bounds it is the vector unit: per state one exponential (measured: the time of 1.6 to 2 fp32 operations) and three fp32
+// operations, per token and channel about 45 more: 119 issue slots at 16 states, 35e12 lane-slots/s of the chip.  4 x 2048 x 2048 bf16:
+// 93 us of 56 us of slots (waves at two to a SIMD wait for their loads and for the chain of a state from token to token), 1.5 TB/s;
+// 32 768 x 2048 468 us with both passes of 226 us of slots for one.
 //
 // Few long sequences do not fill the chip with B * D / 64 waves: the time axis is cut into chunks (urnn_scan_chunks).  The recurrence
 // is linear, h_end = P h_begin + S with S the state of a chunk that starts from zero and P = exp(A * sum of its steps): one pass
 // leaves (S, sum of steps) of every chunk, a short kernel carries the states over the chunks, and the full pass starts each chunk
-// from its true state.  The first pass costs the exponentials once more.  The same kernel, run from the last token to the first, gives
-// the backward its chunk summaries.
+// from its true state.  The first pass costs the exponentials once more (32 768 x 2048: 222 us next to the full pass's 286).  The same
+// kernel, run from the last token to the first, gives the backward its chunk summaries.
 #include "urnn_seq.h"
 
 #include <type_traits>
@@ -192,7 +197,8 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
 
 // S[c] (a chunk's end state from a zero start; chunk 0 from the given state) -> the end state itself:
 // H[c] = exp(A sum[c]) H[c - 1] + S[c].  One thread per (b, d, n); the loads do not depend on the chain.  A chunk without tokens
-// (sum 0) passes the state on as it is, also where A is infinite.
+// (sum 0) passes the state on as it is, also where A is infinite; a state of zero stays out of it, also where A is positive and the
+// product of a chunk's decays overflows.
 template <int NP>
 __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict__ A, const float *__restrict__ sum, float *S, int dim, int N, int chunks, long count)
 {
@@ -216,7 +222,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
 #pragma unroll
         for (int k = 0; k < U; ++k)
             if (c0 + k < chunks) {
-                h = wv[k] == 0.0f ? h + sv[k] : fmaf(__builtin_amdgcn_exp2f(wv[k] * A2), h, sv[k]);
+                h = wv[k] == 0.0f || h == 0.0f ? h + sv[k] : fmaf(__builtin_amdgcn_exp2f(wv[k] * A2), h, sv[k]);
                 s[(long)(c0 + k) * dim * NP] = h;
             }
     }
@@ -261,7 +267,8 @@ static hipError_t launch_scan(const ScanParams &p, hipStream_t st)
 
 // One token: state and inputs are read once, the new state and y written once.  A quad per channel, no LDS; a thread takes the same
 // channel of R sequences, so that their loads are in flight together and A, bias and skip are read once for them.  state_out may be
-// state: every thread reads its own states before it writes them.
+// state: every thread reads its own states before it writes them.  Memory-bound: 256 x 4096 channels of 16 states 29.6 us, 4.8 TB/s;
+// one sequence of 192 channels 3 us, and 14 for the call.
 template <typename T, int E>
 __device__ __forceinline__ void load_row(const T *row, int q, int N, bool vec, float (&v)[E])
 {
@@ -328,7 +335,8 @@ static hipError_t launch_step_rows(const ScanParams &p, hipStream_t st)
     scan_step_kernel<T, NP, R><<<dim3((unsigned)((items + 63) / 64)), 256, 0, st>>>(p);
     return hipGetLastError();
 }
-// Four sequences to a thread once the threads still fill the chip (2048 blocks of 256)
+// Four sequences to a thread once the threads still fill the chip (2048 blocks of 256): 256 x 4096 44 us with one, 33 with four; fewer
+// blocks would leave compute units idle, which a single sequence's call at 192 channels cannot afford.
 template <typename T, int NP>
 static hipError_t launch_step(const ScanParams &p, hipStream_t st)
 {
