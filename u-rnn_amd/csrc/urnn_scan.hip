@@ -229,13 +229,13 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
 }
 
 // Chunks of the time axis: one from 640 waves on, where the pass over the chunks' ends would cost more than the waves it wins;
-// below that as many as give 6144 waves (three turns of two waves on each of the 1024 SIMDs), but none shorter than 32 tokens.
-// Measured with 3000 waves of 64 tokens at least and with 6144 of 32: 32 768 tokens of 2048 channels 483 and 468 us, seven
+// below that as many as give 9216 waves (three turns of the three that each of the 1024 SIMDs holds), but none shorter than 32 tokens.
+// Measured with 3000 waves of 64 tokens at least and with 9216 of 32: 32 768 tokens of 2048 channels 483 and 462 us (12 288: 476), seven
 // sequences of up to 1021 tokens of 1000 channels 72 and 67 us, forward and backward of 4 x 2048 x 2048 491 and 492 us.
 int urnn_scan_chunks(int B, int L, int D, int *CL)
 {
     const long waves = (long)B * ((D + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
-    long want = waves >= 640 ? 1 : (6144 + waves - 1) / waves;
+    long want = waves >= 640 ? 1 : (9216 + waves - 1) / waves;
     const long most = (L + 31) / 32;
     if (want > most) want = most;
     if (want < 1) want = 1;

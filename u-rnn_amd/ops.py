@@ -524,12 +524,15 @@ def _span(t):
 def _seq_out(what, name, t, shape, dtype, inputs, same=()):
     """A given output buffer: contiguous, of the result's shape, and apart from every input (``same``: inputs it may be exactly)."""
     _seq_check(what, name, t, shape, dtype, contiguous=True)
-    lo, hi = _span(t)
+    lo = t.data_ptr()
+    hi = lo + t.numel() * t.element_size()
     for x in inputs:
-        if x is None or x.numel() == 0:
+        if x is None:
             continue
-        a, b = _span(x)
-        if a < hi and lo < b and not any(x is s and a == lo and x.is_contiguous() for s in same):
+        a = x.data_ptr()
+        if a >= hi or (a < lo and _span(x)[1] <= lo) or x.numel() == 0:
+            continue
+        if a != lo or not any(x is s for s in same) or not x.is_contiguous():
             raise RuntimeError(f"{what}: {name} overlaps an input")
 
 
@@ -569,6 +572,10 @@ def _conv_seq_check(what, x, weight, bias, state, lead):
     if weight.dim() != 2 or weight.shape[0] != D or not 2 <= weight.shape[1] <= 4:
         raise RuntimeError(f"{what}: weight has shape {tuple(weight.shape)}, expected ({D}, 2..4)")
     K = weight.shape[1]
+    if (x.shape == lead + (D,) and x.stride(-1) == 1 and weight.dtype is torch.float32 and weight.is_contiguous()      # the usual call, in one go
+            and (bias is None or (bias.shape == (D,) and bias.dtype is torch.float32 and bias.is_contiguous()))
+            and (state is None or (state.shape == (lead[0], K - 1, D) and state.dtype is x.dtype and state.is_contiguous()))):
+        return D, K
     _seq_check(what, "x", x, lead + (D,), x.dtype)
     _seq_check(what, "weight", weight, (D, K), torch.float32, contiguous=True)
     if bias is not None:
@@ -638,6 +645,17 @@ def _scan_check(what, u, delta, A, B, C, D, z, delta_bias, lead):
     if A.dim() != 2 or A.shape[0] != dim or not 1 <= A.shape[1] <= 64:
         raise RuntimeError(f"{what}: A has shape {tuple(A.shape)}, expected ({dim}, 1..64)")
     N = A.shape[1]
+    dt, f32, shape = u.dtype, torch.float32, u.shape
+    if B.dim() == len(lead) + 2 and shape == lead + (dim,) and delta.shape == shape and delta.dtype is dt and A.dtype is f32 and A.is_contiguous():
+        G = B.shape[-2]                                  # the usual call, in one go; whatever it does not settle goes through the list below
+        rows, par = lead + (G, N), (dim,)
+        if (G >= 1 and dim % G == 0 and B.shape == rows and C.shape == rows and B.dtype is dt and C.dtype is dt
+                and u.stride(-1) == delta.stride(-1) == B.stride(-1) == C.stride(-1) == 1
+                and (G == 1 or B.stride(-2) == C.stride(-2) == N)
+                and (z is None or (z.shape == shape and z.dtype is dt and z.stride(-1) == 1))
+                and (D is None or (D.shape == par and D.dtype is f32 and D.is_contiguous()))
+                and (delta_bias is None or (delta_bias.shape == par and delta_bias.dtype is f32 and delta_bias.is_contiguous()))):
+            return dim, G, N, B, C
     _seq_check(what, "u", u, lead + (dim,), u.dtype)
     _seq_check(what, "delta", delta, lead + (dim,), u.dtype)
     if z is not None:
@@ -744,9 +762,12 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
 
 def _rows(what, name, t, shape, dtype):
     """(..., D): strides of the rows, as (outer, inner) of a (B, L, D) tensor or (anything, row) of evenly spaced rows."""
-    _seq_check(what, name, t, shape, dtype)
     if len(shape) == 2:
-        return 0, t.stride(0) if shape[0] > 1 else shape[1]
+        inner, channel = t.stride()[-2:] if t.shape == shape else (0, 0)
+        if channel != 1 or t.dtype is not dtype:
+            _seq_check(what, name, t, shape, dtype)
+        return 0, inner if shape[0] > 1 else shape[1]
+    _seq_check(what, name, t, shape, dtype)
     if len(shape) == 3:
         return t.stride()[:2]
     stride, n = None, 1
@@ -769,7 +790,7 @@ def _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act):
     if D > 16384:
         raise RuntimeError(f"{what}: {D} channels (at most 16384)")
     for name, t in (("pre_w", pre_w), ("post_w", post_w), ("scale", scale)):
-        if t is not None:
+        if t is not None and not (t.shape == (D,) and t.dtype is torch.float32 and t.is_contiguous()):
             _seq_check(what, name, t, (D,), torch.float32, contiguous=True)
     return _row_strides(what, y, (("y", y), ("gate", gate), ("residual", residual)))
 
