@@ -61,19 +61,21 @@ __device__ __forceinline__ const T *row_at(const void *base, const SeqStride &s,
     const unsigned r = (unsigned)row;                // at most 2^23 rows
     return reinterpret_cast<const T *>(base) + (long)(r / inner) * s.b + (long)(r % inner) * s.t;
 }
-template <typename T, int V, int NT, int EPT>
+// WIDE: rows start on 16 bytes and hold whole groups.
+template <typename T, int V, int NT, int EPT, bool WIDE>
 __device__ __forceinline__ void row_load(const T *row, int ln, int D, float (&v)[EPT])
 {
 #pragma unroll
     for (int c = 0; c < EPT / V; ++c) {
         const int d = (c * NT + ln) * V;
         Pack<T, V> t = {};
-        if (d < D) t = *reinterpret_cast<const Pack<T, V> *>(row + d);
+        if constexpr (!WIDE) t = load_loose<T, V>(row + d, D - d);
+        else if (d < D) t = *reinterpret_cast<const Pack<T, V> *>(row + d);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[c * V + i] = to_f(t.v[i]);
     }
 }
-template <typename T, int V, int NT, int EPT>
+template <typename T, int V, int NT, int EPT, bool WIDE>
 __device__ __forceinline__ void row_store(T *row, int ln, int D, const float (&v)[EPT])
 {
 #pragma unroll
@@ -82,11 +84,12 @@ __device__ __forceinline__ void row_store(T *row, int ln, int D, const float (&v
         Pack<T, V> t;
 #pragma unroll
         for (int i = 0; i < V; ++i) t.v[i] = from_f<T>(v[c * V + i]);
-        if (d < D) stream_store(row + d, t);
+        if constexpr (!WIDE) store_loose<T, V>(row + d, t, D - d);
+        else if (d < D) stream_store(row + d, t);
     }
 }
 // A parameter (fp32): in groups of at most four
-template <int V, int NT, int EPT>
+template <int V, int NT, int EPT, bool WIDE>
 __device__ __forceinline__ void par_load(const float *w, int ln, int D, float fill, float (&v)[EPT])
 {
     constexpr int W = V % 4 == 0 ? 4 : 1;
@@ -98,13 +101,16 @@ __device__ __forceinline__ void par_load(const float *w, int ln, int D, float fi
             Pack<float, W> t;
 #pragma unroll
             for (int i = 0; i < W; ++i) t.v[i] = fill;
-            if (w && d < D) t = *reinterpret_cast<const Pack<float, W> *>(w + d);
+            if (w && d < D) {
+                if constexpr (WIDE) t = *reinterpret_cast<const Pack<float, W> *>(w + d);
+                else t = load_loose<float, W>(w + d, D - d);
+            }
 #pragma unroll
             for (int i = 0; i < W; ++i) v[c * V + k + i] = t.v[i];
         }
 }
 
-template <int V, int NT, int EPT>
+template <int V, int NT, int EPT, bool WIDE>
 __device__ __forceinline__ void par_store(float *w, int ln, int D, const float (&v)[EPT])
 {
     constexpr int W = V % 4 == 0 ? 4 : 1;
@@ -116,11 +122,12 @@ __device__ __forceinline__ void par_store(float *w, int ln, int D, const float (
             Pack<float, W> t;
 #pragma unroll
             for (int i = 0; i < W; ++i) t.v[i] = v[c * V + k + i];
-            if (d < D) *reinterpret_cast<Pack<float, W> *>(w + d) = t;
+            if constexpr (!WIDE) store_loose<float, W>(w + d, t, D - d);
+            else if (d < D) *reinterpret_cast<Pack<float, W> *>(w + d) = t;
         }
 }
 
-template <typename T, int V, int NT, int EPT>
+template <typename T, int V, int NT, int EPT, bool WIDE>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const NormParams p)
 {
     __shared__ float red[2][NT < 256 ? 4 : NT / 64][2];
@@ -131,15 +138,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const NormPar
     const long row = ok ? row0 : 0;
     const float inv = 1.0f / (float)D;
     float y[EPT], r[EPT], w[EPT], s[EPT], v[EPT];
-    row_load<T, V, NT, EPT>(row_at<T>(p.y, p.sy, row, p.inner), ln, D, y);
+    row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.y, p.sy, row, p.inner), ln, D, y);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) r[i] = 0.0f;
-    if (p.residual) row_load<T, V, NT, EPT>(row_at<T>(p.residual, p.sr, row, p.inner), ln, D, r);
+    if (p.residual) row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.residual, p.sr, row, p.inner), ln, D, r);
     float g[EPT];
-    if (p.gate) row_load<T, V, NT, EPT>(row_at<T>(p.gate, p.sg, row, p.inner), ln, D, g);
-    par_load<V, NT, EPT>(p.post_w, ln, D, 1.0f, w);
-    par_load<V, NT, EPT>(p.scale, ln, D, 1.0f, s);
-    par_load<V, NT, EPT>(p.pre_w, ln, D, 0.0f, v);
+    if (p.gate) row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.gate, p.sg, row, p.inner), ln, D, g);
+    par_load<V, NT, EPT, WIDE>(p.post_w, ln, D, 1.0f, w);
+    par_load<V, NT, EPT, WIDE>(p.scale, ln, D, 1.0f, s);
+    par_load<V, NT, EPT, WIDE>(p.pre_w, ln, D, 0.0f, v);
     float ss = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) ss = fmaf(y[i], y[i], ss);
@@ -160,13 +167,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const NormPar
     row_sum2<NT>(ss, none, red[1]);
     const float rr = __builtin_amdgcn_rsqf(fmaf(ss, inv, p.eps));
     if (!ok) return;
-    if (p.res_out) row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.res_out) + row * D, ln, D, r);
+    if (p.res_out) row_store<T, V, NT, EPT, WIDE>(reinterpret_cast<T *>(p.res_out) + row * D, ln, D, r);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) r[i] *= rr * v[i];
-    row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.normed) + row * D, ln, D, r);
+    row_store<T, V, NT, EPT, WIDE>(reinterpret_cast<T *>(p.normed) + row * D, ln, D, r);
 }
 
-template <typename T, int V, int NT, int EPT>
+template <typename T, int V, int NT, int EPT, bool WIDE>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(const NormParams p)
 {
     __shared__ float red[3][NT < 256 ? 4 : NT / 64][2];
@@ -175,21 +182,21 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(cons
     const int ln = threadIdx.x % NT, rg = threadIdx.x / NT, D = p.dim;
     const float inv = 1.0f / (float)D;
     float w[EPT], s[EPT], v[EPT], cv[EPT] = {}, cw[EPT] = {}, cs[EPT] = {};
-    par_load<V, NT, EPT>(p.post_w, ln, D, 1.0f, w);
-    par_load<V, NT, EPT>(p.scale, ln, D, 1.0f, s);
-    par_load<V, NT, EPT>(p.pre_w, ln, D, 0.0f, v);
+    par_load<V, NT, EPT, WIDE>(p.post_w, ln, D, 1.0f, w);
+    par_load<V, NT, EPT, WIDE>(p.scale, ln, D, 1.0f, s);
+    par_load<V, NT, EPT, WIDE>(p.pre_w, ln, D, 0.0f, v);
     for (long base = (long)blockIdx.x * RB; base < p.rows; base += (long)gridDim.x * RB) {
         const long row0 = base + rg;
         const bool ok = row0 < p.rows;
         const long row = ok ? row0 : base;
         float y[EPT], r[EPT], g[EPT], dn[EPT], dr[EPT], a[EPT], da[EPT];
-        row_load<T, V, NT, EPT>(row_at<T>(p.y, p.sy, row, p.inner), ln, D, y);
+        row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.y, p.sy, row, p.inner), ln, D, y);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) { r[i] = dn[i] = dr[i] = 0.0f; a[i] = 1.0f; da[i] = 0.0f; }
-        if (p.residual) row_load<T, V, NT, EPT>(row_at<T>(p.residual, p.sr, row, p.inner), ln, D, r);
-        if (p.gate) row_load<T, V, NT, EPT>(row_at<T>(p.gate, p.sg, row, p.inner), ln, D, g);
-        if (p.dnormed) row_load<T, V, NT, EPT>(row_at<T>(p.dnormed, p.sdn, row, p.inner), ln, D, dn);
-        if (p.dres) row_load<T, V, NT, EPT>(row_at<T>(p.dres, p.sdr, row, p.inner), ln, D, dr);
+        if (p.residual) row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.residual, p.sr, row, p.inner), ln, D, r);
+        if (p.gate) row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.gate, p.sg, row, p.inner), ln, D, g);
+        if (p.dnormed) row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.dnormed, p.sdn, row, p.inner), ln, D, dn);
+        if (p.dres) row_load<T, V, NT, EPT, WIDE>(row_at<T>(p.dres, p.sdr, row, p.inner), ln, D, dr);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) s1 = fmaf(y[i], y[i], s1);
@@ -225,17 +232,17 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(cons
         row_sum2<NT>(s1, s2, red[2]);
         const float m2 = p.post_w ? s2 * inv : 0.0f;
         if (ok) {
-            if (p.dresidual) row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.dresidual) + row * D, ln, D, dr);
-            if (p.dgate) row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.dgate) + row * D, ln, D, da);
+            if (p.dresidual) row_store<T, V, NT, EPT, WIDE>(reinterpret_cast<T *>(p.dresidual) + row * D, ln, D, dr);
+            if (p.dgate) row_store<T, V, NT, EPT, WIDE>(reinterpret_cast<T *>(p.dgate) + row * D, ln, D, da);
 #pragma unroll
             for (int i = 0; i < EPT; ++i) r[i] = ry * fmaf(-y[i], m2, r[i]);
-            row_store<T, V, NT, EPT>(reinterpret_cast<T *>(p.dy) + row * D, ln, D, r);
+            row_store<T, V, NT, EPT, WIDE>(reinterpret_cast<T *>(p.dy) + row * D, ln, D, r);
         }
     }
     auto put = [&](int which, const float (&c)[EPT]) {
         float *out = p.partial + ((long)blockIdx.x * 3 + which) * D;
         if (RB == 1) {
-            par_store<V, NT, EPT>(out, ln, D, c);
+            par_store<V, NT, EPT, WIDE>(out, ln, D, c);
         } else {
             __syncthreads();
 #pragma unroll
@@ -302,31 +309,31 @@ int urnn_norm_parts(long rows, int D)
     return (int)((blocks + turns - 1) / turns);
 }
 
-template <typename T, int V, int NT, int EPT>
+template <typename T, int V, int NT, int EPT, bool WIDE>
 static hipError_t launch_norm(const NormParams &p, bool backward, hipStream_t st)
 {
     constexpr int threads = NT < 256 ? 256 : NT, RB = NT < 256 ? 256 / NT : 1;
-    if (backward) norm_backward_kernel<T, V, NT, EPT><<<dim3((unsigned)p.parts), threads, 0, st>>>(p);
-    else norm_kernel<T, V, NT, EPT><<<dim3((unsigned)((p.rows + RB - 1) / RB)), threads, 0, st>>>(p);
+    if (backward) norm_backward_kernel<T, V, NT, EPT, WIDE><<<dim3((unsigned)p.parts), threads, 0, st>>>(p);
+    else norm_kernel<T, V, NT, EPT, WIDE><<<dim3((unsigned)((p.rows + RB - 1) / RB)), threads, 0, st>>>(p);
     return hipGetLastError();
 }
-template <typename T, int V>
+template <typename T, int V, bool WIDE>
 static hipError_t by_width(const NormParams &p, bool backward, hipStream_t st)
 {
     const int D = p.dim;
-    if (D <= 128) return launch_norm<T, V, 16, 8>(p, backward, st);
-    if (D <= 512) return launch_norm<T, V, 64, 8>(p, backward, st);
-    if (D <= 1024) return launch_norm<T, V, 128, 8>(p, backward, st);
-    if (D <= 2048) return launch_norm<T, V, 256, 8>(p, backward, st);
-    if (D <= 4096) return launch_norm<T, V, 512, 8>(p, backward, st);
-    if (D <= 8192) return launch_norm<T, V, 1024, 8>(p, backward, st);
-    return launch_norm<T, V, 1024, 16>(p, backward, st);
+    if (D <= 128) return launch_norm<T, V, 16, 8, WIDE>(p, backward, st);
+    if (D <= 512) return launch_norm<T, V, 64, 8, WIDE>(p, backward, st);
+    if (D <= 1024) return launch_norm<T, V, 128, 8, WIDE>(p, backward, st);
+    if (D <= 2048) return launch_norm<T, V, 256, 8, WIDE>(p, backward, st);
+    if (D <= 4096) return launch_norm<T, V, 512, 8, WIDE>(p, backward, st);
+    if (D <= 8192) return launch_norm<T, V, 1024, 8, WIDE>(p, backward, st);
+    return launch_norm<T, V, 1024, 16, WIDE>(p, backward, st);
 }
 static hipError_t by_type(const NormParams &p, int dtype, bool wide, bool backward, hipStream_t st)
 {
-    if (dtype == URNN_F32) return wide ? by_width<float, 4>(p, backward, st) : by_width<float, 1>(p, backward, st);
-    if (dtype == URNN_BF16) return wide ? by_width<bf16_t, 8>(p, backward, st) : by_width<bf16_t, 1>(p, backward, st);
-    return wide ? by_width<f16_t, 8>(p, backward, st) : by_width<f16_t, 1>(p, backward, st);
+    if (dtype == URNN_F32) return wide ? by_width<float, 4, true>(p, backward, st) : by_width<float, 4, false>(p, backward, st);
+    if (dtype == URNN_BF16) return wide ? by_width<bf16_t, 8, true>(p, backward, st) : by_width<bf16_t, 8, false>(p, backward, st);
+    return wide ? by_width<f16_t, 8, true>(p, backward, st) : by_width<f16_t, 8, false>(p, backward, st);
 }
 
 hipError_t urnn_launch_norm(const NormParams &p, int dtype, bool wide, hipStream_t st) { return by_type(p, dtype, wide, false, st); }

@@ -57,8 +57,8 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
     const int lane = threadIdx.x;
     const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
-    const int walked = FULL ? p.chunks : p.chunks - 1;           // nothing reads the summary of the last chunk (BACK: the first)
-    const int chunk = (BACK ? 1 : 0) + blockIdx.x / (cbs * p.G) % walked, b = blockIdx.x / (cbs * p.G) / walked;
+    // the sequences of a chunk before the next chunk: those of a padded batch end in the same late blocks, spread over the chip
+    const int rest = blockIdx.x / (cbs * p.G), b = rest % p.batch, chunk = (BACK ? 1 : 0) + rest / p.batch;
     const int len = __builtin_amdgcn_readfirstlane(seq_len(p.lengths, b, p.L));
     const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L, te = tfull < len ? tfull : len;
     const int n = te > tb ? (int)(te - tb) : 0;                  // tokens to walk; token i is first + dir i

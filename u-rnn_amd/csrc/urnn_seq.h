@@ -64,6 +64,35 @@ __device__ __forceinline__ float quad_sum(float v)
     return v;
 }
 
+// V elements of a row of which only the element's own alignment is known: one 16-byte access all the same (global memory takes any
+// alignment); the row's last group, of `left` < V elements, one by one, zeros behind them.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_loose(const T *src, int left)
+{
+    Pack<T, V> t = {};
+    if (left >= V) {
+        __builtin_memcpy(&t, src, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) t.v[i] = src[i];
+    }
+    return t;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_loose(T *dst, const Pack<T, V> &t, int left)
+{
+    typedef unsigned loose __attribute__((ext_vector_type(4), aligned(2)));
+    if (left >= V) {
+        if constexpr (sizeof(t) == 16) __builtin_nontemporal_store(__builtin_bit_cast(loose, t), reinterpret_cast<loose *>(dst));
+        else __builtin_memcpy(dst, &t, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) dst[i] = t.v[i];
+    }
+}
+
 // Tokens of sequence b that count: lengths clamped to [0, L], so that no length can reach outside the tensors.
 __device__ __forceinline__ int seq_len(const int *lengths, int b, int L)
 {
