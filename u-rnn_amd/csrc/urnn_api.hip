@@ -1608,11 +1608,7 @@ extern "C" int urnn_causal_conv_backward(const void *x, long x_batch, long x_tok
     p.weight = weight; p.bias = bias; p.state = state; p.lengths = lengths; p.dstate_out = dstate_out; p.dx = dx; p.dstate = dstate;
     p.partial = reinterpret_cast<float *>(workspace);
     p.batch = B; p.L = L; p.dim = D; p.K = K; p.silu = silu;
-    const int e = seq_elem(dtype);
-    const bool wide = wide_rows(x, x_batch, x_token, e) && wide_rows(dout, dout_batch, dout_token, e) && (long)D * e % 16 == 0 && aligned16(dx) &&
-                      aligned16(weight) && (!bias || aligned16(bias)) && (!state || aligned16(state)) && (!dstate || aligned16(dstate)) &&
-                      (!dstate_out || aligned16(dstate_out));
-    CHECK_HIP(urnn_launch_conv_seq_backward(p, dtype, wide, dweight, dbias, accumulate, (hipStream_t)stream), "causal_conv_backward");
+    CHECK_HIP(urnn_launch_conv_seq_backward(p, dtype, dweight, dbias, accumulate, (hipStream_t)stream), "causal_conv_backward");
     return URNN_OK;
 }
 

@@ -9,6 +9,8 @@
 // takes; 6 x 1531 x 1001 fp32 (no row aligned, padded): 12.4 us, backward 25.4 + 4.3 us for the sums, 2.8 TB/s.
 #include "urnn_seq.h"
 
+#include <type_traits>
+
 template <typename T, int V>
 __device__ __forceinline__ void load_v(const T *src, float (&v)[V])
 {
@@ -23,6 +25,23 @@ __device__ __forceinline__ void store_v(T *dst, const float (&v)[V])
 #pragma unroll
     for (int i = 0; i < V; ++i) t.v[i] = from_f<T>(v[i]);
     stream_store(dst, t);
+}
+
+// The same for the backward's groups, at rows of any alignment.
+template <typename T, int V>
+__device__ __forceinline__ void load_l(const T *src, float (&v)[V])
+{
+    const Pack<T, V> t = load_any<T, V>(src);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f(t.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_l(T *dst, const float (&v)[V])
+{
+    Pack<T, V> t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t.v[i] = from_f<T>(v[i]);
+    store_any<T, V>(dst, t);
 }
 
 // The taps of V channels: w[k] belongs to line[t + k].  The weights of V adjacent channels are V K adjacent floats.
@@ -139,13 +158,19 @@ template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqParams p, int xb)
 {
     __shared__ float s_sum[256 * V];
-    const int nv = p.dim / V, yb = 256 / xb, xi = threadIdx.x % xb, yi = threadIdx.x / xb;
+    const int nv = (p.dim + V - 1) / V, yb = 256 / xb, xi = threadIdx.x % xb, yi = threadIdx.x / xb;
     const int cbs = (nv + xb - 1) / xb, cb = blockIdx.x % cbs, part = blockIdx.x / cbs;
     const int cv = cb * xb + xi;
     const bool ok = cv < nv;
-    const int d = ok ? cv * V : 0;
+    auto channel = [&](int c) { return c * V < p.dim - V ? c * V : p.dim - V; };     // the last group repeats channels of the one before it, bit for bit
+    const int d = ok ? channel(cv) : 0;
     float w[K][V], bias[V], dw[K][V] = {}, db[V] = {};
-    load_taps<V, K>(p, d, w, bias);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = p.bias ? p.bias[d + i] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][i] = p.weight[(long)(d + i) * K + k];
+    }
     const long all = (long)p.batch * p.chunks;
     for (long c = (long)part * yb + yi; ok && c < all; c += (long)p.parts * yb) {
         const int b = (int)(c / p.chunks);
@@ -161,8 +186,8 @@ __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqPar
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] = 0.0f;
             if (j >= 0) {
-                if (j < len) load_v<T, V>(x + j * p.sx.t, v);
-            } else if (state && j >= -(K - 1)) load_v<T, V>(state + (j + K - 1) * p.dim, v);
+                if (j < len) load_l<T, V>(x + j * p.sx.t, v);
+            } else if (state && j >= -(K - 1)) load_l<T, V>(state + (j + K - 1) * p.dim, v);
         };
         // dp and the line's window of token s: win[k] = line entry s - K + 1 + k
         float win[K][V], dp[K][V];                             // dp[k]: token s - K + 1 + k
@@ -183,8 +208,8 @@ __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqPar
 #pragma unroll
                     for (int i = 0; i < V; ++i) ahead[a][i] = dahead[a][i] = 0.0f;
                     if (s0 + a < len && s0 + a < send) {
-                        load_v<T, V>(x + (s0 + a) * p.sx.t, ahead[a]);
-                        load_v<T, V>(dy + (s0 + a) * p.so.t, dahead[a]);
+                        load_l<T, V>(x + (s0 + a) * p.sx.t, ahead[a]);
+                        load_l<T, V>(dy + (s0 + a) * p.so.t, dahead[a]);
                     }
                 }
 #pragma unroll
@@ -229,17 +254,17 @@ __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqPar
                     }
                     if (dso && j >= (long)len - (K - 1)) {
                         float v[V];
-                        load_v<T, V>(dso + (j - ((long)len - (K - 1))) * p.dim, v);
+                        load_l<T, V>(dso + (j - ((long)len - (K - 1))) * p.dim, v);
 #pragma unroll
                         for (int i = 0; i < V; ++i) o[i] += v[i];
                     }
-                    if (j >= 0) store_v<T, V>(dx + j * p.dim, o);
-                    else if (dst) store_v<T, V>(dst + (j + K - 1) * p.dim, o);
+                    if (j >= 0) store_l<T, V>(dx + j * p.dim, o);
+                    else if (dst) store_l<T, V>(dst + (j + K - 1) * p.dim, o);
                 }
             }
         }
         float zero[V] = {};
-        for (long t = te > t0 ? te : t0; t < tend; ++t) store_v<T, V>(dx + t * p.dim, zero);
+        for (long t = te > t0 ? te : t0; t < tend; ++t) store_l<T, V>(dx + t * p.dim, zero);
     }
     // fold the token lanes, K taps and the bias one after the other
     for (int k = 0; k <= K; ++k) {
@@ -256,13 +281,14 @@ __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqPar
             float a = 0.0f;
             for (int l = 0; l < yb; ++l) a += s_sum[l * V * xb + r];
             const int i = r / xb, c = cb * xb + r % xb;
-            if (c < nv) p.partial[(long)part * (K + 1) * p.dim + (k < K ? (c * V + i) * K + k : K * p.dim + c * V + i)] = a;
+            if (c < nv) p.partial[(long)part * (K + 1) * p.dim + (k < K ? (channel(c) + i) * K + k : K * p.dim + channel(c) + i)] = a;
         }
     }
 }
 
 // Work split of the backward: a block takes XB channel vectors, parts x 256 / XB token lanes share the chunks.  1024 blocks: four to a
 // compute unit; twice as many lose 3 % at 6 x 1531 x 1001 (more partial sums, no more bytes in flight).
+enum { BV = 2 };
 static int conv_xb(int nv) { int xb = 8; while (xb < 64 && xb < nv) xb <<= 1; return xb; }
 static int conv_parts(int B, int L, int D, int cover)
 {
@@ -272,24 +298,28 @@ static int conv_parts(int B, int L, int D, int cover)
     if (parts > most) parts = most;
     return parts < 1 ? 1 : (int)parts;
 }
-int urnn_conv_seq_parts(int B, int L, int D) { return conv_parts(B, L, D, 512); }       // the most that any vector width takes
+int urnn_conv_seq_parts(int B, int L, int D) { return conv_parts(B, L, D, 64 * BV); }
+
+template <typename T, int V, int K>
+static hipError_t launch_conv_backward(ConvSeqParams p, hipStream_t st)
+{
+    const int nv = (p.dim + V - 1) / V;
+    const int xb = conv_xb(nv), cbs = (nv + xb - 1) / xb;
+    p.parts = urnn_conv_seq_parts(p.batch, p.L, p.dim);
+    const long lanes = (long)p.parts * (256 / xb);
+    long T_ = ((long)p.batch * p.L + lanes - 1) / lanes;     // about one chunk per lane, 8 .. 64 tokens
+    T_ = T_ < 8 ? 8 : T_ > 64 ? 64 : T_;
+    if (T_ > p.L) T_ = p.L;
+    p.T = (int)T_;
+    p.chunks = (p.L + p.T - 1) / p.T;
+    conv_seq_backward_kernel<T, V, K><<<dim3((unsigned)(cbs * p.parts)), 256, 0, st>>>(p, xb);
+    return hipGetLastError();
+}
 
 template <typename T, int V, int K>
 static hipError_t launch_conv(ConvSeqParams p, int what, hipStream_t st)
 {
     const int nv = p.dim / V;
-    if (what == 2) {
-        const int xb = conv_xb(nv), cbs = (nv + xb - 1) / xb;
-        p.parts = conv_parts(p.batch, p.L, p.dim, 64 * V);
-        const long lanes = (long)p.parts * (256 / xb);
-        long T_ = ((long)p.batch * p.L + lanes - 1) / lanes;     // about one chunk per lane, 8 .. 64 tokens
-        T_ = T_ < 8 ? 8 : T_ > 64 ? 64 : T_;
-        if (T_ > p.L) T_ = p.L;
-        p.T = (int)T_;
-        p.chunks = (p.L + p.T - 1) / p.T;
-        conv_seq_backward_kernel<T, V, K><<<dim3((unsigned)(cbs * p.parts)), 256, 0, st>>>(p, xb);
-        return hipGetLastError();
-    }
     if (what == 1) {
         const long items = (long)p.batch * nv;
         conv_seq_step_kernel<T, V, K><<<dim3((unsigned)((items + 255) / 256)), 256, 0, st>>>(p);
@@ -318,14 +348,23 @@ static hipError_t by_type(const ConvSeqParams &p, int dtype, bool wide, int what
     return wide ? by_taps<f16_t, 8>(p, what, st) : by_taps<f16_t, 1>(p, what, st);
 }
 
+template <typename T, int V>
+static hipError_t backward_by_taps(const ConvSeqParams &p, hipStream_t st)
+{
+    return p.K == 2 ? launch_conv_backward<T, V, 2>(p, st) : p.K == 3 ? launch_conv_backward<T, V, 3>(p, st) : launch_conv_backward<T, V, 4>(p, st);
+}
+
 hipError_t urnn_launch_conv_seq(ConvSeqParams p, int dtype, bool wide, hipStream_t st) { return by_type(p, dtype, wide, 0, st); }
 hipError_t urnn_launch_conv_seq_step(const ConvSeqParams &p, int dtype, bool wide, hipStream_t st) { return by_type(p, dtype, wide, 1, st); }
-hipError_t urnn_launch_conv_seq_backward(ConvSeqParams p, int dtype, bool wide, float *dweight, float *dbias, int accumulate, hipStream_t st)
+hipError_t urnn_launch_conv_seq_backward(const ConvSeqParams &p, int dtype, float *dweight, float *dbias, int accumulate, hipStream_t st)
 {
-    const hipError_t e = by_type(p, dtype, wide, 2, st);
+    auto go = [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        return dtype == URNN_F32 ? backward_by_taps<float, V>(p, st) : dtype == URNN_BF16 ? backward_by_taps<bf16_t, V>(p, st) : backward_by_taps<f16_t, V>(p, st);
+    };
+    const hipError_t e = p.dim >= BV ? go(std::integral_constant<int, BV>()) : go(std::integral_constant<int, 1>());
     if (e != hipSuccess) return e;
-    const int parts = conv_parts(p.batch, p.L, p.dim, 64 * (!wide ? 1 : dtype == URNN_F32 ? 4 : 8));
     const long sizes[3] = {(long)p.dim * p.K, p.dim, 0};
     float *const outs[3] = {dweight, dbias, nullptr};
-    return urnn_launch_sum_parts(p.partial, parts, sizes, outs, accumulate, st);
+    return urnn_launch_sum_parts(p.partial, urnn_conv_seq_parts(p.batch, p.L, p.dim), sizes, outs, accumulate, st);
 }

@@ -61,7 +61,7 @@ __device__ __forceinline__ const T *row_at(const void *base, const SeqStride &s,
     const unsigned r = (unsigned)row;                // at most 2^23 rows
     return reinterpret_cast<const T *>(base) + (long)(r / inner) * s.b + (long)(r % inner) * s.t;
 }
-// WIDE: rows start on 16 bytes and hold whole groups.
+// WIDE: rows start on 16 bytes and hold whole groups; otherwise a row holds one group at least (or V is 1).
 template <typename T, int V, int NT, int EPT, bool WIDE>
 __device__ __forceinline__ void row_load(const T *row, int ln, int D, float (&v)[EPT])
 {
@@ -69,7 +69,7 @@ __device__ __forceinline__ void row_load(const T *row, int ln, int D, float (&v)
     for (int c = 0; c < EPT / V; ++c) {
         const int d = (c * NT + ln) * V;
         Pack<T, V> t = {};
-        if constexpr (!WIDE) t = load_loose<T, V>(row + d, D - d);
+        if constexpr (!WIDE) t = load_tail<T, V>(row, d, D);
         else if (d < D) t = *reinterpret_cast<const Pack<T, V> *>(row + d);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[c * V + i] = to_f(t.v[i]);
@@ -84,7 +84,7 @@ __device__ __forceinline__ void row_store(T *row, int ln, int D, const float (&v
         Pack<T, V> t;
 #pragma unroll
         for (int i = 0; i < V; ++i) t.v[i] = from_f<T>(v[c * V + i]);
-        if constexpr (!WIDE) store_loose<T, V>(row + d, t, D - d);
+        if constexpr (!WIDE) store_tail<T, V>(row, t, d, D);
         else if (d < D) stream_store(row + d, t);
     }
 }
@@ -101,10 +101,9 @@ __device__ __forceinline__ void par_load(const float *w, int ln, int D, float fi
             Pack<float, W> t;
 #pragma unroll
             for (int i = 0; i < W; ++i) t.v[i] = fill;
-            if (w && d < D) {
-                if constexpr (WIDE) t = *reinterpret_cast<const Pack<float, W> *>(w + d);
-                else t = load_loose<float, W>(w + d, D - d);
-            }
+            if constexpr (!WIDE) {
+                if (w) t = load_tail<float, W>(w, d, D);
+            } else if (w && d < D) t = *reinterpret_cast<const Pack<float, W> *>(w + d);
 #pragma unroll
             for (int i = 0; i < W; ++i) v[c * V + k + i] = t.v[i];
         }
@@ -122,7 +121,7 @@ __device__ __forceinline__ void par_store(float *w, int ln, int D, const float (
             Pack<float, W> t;
 #pragma unroll
             for (int i = 0; i < W; ++i) t.v[i] = v[c * V + k + i];
-            if constexpr (!WIDE) store_loose<float, W>(w + d, t, D - d);
+            if constexpr (!WIDE) store_tail<float, W>(w, t, d, D);
             else if (d < D) *reinterpret_cast<Pack<float, W> *>(w + d) = t;
         }
 }
@@ -321,6 +320,7 @@ template <typename T, int V, bool WIDE>
 static hipError_t by_width(const NormParams &p, bool backward, hipStream_t st)
 {
     const int D = p.dim;
+    if (!WIDE && D < V) return launch_norm<T, 1, 16, 8, true>(p, backward, st);
     if (D <= 128) return launch_norm<T, V, 16, 8, WIDE>(p, backward, st);
     if (D <= 512) return launch_norm<T, V, 64, 8, WIDE>(p, backward, st);
     if (D <= 1024) return launch_norm<T, V, 128, 8, WIDE>(p, backward, st);

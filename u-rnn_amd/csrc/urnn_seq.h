@@ -64,32 +64,45 @@ __device__ __forceinline__ float quad_sum(float v)
     return v;
 }
 
-// V elements of a row of which only the element's own alignment is known: one 16-byte access all the same (global memory takes any
-// alignment); the row's last group, of `left` < V elements, one by one, zeros behind them.
+// V elements at the element's own alignment: one access of V * sizeof(T) bytes all the same (global memory takes any alignment).
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_loose(const T *src, int left)
+__device__ __forceinline__ Pack<T, V> load_any(const T *src)
 {
-    Pack<T, V> t = {};
-    if (left >= V) {
-        __builtin_memcpy(&t, src, sizeof(t));
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) t.v[i] = src[i];
-    }
+    Pack<T, V> t;
+    __builtin_memcpy(&t, src, sizeof(t));
     return t;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_loose(T *dst, const Pack<T, V> &t, int left)
+__device__ __forceinline__ void store_any(T *dst, const Pack<T, V> &t)
 {
-    typedef unsigned loose __attribute__((ext_vector_type(4), aligned(2)));
-    if (left >= V) {
-        if constexpr (sizeof(t) == 16) __builtin_nontemporal_store(__builtin_bit_cast(loose, t), reinterpret_cast<loose *>(dst));
-        else __builtin_memcpy(dst, &t, sizeof(t));
-    } else {
+    typedef unsigned any4 __attribute__((ext_vector_type(4), aligned(2)));
+    if constexpr (sizeof(t) == 16) __builtin_nontemporal_store(__builtin_bit_cast(any4, t), reinterpret_cast<any4 *>(dst));
+    else __builtin_memcpy(dst, &t, sizeof(t));
+}
+// Group d .. d + V - 1 of a row of D >= V elements, those from D on as zeros: the row's last V elements, moved down (16 bytes; no branch,
+// which would make every load wait for the one before it).
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_tail(const T *row, int d, int D)
+{
+    static_assert(sizeof(T) * V == 16, "two 64-bit halves");
+    struct Halves { unsigned long long lo, hi; };
+    const int at = d + V <= D ? d : D - V, out = d - at;         // elements to drop, V or more: all
+    Halves h = __builtin_bit_cast(Halves, load_any<T, V>(row + at));
+    const int bits = (out & (V - 1)) * 8 * (int)sizeof(T), sh = bits & 63;
+    const unsigned long long down = sh ? (h.lo >> sh) | (h.hi << (64 - sh)) : h.lo, hi = h.hi >> sh;
+    h.lo = out >= V ? 0 : bits >= 64 ? hi : down;
+    h.hi = out >= V || bits >= 64 ? 0 : hi;
+    return __builtin_bit_cast(Pack<T, V>, h);
+}
+// ... stored element by element where it is not whole
+template <typename T, int V>
+__device__ __forceinline__ void store_tail(T *row, const Pack<T, V> &t, int d, int D)
+{
+    if (d + V <= D) store_any<T, V>(row + d, t);
+    else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (i < left) dst[i] = t.v[i];
+            if (d + i < D) row[d + i] = t.v[i];
     }
 }
 
@@ -228,7 +241,7 @@ struct ConvSeqParams {
 
 hipError_t urnn_launch_conv_seq(ConvSeqParams p, int dtype, bool wide, hipStream_t st);
 hipError_t urnn_launch_conv_seq_step(const ConvSeqParams &p, int dtype, bool wide, hipStream_t st);
-hipError_t urnn_launch_conv_seq_backward(ConvSeqParams p, int dtype, bool wide, float *dweight, float *dbias, int accumulate, hipStream_t st);
+hipError_t urnn_launch_conv_seq_backward(const ConvSeqParams &p, int dtype, float *dweight, float *dbias, int accumulate, hipStream_t st);
 int urnn_conv_seq_parts(int B, int L, int D);
 
 // ---- norms around a block ----------------------------------------------------------------------------------------------
