@@ -6,7 +6,7 @@
 // Memory-bound: one read of x, one write of y.  A thread holds V adjacent channels (16 bytes) and walks T tokens with the last
 // K - 1 inputs in registers, so that an input is read once but for the K - 1 rows before a chunk; threads of a wave are adjacent in
 // the channels.  V = 1 where rows are not 16-byte aligned.  2 x 4096 x 4096 bf16: 26.4 us, 5.1 TB/s, what a copy of those bytes
-// takes; 6 x 1531 x 1001 fp32 (no row aligned, padded): 12.4 us, backward 25.4 + 4.3 us for the sums, 2.8 TB/s.
+// takes; 6 x 1531 x 1001 fp32 (no row aligned, padded): 12.4 us, with the backward and its sums 48 us, 3.1 TB/s.
 #include "urnn_seq.h"
 
 #include <type_traits>
@@ -286,8 +286,10 @@ __global__ __launch_bounds__(256) void conv_seq_backward_kernel(const ConvSeqPar
     }
 }
 
-// Work split of the backward: a block takes XB channel vectors, parts x 256 / XB token lanes share the chunks.  1024 blocks: four to a
-// compute unit; twice as many lose 3 % at 6 x 1531 x 1001 (more partial sums, no more bytes in flight).
+// Work split of the backward: a block takes XB groups of BV channels, parts x 256 / XB token lanes share the chunks.  1024 blocks: four to a
+// compute unit; twice as many lose 3 % at 6 x 1531 x 1001 (more partial sums, no more bytes in flight).  Two channels to a thread: the
+// window, the sums and what is in flight are 11 values of each, and four or eight channels leave too few waves to wait for memory.  With
+// the forward, 2 x 4096 x 2000 bf16 60 us with two, 80 with four, 110 with eight; x 2001 77 us, 99 with one.
 enum { BV = 2 };
 static int conv_xb(int nv) { int xb = 8; while (xb < 64 && xb < nv) xb <<= 1; return xb; }
 static int conv_parts(int B, int L, int D, int cover)

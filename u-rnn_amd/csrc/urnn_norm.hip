@@ -11,8 +11,12 @@
 // taken on the way: NT = 16 (D <= 128), 64 (<= 512), 128, 256, 512, 1024, eight values to a thread (sixteen beyond 8192 channels;
 // sixteen at half the threads: 8192 x 4096 77 us against 70, fewer waves wait for memory).  The backward reads y, g, r again instead
 // of r' and the forward's statistics: r' was rounded on its way out, and it is as many bytes.  Its column sums stay in registers over
-// all rows of a block and are folded in a fixed order.  8192 x 4096 bf16: 70 us, 4.8 TB/s; 12 345 x 1001 fp32, no row aligned: 52 us,
-// backward 82 + 6 us for the sums, 4.5 to 4.8 TB/s -- a copy's 5.0.
+// all rows of a block and are folded in a fixed order.  8192 x 4096 bf16: 70 us, 4.8 TB/s.
+//
+// Widths that no 16 bytes divide take the same accesses at the element's alignment; a row's last group is its last V elements moved
+// down in registers, so that no branch makes one load wait for another.  12 345 x 1001 fp32 50 us, with the backward 126, 5.1 TB/s (element
+// by element 139); 8192 x 2001 bf16 43 us, with the backward 120 (element by element 80 and 298; with a branch at the last group 59
+// and 143; x 2000 35 and 107).
 #include "urnn_seq.h"
 
 enum { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_SILU = 2 };

@@ -16,7 +16,7 @@
 // What bounds it is the vector unit: per state one exponential (measured: the time of 1.6 to 2 fp32 operations) and three fp32
 // operations, per token and channel about 45 more: 119 issue slots at 16 states, 35e12 lane-slots/s of the chip.  4 x 2048 x 2048 bf16:
 // 93 us of 56 us of slots (waves at two to a SIMD wait for their loads and for the chain of a state from token to token), 1.5 TB/s;
-// 32 768 x 2048 468 us with both passes of 226 us of slots for one.
+// 32 768 x 2048 460 us with both passes, of 226 us of slots for one.
 //
 // Few long sequences do not fill the chip with B * D / 64 waves: the time axis is cut into chunks (urnn_scan_chunks).  The recurrence
 // is linear, h_end = P h_begin + S with S the state of a chunk that starts from zero and P = exp(A * sum of its steps): one pass
