@@ -57,8 +57,8 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
     const int lane = threadIdx.x;
     const int Dg = p.dim / p.G, cbs = (Dg + CB - 1) / CB;
     const int cb = blockIdx.x % (cbs * p.G), g = cb / cbs, c0 = g * Dg + (cb % cbs) * CB, cend = (g + 1) * Dg;
-    // the sequences of a chunk before the next chunk: those of a padded batch end in the same late blocks, spread over the chip
-    const int rest = blockIdx.x / (cbs * p.G), b = rest % p.batch, chunk = (BACK ? 1 : 0) + rest / p.batch;
+    const int walked = FULL ? p.chunks : p.chunks - 1;           // nothing reads the summary of the last chunk (BACK: the first)
+    const int rest = blockIdx.x / (cbs * p.G), chunk = (BACK ? 1 : 0) + rest % walked, b = rest / walked;
     const int len = __builtin_amdgcn_readfirstlane(seq_len(p.lengths, b, p.L));
     const long tb = (long)chunk * p.CL, tfull = tb + p.CL < p.L ? tb + p.CL : p.L, te = tfull < len ? tfull : len;
     const int n = te > tb ? (int)(te - tb) : 0;                  // tokens to walk; token i is first + dir i
@@ -228,10 +228,13 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
     }
 }
 
+// A launch's blocks: the chunks of a sequence, then the next sequence.  (The sequences of a chunk first, so that a padded batch's empty
+// chunks come last: 7 x 1021 x 1000 63 against 67 us, but 2 x 19 166 x 1032 359 against 333 and 12 x 3000 x 1500 277 against 257.)
+//
 // Chunks of the time axis: one from 640 waves on, where the pass over the chunks' ends would cost more than the waves it wins;
 // below that as many as give 9216 waves (three turns of the three that each of the 1024 SIMDs holds), but none shorter than 32 tokens.
 // Measured with 3000 waves of 64 tokens at least and with 9216 of 32: 32 768 tokens of 2048 channels 483 and 462 us (12 288: 476), seven
-// sequences of up to 1021 tokens of 1000 channels 72 and 67 us, forward and backward of 4 x 2048 x 2048 491 and 492 us.
+// sequences of up to 1021 tokens of 1000 channels 72 and 67 us.
 int urnn_scan_chunks(int B, int L, int D, int *CL)
 {
     const long waves = (long)B * ((D + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
