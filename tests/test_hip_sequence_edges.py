@@ -1,0 +1,38 @@
+"""The sequence operators at the edges of what their documentation allows: parameters at the ends of float32, buffers in unusual places,
+sizes near the limits of a launch.  Bounds on errors are those of seq_bounds."""
+import pytest
+import torch
+
+import seq_bounds
+from test_hip_sequence import make, rng, scan_case
+from urnn_amd import ops, train_ops
+
+gpu = pytest.mark.gpu
+GRADS = ("du", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias", "dstate")
+WIDE = ("dA", "dD", "ddelta_bias", "dstate")
+
+
+def scan_gradients(c, dout, lengths=None, dstate_out=None):
+    ws = ops.selective_scan_workspace(c["u"], c["A"])
+    y, st = ops.selective_scan(**c, lengths=lengths, ws=ws, want_state=True)
+    got = train_ops.selective_scan_backward(**{k: v for k, v in c.items() if k != "state"}, dout=dout, fwd_ws=ws, lengths=lengths,
+                                            dstate_out=dstate_out, want_dstate=True)
+    return {"y": y, "state": st, **got}
+
+
+# ---- the scan's A at the ends of float32 -----------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("L,dim,N,G", [(70, 20, 4, 1), (9, 20, 16, 1), (130, 10, 32, 1), (5, 7, 64, 1), (40, 24, 8, 4)])
+def test_selective_scan_backward_where_states_die_at_once(L, dim, N, G, dtype):
+    """A = -inf in one state of every channel, in blocks that their channels do not fill: every gradient is finite, that of the other
+    states as well.  The reference takes -1e30, whose decay is zero too (steps are above 1e-4 here)."""
+    c, _ = scan_case(2, L, dim, N, G, dtype, L + N)
+    dout, dso = make(rng(3), 2, L, dim, dtype=dtype), make(rng(4), 2, dim, N)
+    finite = c["A"].clone()
+    finite[:, 1] = -1e30
+    ref = seq_bounds.selective_scan(**{**c, "A": finite}, dout=dout, dstate_out=dso, reach=64, chain=2 * L)
+    c["A"][:, 1] = float("-inf")
+    got = scan_gradients(c, dout, dstate_out=dso)
+    for k in ("y", "state", *GRADS):
+        seq_bounds.check(got[k], ref[k], torch.float32 if k in WIDE or k == "state" else dtype, k)
