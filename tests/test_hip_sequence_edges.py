@@ -36,3 +36,23 @@ def test_selective_scan_backward_where_states_die_at_once(L, dim, N, G, dtype):
     got = scan_gradients(c, dout, dstate_out=dso)
     for k in ("y", "state", *GRADS):
         seq_bounds.check(got[k], ref[k], torch.float32 if k in WIDE or k == "state" else dtype, k)
+
+
+@gpu
+@pytest.mark.parametrize("N", [4, 16, 32])
+def test_selective_scan_largest_decay_rate_at_steps_of_zero(N):
+    """A = -(largest float32) and steps that are exactly zero (softplus(-200)) between others: exp(0 A) = 1, the state stays.  Its gradients
+    likewise; those of the steps are a product of |A| with sums that float32 does not hold, and are not looked at."""
+    c, _ = scan_case(2, 70, 20, N, 1, torch.float32, N, bias=False)
+    c["A"][:, 0] = -torch.finfo(torch.float32).max
+    c["delta"][:, 1:40] = -200.0                               # one token of decay first; whole chunks of zero steps behind it
+    c["delta"][1] = -200.0                                     # no step at all in the second sequence
+    dout, dso = make(rng(3), 2, 70, 20), make(rng(4), 2, 20, N)
+    ref = seq_bounds.selective_scan(**c, dout=dout, dstate_out=dso, reach=64, chain=140)
+    got = scan_gradients(c, dout, dstate_out=dso)
+    for k in ("y", "state", "du", "dz", "dB", "dC", "dD", "dstate"):
+        seq_bounds.check(got[k], ref[k], torch.float32, k)
+    h = c["state"]                                             # and token by token
+    for t in range(3):
+        y, h = ops.selective_scan_step(**{**c, **{k: c[k][:, t] for k in ("u", "delta", "B", "C", "z")}, "state": h})
+        seq_bounds.check(y, tuple(v[:, t] for v in ref["y"]), torch.float32, "step y")

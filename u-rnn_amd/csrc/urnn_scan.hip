@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64, 2) void scan_kernel(const ScanParams p)
     f32x4 h[NP / 4];
     load_states<NP>(p.A + (long)ch * p.N, 0, p.N, states_vec(p.A, p.N, 4), A2);
 #pragma unroll
-    for (int k = 0; k < NP; ++k) { A2[k] *= URNN_LOG2E; h0[k] = 0.0f; }
+    for (int k = 0; k < NP; ++k) { A2[k] = a_log2(A2[k]); h0[k] = 0.0f; }
     if (FULL && chunk > 0) load_states<NP>(p.S + (((long)b * p.chunks + chunk - 1) * p.dim + ch) * NP, 0, NP, true, h0);
     else if (!BACK && p.state && chunk == 0) load_states<NP>(p.state + ((long)b * p.dim + ch) * p.N, 0, p.N, states_vec(p.state, p.N, 4), h0);
 #pragma unroll
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
     if (i >= count) return;
     const long b = i / ((long)dim * NP), r = i % ((long)dim * NP);
     const int d = (int)(r / NP), n = (int)(r % NP);
-    const float A2 = n < N ? A[(long)d * N + n] * URNN_LOG2E : 0.0f;
+    const float A2 = n < N ? a_log2(A[(long)d * N + n]) : 0.0f;
     float *s = S + b * chunks * dim * NP + r;
     const float *w = sum + b * chunks * dim + d;
     float h = s[0];

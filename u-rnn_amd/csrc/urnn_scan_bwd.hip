@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void scan_back_carry_kernel(const float *__res
     if (i >= count) return;
     const long b = i / ((long)dim * NP), r = i % ((long)dim * NP);
     const int d = (int)(r / NP), n = (int)(r % NP);
-    const float A2 = n < N ? A[(long)d * N + n] * URNN_LOG2E : 0.0f;
+    const float A2 = n < N ? a_log2(A[(long)d * N + n]) : 0.0f;
     float *s = S + b * chunks * dim * NP + r;
     const float *w = sum + b * chunks * dim + d;
     float k = dstate_out && n < N ? dstate_out[(b * dim + d) * N + n] : 0.0f;
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256, NP <= 8 ? 3 : 2) void scan_backward_kernel(con
         load_states<E>(p.A + (long)sch[k] * p.N, q, p.N, states_vec(p.A, p.N, W), A2[k]);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            A2[k][e] = sok[k] ? A2[k][e] * URNN_LOG2E : 0.0f;                // not a product with 0: A may be -inf
+            A2[k][e] = sok[k] ? a_log2(A2[k][e]) : 0.0f;                     // not a product with 0: A may be -inf
             A2[k][e] = A2[k][e] < -3.0e38f ? -3.0e38f : A2[k][e];            // 0 * A2 stays 0: a step of 0 keeps the state
             dA[k][e] = 0.0f;
         }

@@ -33,6 +33,14 @@ __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp
 __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x)); }
 __device__ __forceinline__ float silu_f(float x) { return x * sigmoid_f(x); }
 
+// The scan's A for decays as powers of two.  The product of a finite A beyond 2.36e38 leaves float32: it is held at the largest float, so that
+// a step of 0 keeps the state (0 inf would be NaN).  An A that is infinite itself stays so.
+__device__ __forceinline__ float a_log2(float A)
+{
+    const float a = A * URNN_LOG2E;
+    return fabsf(A) <= __FLT_MAX__ ? fminf(fmaxf(a, -__FLT_MAX__), __FLT_MAX__) : a;
+}
+
 // softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1].  log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the series
 // 2 s (1 + s^2/3 + s^4/5 + ...) to s^12/13 leaves 1.4e-8 of the value, and keeps full relative accuracy where e is tiny (a step of
 // exp(x) for x << 0), which log(1 + e) loses.
