@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import seq_bounds
-from test_hip_sequence import make, rng, scan_case
+from test_hip_sequence import make, refused, rng, scan_case
 from urnn_amd import ops, train_ops
 
 gpu = pytest.mark.gpu
@@ -56,3 +56,12 @@ def test_selective_scan_largest_decay_rate_at_steps_of_zero(N):
     for t in range(3):
         y, h = ops.selective_scan_step(**{**c, **{k: c[k][:, t] for k in ("u", "delta", "B", "C", "z")}, "state": h})
         seq_bounds.check(y, tuple(v[:, t] for v in ref["y"]), torch.float32, "step y")
+
+
+# ---- refusals (no GPU) ----------------------------------------------------------------------------------------------------------
+def test_conv_gradients_without_a_bias_take_no_buffer_for_one():
+    """A dbias in grads (of another layer, of any size) is neither written nor handed back as a gradient."""
+    x, w = torch.zeros(2, 5, 8), torch.zeros(8, 4)
+    for buf in (torch.zeros(8), torch.zeros(3), torch.zeros(8, dtype=torch.bfloat16)):
+        refused("dbias in grads, but there is no bias", train_ops.causal_conv_backward, x, w, x, grads={"dbias": buf})
+    refused("no CPU path", train_ops.causal_conv_backward, x, w, x, grads={"dbias": None})     # what a call without one leaves

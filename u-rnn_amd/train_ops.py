@@ -190,9 +190,13 @@ def adam_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.9
 
 
 # ---- sequence operators (ops.causal_conv, ops.selective_scan, ops.norm_residual) --------------------------------------------
-def _param_grads_check(what, grads, accumulate, params, inputs):
-    """-> (the dict that receives the gradients, the buffers in it that the caller gave: apart from the inputs and from one another)."""
+def _param_grads_check(what, grads, accumulate, params, inputs, absent=()):
+    """-> (the dict that receives the gradients, the buffers in it that the caller gave: apart from the inputs and from one another).
+    ``absent``: gradients of parameters that this call does not have; a buffer for one would come back as if it were a gradient."""
     g = {} if grads is None else grads
+    for k in absent:
+        if g.get(k) is not None:
+            raise RuntimeError(f"{what}: {k} in grads, but there is no {k[1:]}")
     if accumulate and any(g.get(k) is None for k in params):
         raise RuntimeError(f"{what}: accumulate needs the gradients {sorted(params)} in grads")
     given = [g[k] for k in params if g.get(k) is not None]
@@ -219,7 +223,7 @@ def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, s
                          scratch=None):
     """Backward of ``ops.causal_conv`` given dout (B,L,D) and, where the returned state was used further, ``dstate_out`` (B,K-1,D).
     Returns a dict: dx, dstate (None without state), dweight, dbias (None without bias); parameter gradients are float32, into the buffers
-    of ``grads`` if given, added to them with ``accumulate``."""
+    of ``grads`` if given, added to them with ``accumulate``; a buffer for a parameter that the call does not have is refused."""
     what = "causal_conv_backward"
     dt = ops._seq_dtype(what, x)
     if x.dim() != 3:
@@ -232,7 +236,7 @@ def causal_conv_backward(x, weight, dout, bias=None, state=None, lengths=None, s
         ops._seq_check(what, "dstate_out", dstate_out, (B, K - 1, D), x.dtype, contiguous=True)
     params = {"dweight": weight, **({"dbias": bias} if bias is not None else {})}
     inputs = (x, weight, dout, bias, state, lengths, dstate_out)
-    g, given = _param_grads_check(what, grads, accumulate, params, inputs)
+    g, given = _param_grads_check(what, grads, accumulate, params, inputs, absent=("dbias",) if bias is None else ())
     stream = ops._seq_device(what, *inputs, *given)
     L_ = lib()
     _param_grads(g, params)
