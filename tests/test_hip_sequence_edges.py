@@ -65,3 +65,16 @@ def test_conv_gradients_without_a_bias_take_no_buffer_for_one():
     for buf in (torch.zeros(8), torch.zeros(3), torch.zeros(8, dtype=torch.bfloat16)):
         refused("dbias in grads, but there is no bias", train_ops.causal_conv_backward, x, w, x, grads={"dbias": buf})
     refused("no CPU path", train_ops.causal_conv_backward, x, w, x, grads={"dbias": None})     # what a call without one leaves
+
+
+def test_gradients_of_absent_parameters_are_not_handed_back():
+    """grads of a call with more parameters: what they hold is no gradient of this call."""
+    c, _ = scan_case(2, 5, 8, 4, 2, torch.float32, 0, bias=False, skip=False, dev="cpu")
+    back = {k: v for k, v in c.items() if k != "state"}
+    ws, v, y = torch.zeros(1 << 16, dtype=torch.uint8), torch.zeros(8), torch.zeros(3, 8)
+    refused("dD in grads, but there is no D", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, grads={"dD": v})
+    refused("ddelta_bias in grads, but there is no delta_bias", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, grads={"ddelta_bias": v})
+    refused("no CPU path", train_ops.selective_scan_backward, **back, dout=c["u"], fwd_ws=ws, grads={"dD": None, "ddelta_bias": None})
+    refused("dpost_w in grads, but there is no post_w", train_ops.norm_residual_backward, y, v, y, scale=v, grads={"dpost_w": v})
+    refused("dscale in grads, but there is no scale", train_ops.norm_residual_backward, y, v, y, post_w=v, grads={"dscale": v})
+    refused("no CPU path", train_ops.norm_residual_backward, y, v, y, grads={"dscale": None, "dpost_w": None})

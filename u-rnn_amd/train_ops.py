@@ -274,7 +274,7 @@ def norm_residual_backward(y, pre_w, dnormed, dresidual_out=None, residual=None,
     every = {"dpre_w": pre_w, "dpost_w": post_w, "dscale": scale}
     params = {k: w for k, w in every.items() if w is not None}
     inputs = (y, pre_w, dnormed, dresidual_out, residual, post_w, gate, scale)
-    g, given = _param_grads_check(what, grads, accumulate, params, inputs)
+    g, given = _param_grads_check(what, grads, accumulate, params, inputs, absent=every.keys() - params)
     stream = ops._seq_device(what, *inputs, *given)
     L_ = lib()
     _param_grads(g, params)
@@ -312,13 +312,10 @@ def selective_scan_backward(u, delta, A, B, C, dout, fwd_ws, D=None, z=None, del
         ops._seq_check(what, "dstate_out", dstate_out, (nb, dim, N), torch.float32, contiguous=True)
     if fwd_ws is None:
         raise RuntimeError(f"{what}: fwd_ws is None: run the forward with ws=ops.selective_scan_workspace(u, A)")
-    params = {"dA": A}
-    if D is not None:
-        params["dD"] = D
-    if delta_bias is not None:
-        params["ddelta_bias"] = delta_bias
+    every = {"dA": A, "dD": D, "ddelta_bias": delta_bias}
+    params = {k: w for k, w in every.items() if w is not None}
     inputs = (u, delta, A, B, C, D, z, delta_bias, dout, lengths, dstate_out)
-    g, given = _param_grads_check(what, grads, accumulate, params, inputs)
+    g, given = _param_grads_check(what, grads, accumulate, params, inputs, absent=every.keys() - params)
     L_ = lib()
     record = ops._seq_buffer(what, "fwd_ws", fwd_ws, L_.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1), given)
     stream = ops._seq_device(what, *inputs, *given, record)
