@@ -78,3 +78,13 @@ def test_gradients_of_absent_parameters_are_not_handed_back():
     refused("dpost_w in grads, but there is no post_w", train_ops.norm_residual_backward, y, v, y, scale=v, grads={"dpost_w": v})
     refused("dscale in grads, but there is no scale", train_ops.norm_residual_backward, y, v, y, post_w=v, grads={"dscale": v})
     refused("no CPU path", train_ops.norm_residual_backward, y, v, y, grads={"dscale": None, "dpost_w": None})
+
+
+def test_norm_outputs_apart_from_the_parameters():
+    """An output over a weight would be read by rows that are not done yet."""
+    y, both = torch.zeros(4, 8), torch.zeros(6, 8)
+    for name in ("pre_w", "post_w", "scale"):
+        par = {"pre_w": torch.ones(8), name: both[4]}
+        refused("out overlaps an input", ops.norm_residual, y, out=both[2:], **par)
+        refused("residual_out overlaps an input", ops.norm_residual, y, residual_out=both[1:5], **par)
+        refused("no CPU path", ops.norm_residual, y, out=both[:4], **par)

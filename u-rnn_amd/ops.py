@@ -818,11 +818,11 @@ def norm_residual(y, pre_w, residual=None, post_w=None, gate=None, scale=None, g
     what = "norm_residual"
     dt = _seq_dtype(what, y)
     strides = _norm_check(what, y, pre_w, residual, post_w, gate, scale, gate_act)
-    shape, inputs = tuple(y.shape), (y, residual, gate)
+    shape, rows_in, inputs = tuple(y.shape), (y, residual, gate), (y, residual, gate, pre_w, post_w, scale)
     if out is not None:
-        _seq_out(what, "out", out, shape, y.dtype, inputs + (residual_out,), same=inputs)
+        _seq_out(what, "out", out, shape, y.dtype, inputs + (residual_out,), same=rows_in)
     if residual_out is not None:
-        _seq_out(what, "residual_out", residual_out, shape, y.dtype, inputs, same=inputs)
+        _seq_out(what, "residual_out", residual_out, shape, y.dtype, inputs, same=rows_in)
     stream = _seq_device(what, y, pre_w, residual, post_w, gate, scale, out, residual_out)
     if out is None:
         out = _empty_as(y)
