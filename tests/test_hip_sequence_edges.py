@@ -88,3 +88,16 @@ def test_norm_outputs_apart_from_the_parameters():
         refused("out overlaps an input", ops.norm_residual, y, out=both[2:], **par)
         refused("residual_out overlaps an input", ops.norm_residual, y, residual_out=both[1:5], **par)
         refused("no CPU path", ops.norm_residual, y, out=both[:4], **par)
+
+
+def test_outputs_apart_from_the_lengths():
+    """lengths are read by every block until the last one is done."""
+    c, _ = scan_case(2, 5, 8, 4, 2, torch.float32, 0, dev="cpu")
+    out, st = torch.zeros(2, 5, 8), torch.zeros(2, 8, 4)
+    n, m = out.view(torch.int32)[0, 0, :2], st.view(torch.int32)[1, 7, 2:]
+    refused("out overlaps an input", ops.selective_scan, **c, lengths=n, out=out)
+    refused("state_out overlaps an input", ops.selective_scan, **c, lengths=m, want_state=True, state_out=st)
+    x, w, cs = torch.zeros(2, 5, 8), torch.zeros(8, 4), torch.zeros(2, 3, 8)
+    refused("out overlaps an input", ops.causal_conv, x, w, lengths=n, out=out)
+    refused("state_out overlaps an input", ops.causal_conv, x, w, lengths=cs.view(torch.int32)[0, 0, :2], want_state=True, state_out=cs)
+    refused("no CPU path", ops.causal_conv, x, w, lengths=n, out=torch.zeros(2, 5, 8))

@@ -600,9 +600,9 @@ def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, out=N
     D, K = _conv_seq_check(what, x, weight, bias, state, (B, L))
     _lengths_check(what, lengths, B)
     if out is not None:
-        _seq_out(what, "out", out, (B, L, D), x.dtype, (x, weight, bias, state, state_out))
+        _seq_out(what, "out", out, (B, L, D), x.dtype, (x, weight, bias, state, lengths, state_out))
     if state_out is not None:
-        _seq_out(what, "state_out", state_out, (B, K - 1, D), x.dtype, (x, weight, bias, state))
+        _seq_out(what, "state_out", state_out, (B, K - 1, D), x.dtype, (x, weight, bias, state, lengths))
     stream = _seq_device(what, x, weight, bias, state, lengths, out, state_out)
     if out is None:
         out = _empty_as(x)
@@ -707,7 +707,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     if state is not None:
         _seq_check(what, "state", state, (nb, dim, N), torch.float32, contiguous=True)
     _lengths_check(what, lengths, nb)
-    inputs = (u, delta, A, B, C, D, z, delta_bias, state)
+    inputs = (u, delta, A, B, C, D, z, delta_bias, state, lengths)
     if out is not None:
         _seq_out(what, "out", out, (nb, L, dim), u.dtype, inputs + (state_out,))
     if state_out is not None:
@@ -716,8 +716,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     keep = ws is not None
     nbytes = Lb.urnn_selective_scan_workspace_bytes(nb, L, dim, N, 1 if keep else 0)
     if keep:
-        _seq_buffer(what, "ws", ws, nbytes, inputs + (lengths, out, state_out))
-    stream = _seq_device(what, *inputs, lengths, out, state_out, ws)
+        _seq_buffer(what, "ws", ws, nbytes, inputs + (out, state_out))
+    stream = _seq_device(what, *inputs, out, state_out, ws)
     if nbytes and not keep:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=u.device)
     if out is None:
