@@ -101,3 +101,15 @@ def test_outputs_apart_from_the_lengths():
     refused("out overlaps an input", ops.causal_conv, x, w, lengths=n, out=out)
     refused("state_out overlaps an input", ops.causal_conv, x, w, lengths=cs.view(torch.int32)[0, 0, :2], want_state=True, state_out=cs)
     refused("no CPU path", ops.causal_conv, x, w, lengths=n, out=torch.zeros(2, 5, 8))
+
+
+def test_an_arena_of_another_device_is_refused(monkeypatch):
+    """A backward's scratch from an Arena is looked at like a buffer of the caller's."""
+    class Input:                                               # stands for a tensor on the current device
+        is_cuda, device = True, torch.device("cuda:0")
+
+        def get_device(self):
+            return 0
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    refused("op: .* GPU", train_ops._seq_scratch, "op", ops.Arena("cpu"), 64, torch.device("cuda:0"), (Input(),))

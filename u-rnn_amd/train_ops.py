@@ -256,8 +256,9 @@ def _seq_scratch(what, scratch, nbytes, dev, others):
     if scratch is None:
         return torch.empty(int(nbytes), dtype=torch.uint8, device=dev)
     if isinstance(scratch, ops.Arena):
-        return _bwd_scratch(scratch, nbytes, dev)
-    ops._seq_buffer(what, "scratch", scratch, nbytes, others)
+        scratch = _bwd_scratch(scratch, nbytes, dev)
+    else:
+        ops._seq_buffer(what, "scratch", scratch, nbytes, others)
     ops._seq_device(what, others[0], scratch)
     return scratch
 
