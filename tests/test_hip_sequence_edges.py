@@ -113,3 +113,50 @@ def test_an_arena_of_another_device_is_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     refused("op: .* GPU", train_ops._seq_scratch, "op", ops.Arena("cpu"), 64, torch.device("cuda:0"), (Input(),))
+
+
+# ---- sizes near the limits of a launch -------------------------------------------------------------------------------------------
+def test_scan_limits_are_those_of_its_launches():
+    """Waves of 64 channels of a group: fewer than 2^26 (2^32 threads); a token: four threads to a channel.  Sizes that pass go on to the
+    NULL check (-2), the others are refused (-1)."""
+    from urnn_amd._lib import lib
+    L = lib()
+
+    def prompt(B, D, G=1):
+        return L.urnn_selective_scan(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, B, 2, D, G, 4, 1, 0)
+
+    def token(B, D, G=1):
+        return L.urnn_selective_scan_step(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, B, D, G, 4, 1, 0)
+
+    for inside, outside in (((4194305, 24), (1 << 26, 24)), (((1 << 26) - 1, 1), (1 << 26, 1)), (((1 << 25) - 1, 65), (1 << 25, 65)),
+                            ((63, 1 << 20, 1 << 20), (64, 1 << 20, 1 << 20)), ((1, (1 << 30) - 64), (1, (1 << 30) - 63))):
+        assert prompt(*inside) == -2, inside
+        assert prompt(*outside) == -1 and b"one launch" in L.urnn_last_error(), outside
+    for inside, outside in (((4194305, 24), (1 << 26, 24)), (((1 << 30) - 64, 1), ((1 << 30) - 63, 1)), ((1, (1 << 30) - 64), (1, (1 << 30) - 63))):
+        assert token(*inside) == -2, inside
+        assert token(*outside) == -1 and b"one launch" in L.urnn_last_error(), outside
+
+
+@gpu
+def test_scan_of_four_million_short_sequences():
+    """As many waves as sequences: the results are those of the batch's parts, bit for bit."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB")
+    B, L, D, N = 4194305, 2, 24, 4
+    g = torch.Generator(device="cuda").manual_seed(3)
+    t = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=torch.bfloat16)      # noqa: E731
+    c = {"u": t(B, L, D), "delta": t(B, L, D), "B": t(B, L, N), "C": t(B, L, N), "z": t(B, L, D)}
+    par = {"A": -torch.rand(D, N, generator=g, device="cuda"), "D": torch.ones(D, device="cuda")}
+    state, dout = torch.randn(B, D, N, generator=g, device="cuda"), t(B, L, D)
+    got = scan_gradients({**c, **par, "state": state}, dout)
+    y, st = ops.selective_scan_step(**{k: v[:, 0] for k, v in c.items()}, **par, state=state)
+    for lo in range(0, B, 1 << 20):
+        cut = slice(lo, min(lo + (1 << 20), B))
+        part = {k: v[cut] for k, v in c.items()}
+        want = scan_gradients({**part, **par, "state": state[cut]}, dout[cut])
+        for k in ("y", "state", "du", "ddelta", "dz", "dB", "dC", "dstate"):
+            assert torch.equal(got[k][cut], want[k]), (k, lo)
+        yw, sw = ops.selective_scan_step(**{k: v[:, 0] for k, v in part.items()}, **par, state=state[cut])
+        assert torch.equal(y[cut], yw) and torch.equal(st[cut], sw), lo
+    assert all(torch.isfinite(got[k]).all() for k in ("dA", "dD"))

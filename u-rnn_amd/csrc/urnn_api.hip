@@ -1612,14 +1612,16 @@ extern "C" int urnn_causal_conv_backward(const void *x, long x_batch, long x_tok
     return URNN_OK;
 }
 
-static int scan_args(const char *what, int dtype, long B, long L, long D, long G, long N)
+// Fewer than 2^32 threads: a prompt has a wave for 64 channels of a group of a sequence (one that is cut into chunks has few of them, and
+// the backward fewer still), a token four threads for a channel.  Offsets in a row are of 32 bits.
+static int scan_args(const char *what, int dtype, long B, long L, long D, long G, long N, bool token = false)
 {
     if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
     if (B < 1 || L < 1 || D < 1) return fail(URNN_EINVAL, "%s: B=%ld L=%ld D=%ld", what, B, L, D);
     if (G < 1 || D % G) return fail(URNN_EINVAL, "%s: G=%ld groups do not divide D=%ld channels", what, G, D);
     if (N < 1 || N > URNN_SEQ_MAX_STATES) return fail(URNN_EINVAL, "%s: N=%ld states (1..%d)", what, N, URNN_SEQ_MAX_STATES);
     const long cbs = G * ((D / G + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
-    if ((double)B * (cbs > D / 16 ? cbs : D / 16 + 1) > 8388608.0) return fail(URNN_EINVAL, "%s: B=%ld x D=%ld is beyond one launch", what, B, D);
+    if ((token ? (double)B * D > 1073741760.0 : (double)B * cbs >= 67108864.0) || D > 1073741760) return fail(URNN_EINVAL, "%s: B=%ld x D=%ld is beyond one launch", what, B, D);
     return URNN_OK;
 }
 
@@ -1738,7 +1740,7 @@ extern "C" int urnn_selective_scan_step(const void *u, const void *delta, const 
                                         const float *A, const float *skip, const float *delta_bias, const float *state, void *y, float *state_out,
                                         int dtype, int B, int D, int G, int N, int softplus, void *stream)
 {
-    const int rc = scan_args("urnn_selective_scan_step", dtype, B, 1, D, G, N);
+    const int rc = scan_args("urnn_selective_scan_step", dtype, B, 1, D, G, N, true);
     if (rc) return rc;
     if (!u || !delta || !Bmat || !Cmat || !strides || !A || !state || !y || !state_out) return fail(URNN_ENULL, "urnn_selective_scan_step: NULL argument");
     ScanParams p = {};
