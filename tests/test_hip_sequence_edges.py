@@ -160,3 +160,38 @@ def test_scan_of_four_million_short_sequences():
         yw, sw = ops.selective_scan_step(**{k: v[:, 0] for k, v in part.items()}, **par, state=state[cut])
         assert torch.equal(y[cut], yw) and torch.equal(st[cut], sw), lo
     assert all(torch.isfinite(got[k]).all() for k in ("dA", "dD"))
+
+
+def test_norm_limits_are_those_of_its_launches():
+    """Blocks of 256 threads and up, a row to 16 .. 1024 of them by its width: fewer than 2^32 threads.  Sizes that pass go on to the NULL
+    check of the outputs (-2)."""
+    from urnn_amd._lib import lib
+    L = lib()
+    strides = (__import__("ctypes").c_long * 10)()
+    for D, rows in ((1, (1 << 28) - 16), (128, (1 << 28) - 16), (129, (1 << 26) - 4), (512, (1 << 26) - 4), (513, (1 << 25) - 2), (1025, (1 << 24) - 1),
+                    (2048, (1 << 24) - 1), (2049, (1 << 23) - 1), (4096, (1 << 23) - 1), (4097, (1 << 22) - 1), (16384, (1 << 22) - 1)):
+        for n, code in ((rows, -2), (rows + 1, -1)):
+            assert L.urnn_norm_residual(16, 0, 0, strides, 16, 0, 0, 0, 0, 0, n, n, D, 0, 1e-5, 0) == code, (D, n)
+            assert L.urnn_norm_residual_backward(16, 0, 0, 0, 0, strides, 16, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, n, n, D, 0, 1e-5, 0, 0) == code, (D, n)
+        assert b"one launch" in L.urnn_last_error()
+
+
+@gpu
+def test_norms_of_nine_million_rows():
+    """The results are those of the rows' parts, bit for bit."""
+    M, D = 9000001, 24
+    g = torch.Generator(device="cuda").manual_seed(3)
+    t = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=torch.bfloat16)      # noqa: E731
+    c, w = {"y": t(M, D), "residual": t(M, D), "gate": t(M, D)}, torch.rand(3, D, generator=g, device="cuda")
+    par, dn = {"pre_w": w[0], "post_w": w[1], "scale": w[2]}, t(M, D)
+    n, r = ops.norm_residual(**c, **par)
+    got = train_ops.norm_residual_backward(dnormed=dn, **c, **par)
+    for lo in range(0, M, 1 << 22):
+        cut = slice(lo, min(lo + (1 << 22), M))
+        part = {k: v[cut] for k, v in c.items()}
+        nw, rw = ops.norm_residual(**part, **par)
+        want = train_ops.norm_residual_backward(dnormed=dn[cut], **part, **par)
+        assert torch.equal(n[cut], nw) and torch.equal(r[cut], rw), lo
+        for k in ("dy", "dgate", "dresidual"):
+            assert torch.equal(got[k][cut], want[k]), (k, lo)
+    assert all(torch.isfinite(got[k]).all() for k in ("dpre_w", "dpost_w", "dscale"))

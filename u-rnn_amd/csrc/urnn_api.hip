@@ -1756,8 +1756,8 @@ static int norm_args(const char *what, const void *y, const long *strides, const
 {
     if (!y || !strides || !pre_w) return fail(URNN_ENULL, "%s: NULL argument", what);
     if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
-    if (rows < 1 || rows > 8388608 || D < 1 || D > URNN_SEQ_MAX_NORM) return fail(URNN_EINVAL, "%s: rows=%ld (1..8388608) D=%d (1..%d)", what, rows, D, URNN_SEQ_MAX_NORM);
-    if ((D > 4096 && rows > 4194303) || (D > 2048 && rows > 8388607)) return fail(URNN_EINVAL, "%s: rows=%ld of D=%d are beyond one launch", what, rows, D);
+    if (rows < 1 || D < 1 || D > URNN_SEQ_MAX_NORM) return fail(URNN_EINVAL, "%s: rows=%ld D=%d (1..%d)", what, rows, D, URNN_SEQ_MAX_NORM);
+    if (urnn_norm_threads(rows, D) >= 4294967296.0) return fail(URNN_EINVAL, "%s: rows=%ld of D=%d are beyond one launch", what, rows, D);
     if (inner < 1 || inner > rows || rows % inner) return fail(URNN_EINVAL, "%s: %ld rows of %ld each", what, rows, inner);
     if (act < URNN_GATE_NONE || act > URNN_GATE_SILU) return fail(URNN_EINVAL, "%s: act=%d", what, act);
     return URNN_OK;

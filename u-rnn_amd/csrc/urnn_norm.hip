@@ -62,7 +62,7 @@ __device__ __forceinline__ void gate_of(int act, float g, float &a, float &da)
 template <typename T>
 __device__ __forceinline__ const T *row_at(const void *base, const SeqStride &s, long row, unsigned inner)
 {
-    const unsigned r = (unsigned)row;                // at most 2^23 rows
+    const unsigned r = (unsigned)row;                // fewer than 2^28 rows
     return reinterpret_cast<const T *>(base) + (long)(r / inner) * s.b + (long)(r % inner) * s.t;
 }
 // WIDE: rows start on 16 bytes and hold whole groups; otherwise a row holds one group at least (or V is 1).
@@ -304,6 +304,11 @@ hipError_t urnn_launch_sum_parts(const float *src, int parts, const long (&n)[3]
 }
 
 static int row_threads(int D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+double urnn_norm_threads(long rows, int D)
+{
+    const int nt = row_threads(D), rb = nt < 256 ? 256 / nt : 1;
+    return (double)((rows - 1) / rb + 1) * (nt * rb);
+}
 int urnn_norm_parts(long rows, int D)
 {
     const int nt = row_threads(D), rb = nt < 256 ? 256 / nt : 1;

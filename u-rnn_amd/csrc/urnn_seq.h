@@ -269,6 +269,7 @@ struct NormParams {
 hipError_t urnn_launch_norm(const NormParams &p, int dtype, bool wide, hipStream_t st);
 hipError_t urnn_launch_norm_backward(const NormParams &p, int dtype, bool wide, float *dpre, float *dpost, float *dscale, int accumulate, hipStream_t st);
 int urnn_norm_parts(long rows, int D);
+double urnn_norm_threads(long rows, int D);          // of a forward launch
 
 // src [parts][n[0] + n[1] + n[2]] -> out[k] (+)= the sums over parts of its columns; out[k] may be NULL.  In double, in a fixed order.
 hipError_t urnn_launch_sum_parts(const float *src, int parts, const long (&n)[3], float *const (&out)[3], int accumulate, hipStream_t st);
