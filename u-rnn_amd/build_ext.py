@@ -62,9 +62,18 @@ def build(force=False, verbose=False, extra_flags=(), out=None, tag=""):
         with open(stamp, "w") as f:
             f.write(line)
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
+    # ... and the library is left alone if no unit was rebuilt, it is newer than its objects and it was linked by this command line
+    stamp = LIB + ".cmd"
+    same_cmd = os.path.isfile(stamp) and open(stamp).read() == " ".join(cmd)
+    if not procs and same_cmd and os.path.isfile(LIB) and os.path.getmtime(LIB) >= _newest(objs):
+        return LIB
     if verbose:
         print(" ".join(cmd))
+    if os.path.isfile(stamp):
+        os.remove(stamp)
     subprocess.run(cmd, check=True)
+    with open(stamp, "w") as f:
+        f.write(" ".join(cmd))
     return LIB
 
 
