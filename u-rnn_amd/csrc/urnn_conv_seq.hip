@@ -6,7 +6,8 @@
 // Memory-bound: one read of x, one write of y.  A thread holds V adjacent channels (16 bytes) and walks T tokens with the last
 // K - 1 inputs in registers, so that an input is read once but for the K - 1 rows before a chunk; threads of a wave are adjacent in
 // the channels.  V = 1 where rows are not 16-byte aligned.  2 x 4096 x 4096 bf16: 26.4 us, 5.1 TB/s, what a copy of those bytes
-// takes; 6 x 1531 x 1001 fp32 (no row aligned, padded): 12.6 us, with the backward and its sums 44 us, 3.3 TB/s.
+// takes; 6 x 1531 x 1001 fp32 (no row aligned, padded): 12.6 us, with the backward and its sums 44 to 48 us from box to
+// box, about 3 TB/s.
 #include "urnn_seq.h"
 
 #include <type_traits>

@@ -14,14 +14,15 @@
 // elementwise part or pass it on through LDS: the full pass over 32 768 x 2048 took 417 us then and 359 with a lane, at that step.)
 //
 // What bounds it is the vector unit: per state one exponential (measured: the time of 1.6 to 2 fp32 operations) and three fp32
-// operations, per token and channel about 45 more: 119 issue slots at 16 states, 35e12 lane-slots/s of the chip.  4 x 2048 x 2048 bf16:
-// 93 us of 56 us of slots (waves at two to a SIMD wait for their loads and for the chain of a state from token to token), 1.5 TB/s;
-// 32 768 x 2048 460 us with both passes, of 226 us of slots for one.
+// operations, per token and channel about 45 more: 119 issue slots at 16 states, 35e12 lane-slots/s of the chip (by the counters 114
+// instructions, 20 of them exponentials or reciprocals).  4 x 2048 x 2048 bf16: 92 us of 56 us of slots, the vector unit busy in 63 % of
+// the cycles (waves at two to a SIMD wait for their loads and for the chain of a state from token to token), 1.5 TB/s; 32 768 x 2048
+// 460 us with both passes, busy 84 and 89 %, of 226 us of slots for one.
 //
 // Few long sequences do not fill the chip with B * D / 64 waves: the time axis is cut into chunks (urnn_scan_chunks).  The recurrence
 // is linear, h_end = P h_begin + S with S the state of a chunk that starts from zero and P = exp(A * sum of its steps): one pass
 // leaves (S, sum of steps) of every chunk, a short kernel carries the states over the chunks, and the full pass starts each chunk
-// from its true state.  The first pass costs the exponentials once more (32 768 x 2048: 222 us next to the full pass's 286).  The same
+// from its true state.  The first pass costs the exponentials once more (32 768 x 2048: 222 us next to the full pass's 285).  The same
 // kernel, run from the last token to the first, gives the backward its chunk summaries.
 #include "urnn_seq.h"
 
@@ -231,10 +232,13 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(const float *__restrict
 // A launch's blocks: the chunks of a sequence, then the next sequence.  (The sequences of a chunk first, so that a padded batch's empty
 // chunks come last: 7 x 1021 x 1000 63 against 67 us, but 2 x 19 166 x 1032 359 against 333 and 12 x 3000 x 1500 277 against 257.)
 //
-// Chunks of the time axis: one from 640 waves on, where the pass over the chunks' ends would cost more than the waves it wins;
-// below that as many as give 9216 waves (three turns of the three that each of the 1024 SIMDs holds), but none shorter than 32 tokens.
-// Measured with 3000 waves of 64 tokens at least and with 9216 of 32: 32 768 tokens of 2048 channels 483 and 462 us (12 288: 476), seven
-// sequences of up to 1021 tokens of 1000 channels 72 and 67 us.
+// Chunks of the time axis: one from 640 waves on, below that as many as give 9216 waves (three turns of the three that each of the 1024
+// SIMDs holds), but none shorter than 32 tokens.  The border, sequences of 2048 tokens bf16 cut and in one chunk: 128 waves 145 and 659 us,
+// 320 301 and 680, 608 530 and 684, 640 572 and 684, 896 778 and 696 -- the two meet near 800, so that between 640 and there one chunk
+// loses up to a sixth.  Waves are counted as of one group: several narrow groups launch more of them than the rule knows of.
+// The number, measured with 3000 waves of 64 tokens at least and with 9216 of 32: 32 768 tokens of 2048 channels 483 and 462 us (12 288:
+// 476), seven sequences of up to 1021 tokens of 1000 channels 72 and 67; a training step of 4 x 2048 x 2048, whose forward takes the same
+// chunks, loses by it: 482 and 495.
 int urnn_scan_chunks(int B, int L, int D, int *CL)
 {
     const long waves = (long)B * ((D + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
@@ -271,7 +275,7 @@ static hipError_t launch_scan(const ScanParams &p, hipStream_t st)
 // One token: state and inputs are read once, the new state and y written once.  A quad per channel, no LDS; a thread takes the same
 // channel of R sequences, so that their loads are in flight together and A, bias and skip are read once for them.  state_out may be
 // state: every thread reads its own states before it writes them.  Memory-bound: 256 x 4096 channels of 16 states 29.6 us, 4.8 TB/s;
-// one sequence of 192 channels 3 us, and 14 for the call.
+// one sequence of 192 channels 3 us, and 13 for the call.
 template <typename T, int E>
 __device__ __forceinline__ void load_row(const T *row, int q, int N, bool vec, float (&v)[E])
 {

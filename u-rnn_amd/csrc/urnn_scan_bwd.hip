@@ -13,16 +13,18 @@
 // exponentials of one half twice (both halves' values would not leave room for two waves).  A quad holds a channel's states, E = N / 4 to a
 // lane; a lane holds ED = 2 channels (one from 32 states on), so that the two sums of different kind cost little: over the states, two
 // DPP adds per channel and sum; over the channels (dB, dC), first in the lane, then by halving over the wave -- v_permlane32_swap and
-// v_permlane16_swap move two values and add them in one go -- and by two DPP adds: about two issue slots per state against ~17 for the
-// rest.  Blocks of one to four waves, as the channels of a group divide into waves of 16 ED, add their waves' sums through LDS; where a
-// group takes several blocks they leave partial rows in fp32, which a last kernel adds in a fixed order: no atomics.
+// v_permlane16_swap move two values and add them in one go -- and by two DPP adds: about two issue slots per state.  Blocks of one to four
+// waves, as the channels of a group divide into waves of 16 ED, add their waves' sums through LDS; where a group takes several blocks they
+// leave partial rows in fp32, which a last kernel adds in a fixed order: no atomics.
 //
 // Few sequences: the time axis is cut into chunks as in the forward; a first pass leaves what a chunk hands to the left when nothing
 // comes from its right (k' = a_first (..)), and the sum of its steps; a short kernel carries it over the chunks.
 //
-// What bounds it is the issue of the vector unit: 4 x 2048 x 2048 of 16 states bf16 270 us with the unit busy 97 % of them, of 490 us
-// for a whole training step.  15 625 sequences of 12 tokens and 96 channels of 8 states fp32: 277 us, the unit busy 46 %, 1.3 TB/s; blocks of
-// three waves leave one SIMD in four without work there.
+// What bounds it is first the issue of the vector unit: 4 x 2048 x 2048 of 16 states bf16 280 us with the unit busy in 77 % of the cycles, of
+// 493 us for a whole training step.  26.4 vector instructions per state of 64 channels, where the formulas above have 13.6 operations: 9.2
+// fma, 6.1 products, 3.4 sums, 2.0 exponentials (one half's twice, and the elementwise work's), 5.6 lane swaps, selects, conversions and
+// moves.  The rest are two waves to a SIMD that wait for each other's LDS rows and for chains.  15 625 sequences of 12 tokens and 96 channels
+// of 8 states fp32: 277 to 285 us, the unit busy 46 %, 1.3 TB/s; blocks of three waves leave one SIMD in four without work there.
 #include "urnn_seq.h"
 
 #include <type_traits>
