@@ -441,7 +441,8 @@ int urnn_step_f32(const urnn_net_f32 *net, const float *x_t, float *const states
  * No atomics: the same inputs give the same bits.  In-place: only where stated.  Sizes that one launch does not hold (2^32 threads) are
  * refused with URNN_EINVAL: norms of 2^28 rows up to D = 128, 2^26 up to 512, 2^25 up to 1024, 2^24 up to 2048, 2^23 up to 4096 and 2^22
  * beyond (less one block's rows); a scan of 2^26 waves, B * G * ceil(D / G / 64), or more; D, or B * D of its single-token form, beyond
- * 2^30 - 64; in its backward D * (N + 2) beyond 2^26 - 16 and B * L * G * N beyond 2^32 - 256. */
+ * 2^30 - 64; in its backward D * (N + 2) beyond 2^26 - 16 and B * L * G * N beyond 2^32 - 256; a convolution's B * D beyond 2^31, in its
+ * backward D * (K + 1) beyond 2^26 - 16; L beyond 2^31 - 256. */
 #define URNN_F32 0
 #define URNN_BF16 1
 #define URNN_F16 2

@@ -137,6 +137,18 @@ def test_scan_limits_are_those_of_its_launches():
         assert token(*outside) == -1 and b"one launch" in L.urnn_last_error(), outside
 
 
+def test_lengths_that_a_rounding_up_would_overflow_are_refused():
+    """Tokens are counted in int and rounded up to whole chunks: close to 2^31 of them the sum would be negative.  Sizes that pass go on to
+    the NULL check (-2)."""
+    from urnn_amd._lib import lib
+    L = lib()
+    for n, code in (((1 << 31) - 256, -2), ((1 << 31) - 255, -1), ((1 << 31) - 1, -1)):
+        assert L.urnn_causal_conv(16, 1, 1, 16, 0, 0, 0, 0, 0, 1, 1, n, 1, 4, 1, 0) == code
+        assert L.urnn_causal_conv_backward(16, 1, 1, 16, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 0, 0, 0, 1, 1, n, 1, 4, 1, 0, 0) == code
+        assert L.urnn_selective_scan(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 1, n, 1, 1, 4, 1, 0) == code
+        assert L.urnn_selective_scan_backward(*[0] * 13, 0, *[0] * 10, 0, 1, 1, n, 1, 1, 4, 1, 0, 0) == code
+
+
 @gpu
 def test_scan_of_four_million_short_sequences():
     """As many waves as sequences: the results are those of the batch's parts, bit for bit."""

@@ -1539,13 +1539,16 @@ static inline bool wide_rows(const void *base, long s1, long s2, int elem)
 // A launch has fewer than 2^32 threads: the sum over the parts takes 64 for a value.
 static const double SUM_VALUES = 67108848.0;
 
+// Tokens are counted in int and rounded up to whole chunks, of up to 64 tokens where the sum is an int.
+static const long SEQ_TOKENS = 2147483392;
+
 static int conv_seq_args(const char *what, const void *x, const void *weight, int dtype, long B, long L, long D, int K)
 {
     if (!x || !weight) return fail(URNN_ENULL, "%s: NULL argument", what);
     if (!seq_type(dtype)) return fail(URNN_EINVAL, "%s: dtype=%d", what, dtype);
     if (B < 1 || L < 1 || D < 1) return fail(URNN_EINVAL, "%s: B=%ld L=%ld D=%ld", what, B, L, D);
     if (K < 2 || K > URNN_SEQ_MAX_TAPS) return fail(URNN_EINVAL, "%s: K=%d taps (2..%d)", what, K, URNN_SEQ_MAX_TAPS);
-    if ((double)B * D > 2147483648.0) return fail(URNN_EINVAL, "%s: B * D = %ld * %ld is beyond one launch", what, B, D);
+    if ((double)B * D > 2147483648.0 || L > SEQ_TOKENS) return fail(URNN_EINVAL, "%s: B=%ld L=%ld D=%ld is beyond one launch", what, B, L, D);
     return URNN_OK;
 }
 
@@ -1621,7 +1624,8 @@ static int scan_args(const char *what, int dtype, long B, long L, long D, long G
     if (G < 1 || D % G) return fail(URNN_EINVAL, "%s: G=%ld groups do not divide D=%ld channels", what, G, D);
     if (N < 1 || N > URNN_SEQ_MAX_STATES) return fail(URNN_EINVAL, "%s: N=%ld states (1..%d)", what, N, URNN_SEQ_MAX_STATES);
     const long cbs = G * ((D / G + URNN_SCAN_CB - 1) / URNN_SCAN_CB);
-    if ((token ? (double)B * D > 1073741760.0 : (double)B * cbs >= 67108864.0) || D > 1073741760) return fail(URNN_EINVAL, "%s: B=%ld x D=%ld is beyond one launch", what, B, D);
+    if ((token ? (double)B * D > 1073741760.0 : (double)B * cbs >= 67108864.0) || D > 1073741760 || L > SEQ_TOKENS)
+        return fail(URNN_EINVAL, "%s: B=%ld L=%ld D=%ld is beyond one launch", what, B, L, D);
     return URNN_OK;
 }
 
